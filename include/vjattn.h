@@ -71,6 +71,13 @@ enum {
   VJ_KV_QSCALE_MUL_RSQRT_D = 16
 };
 
+/* Element types of the quantised KV cache (vj_kv_store_quantized and the
+ * calls that read what it writes). */
+enum {
+  VJ_CACHE_E4M3 = 1, /* fp8: 4 exponent bits, 3 mantissa bits, largest value 448 */
+  VJ_CACHE_INT8 = 2  /* integers -127..127 */
+};
+
 /* Message of the last failed call on this host thread ("" if none). */
 VJ_API const char *vj_get_last_error(void);
 
@@ -456,6 +463,80 @@ VJ_API vj_status vj_allreduce_add_rmsnorm(
     const void *const *bufs, void *const *results, uint32_t *const *peer_flags,
     uint32_t *flags, int32_t rank, int32_t world, const void *residual, const void *weight,
     void *residual_out, void *y, int64_t rows, int32_t hidden, float eps, cudaStream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * Quantised KV cache. No counterpart in the reference, whose kernels name
+ * quantised pages (k_scales_pages, v_scales_pages:
+ * vllm/kernels/decode_paged_attention.py:300-341) that its cache never holds.
+ *
+ * A cached row (one token, one KV head, K or V) is D = 128 elements of 8 bits
+ * and one scale byte; it stands for element * 2^(byte - 127) (E8M0). The scale
+ * is the smallest power of two that brings the row's largest magnitude to at
+ * most 448 (e4m3) or 127 (int8), never below 2^-126; a row of zeros has byte
+ * 127, a row holding an infinity or NaN has byte 255 and zero elements, and
+ * reads as NaN everywhere. A power of two times an element is a bf16 number,
+ * so reading the cache back rounds nothing.
+ *
+ *   elements: (blk,t,h,d) at base + blk*stride_block + t*stride_token +
+ *   h*stride_head + d, strides multiples of 16, base 16-byte aligned
+ *   scales: (blk,h,t) at base + blk*scale_stride_block + h*scale_stride_head
+ *   + t, strides multiples of 16, base 16-byte aligned
+ *   block_size: a multiple of 16
+ * ------------------------------------------------------------------------- */
+
+/* vj_kv_store_qknorm_rope for the quantised cache: per-head RMSNorm
+ * (VJ_KV_NORM) and RoPE (VJ_KV_ROPE, interleaved pairs, rope_table as there)
+ * of q and k; q_out in bf16, k and v into their slots. All arithmetic of a row
+ * is done in 32 bits (q) or 64 bits (k) and rounded once at the end, so a
+ * cached row is the correctly rounded one (q of vj_kv_store_qknorm_rope is
+ * rounded to bf16 after every step as the reference does, so the two differ by
+ * roundings). Tokens whose slot lies outside [0, num_blocks*block_size) store
+ * nothing (their q is still written). Slots that are stored must differ from
+ * each other within a call. q_out may equal q_in with the same row stride.
+ *   q_out [T,Hq,D] with row stride q_out_row_stride (0: packed); num_q_heads
+ *   may be 0 (q_in, q_out unused). Other flags are rejected. */
+VJ_API vj_status vj_kv_store_quantized(
+    const void *q_in, const void *k_in, const void *v_in, const void *q_norm_w,
+    const void *k_norm_w, const int32_t *positions, const int32_t *slot_mapping, void *q_out,
+    void *k_cache, void *v_cache, void *k_scales, void *v_scales, int32_t cache_dtype,
+    int64_t num_tokens, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+    int64_t num_blocks, int32_t block_size, int64_t stride_block, int64_t stride_token,
+    int64_t stride_head, int64_t scale_stride_block, int64_t scale_stride_head,
+    int64_t q_row_stride, int64_t k_row_stride, int64_t v_row_stride, int64_t q_out_row_stride,
+    const void *rope_table, int32_t rope_table_len, double eps, float rope_theta, int32_t flags,
+    cudaStream_t stream);
+
+/* Read a batch's cache back: k_out/v_out [B, max_len, Hkv, D] bf16, packed, row
+ * t of sequence b = its cached position t for t < min(context_lens[b],
+ * max_len, bt_width*block_size). Rows behind that are zeroed up to max_len
+ * (zero_to = 0), or only up to the next multiple of zero_to (and at least
+ * zero_to) and left as they were from there on. block_tables and context_lens
+ * as in vj_paged_decode. */
+VJ_API vj_status vj_kv_read_quantized(
+    const void *k_cache, const void *v_cache, const void *k_scales, const void *v_scales,
+    int32_t cache_dtype, const int32_t *block_tables, const int32_t *context_lens, void *k_out,
+    void *v_out, int32_t batch, int32_t max_len, int32_t zero_to, int32_t num_kv_heads,
+    int32_t head_dim, int64_t num_blocks, int32_t block_size, int32_t bt_width,
+    int32_t bt_stride, int64_t stride_block, int64_t stride_token, int64_t stride_head,
+    int64_t scale_stride_block, int64_t scale_stride_head, cudaStream_t stream);
+
+/* vj_paged_decode over the quantised cache: q, out [B,Hq,D] bf16, at most 16
+ * query heads per KV head. stride_block must equal block_size*stride_token.
+ * Cached rows past a sequence's context are never used, whatever they hold.
+ *   workspace: vj_paged_decode_quantized_workspace_size(B, Hq, Hkv, D) bytes,
+ *   16-byte aligned, need not be initialised; calls whose kernels may overlap
+ *   need one each
+ *   error_flag: device int32 (may be NULL), set to 1 if a wait timed out */
+VJ_API size_t vj_paged_decode_quantized_workspace_size(int32_t batch, int32_t num_q_heads,
+                                                       int32_t num_kv_heads, int32_t head_dim);
+VJ_API vj_status vj_paged_decode_quantized(
+    const void *q, const void *k_cache, const void *v_cache, const void *k_scales,
+    const void *v_scales, int32_t cache_dtype, const int32_t *block_tables,
+    const int32_t *context_lens, void *out, int32_t batch, int32_t num_q_heads,
+    int32_t num_kv_heads, int32_t head_dim, int64_t num_blocks, int32_t block_size,
+    int32_t bt_width, int32_t bt_stride, int64_t stride_block, int64_t stride_token,
+    int64_t stride_head, int64_t scale_stride_block, int64_t scale_stride_head, float scale,
+    void *workspace, size_t workspace_bytes, int32_t *error_flag, cudaStream_t stream);
 
 #ifdef __cplusplus
 }

@@ -100,6 +100,27 @@ PROTOTYPES: dict[str, tuple] = {
     "vj_ipc_close_handle": (c_int, [c_vp]),
     "vj_allreduce_add_rmsnorm": (c_int, [c_vp, c_vp, c_vp, c_vp, c_i32, c_i32, c_vp, c_vp, c_vp,
                                          c_vp, c_i64, c_i32, ctypes.c_float, c_vp]),
+    "vj_kv_store_quantized": (c_int, [
+        c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp,   # q, k, v, qw, kw, positions, slots, q_out
+        c_vp, c_vp, c_vp, c_vp, c_i32,              # k, v, k_scales, v_scales, cache_dtype
+        c_i64, c_i32, c_i32, c_i32, c_i64, c_i32,   # T, Hq, Hkv, D, nb, bs
+        c_i64, c_i64, c_i64, c_i64, c_i64,          # strides (block, token, head), scale (block, head)
+        c_i64, c_i64, c_i64, c_i64,                 # q/k/v/q_out row strides (0 = packed)
+        c_vp, c_i32, ctypes.c_double, c_f32, c_i32, c_vp]),   # table, len, eps, theta, flags, stream
+    "vj_kv_read_quantized": (c_int, [
+        c_vp, c_vp, c_vp, c_vp, c_i32,              # k, v, k_scales, v_scales, cache_dtype
+        c_vp, c_vp, c_vp, c_vp,                     # bt, lens, k_out, v_out
+        c_i32, c_i32, c_i32, c_i32, c_i32,          # B, max_len, zero_to, Hkv, D
+        c_i64, c_i32, c_i32, c_i32,                 # nb, bs, bt_width, bt_stride
+        c_i64, c_i64, c_i64, c_i64, c_i64, c_vp]),  # strides, scale strides, stream
+    "vj_paged_decode_quantized_workspace_size": (c_sz, [c_i32, c_i32, c_i32, c_i32]),
+    "vj_paged_decode_quantized": (c_int, [
+        c_vp, c_vp, c_vp, c_vp, c_vp, c_i32,        # q, k, v, k_scales, v_scales, cache_dtype
+        c_vp, c_vp, c_vp,                           # bt, lens, out
+        c_i32, c_i32, c_i32, c_i32, c_i64, c_i32,   # B, Hq, Hkv, D, nb, bs
+        c_i32, c_i32,                               # bt_width, bt_stride
+        c_i64, c_i64, c_i64, c_i64, c_i64,          # strides, scale strides
+        c_f32, c_vp, c_sz, c_vp, c_vp]),            # scale, ws, ws_bytes, err, stream
     "vj_sample": (c_int, [c_vp, c_i64, c_i32, c_i32, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp,
                           c_i32, c_vp, c_vp, c_vp]),
 }
@@ -108,6 +129,7 @@ PROTOTYPES: dict[str, tuple] = {
 VJ_OK, VJ_ERR_INVALID_ARGUMENT, VJ_ERR_UNSUPPORTED, VJ_ERR_WORKSPACE, VJ_ERR_CUDA = range(5)
 VJ_KV_NORM, VJ_KV_ROPE, VJ_KV_WRAP_NEGATIVE = 1, 2, 4
 VJ_KV_QSCALE_DIV_SQRT_D, VJ_KV_QSCALE_MUL_RSQRT_D = 8, 16
+VJ_CACHE_E4M3, VJ_CACHE_INT8 = 1, 2
 VJ_META_PREFILL, VJ_META_DECODE, VJ_META_RANGES = 0, 1, 2
 VJ_META_LAST_BLOCK_SLOT = 1
 VJ_GEMM_PLAIN, VJ_GEMM_SWIGLU = 0, 1

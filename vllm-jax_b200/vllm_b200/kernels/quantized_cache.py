@@ -1,0 +1,320 @@
+"""The quantised KV cache and the operators on it, torch-facing.
+
+A cached row (one token, one KV head, K or V) is head_dim 8-bit elements, e4m3
+or int8, and one power-of-two scale, so a cache takes 129 bytes a row instead
+of 256. The calls mirror the bf16 ones:
+
+  kv_store_quantized        kv_store_qknorm_rope with k and v rounded to 8 bits
+  paged_decode_quantized    paged_decode
+  paged_prefill_quantized   paged_prefill
+  read_kv_cache             a batch's K and V back as bf16
+
+vllm-jax names quantised pages in its attention signatures (k_scales_pages,
+v_scales_pages, vllm/kernels/decode_paged_attention.py:300-341) but has no
+cache that holds them; the format here (vj_kv_store_quantized in
+include/vjattn.h) has no counterpart there.
+"""
+from __future__ import annotations
+
+import contextlib
+import math
+from dataclasses import dataclass
+
+import torch
+
+from .. import _native
+from ._util import ptr, require_cuda, require_dtype, stream_ptr
+from .kv_store import rope_table
+from .prefill_paged_attention import _err_flag, paged_prefill
+
+CACHE_DTYPES = {"e4m3": torch.float8_e4m3fn, "int8": torch.int8}
+_CODES = {torch.float8_e4m3fn: _native.VJ_CACHE_E4M3, torch.int8: _native.VJ_CACHE_INT8}
+
+
+@dataclass(frozen=True)
+class QuantizedKVCache:
+    """A layer's pool: `data` (2, num_blocks, block_size, Hkv, head_dim)
+    float8_e4m3fn or int8, and `scales` (2, num_blocks, Hkv, block_size) uint8,
+    the E8M0 byte of each row: a row stands for data * 2^(scales - 127). Any
+    strides that are multiples of 16 do, as long as data's last dim and scales'
+    last dim are contiguous and a block's tokens are evenly strided on to the
+    next block's."""
+    data: torch.Tensor
+    scales: torch.Tensor
+
+    @staticmethod
+    def zeros(num_blocks: int, block_size: int, num_kv_heads: int, head_dim: int = 128,
+              dtype: str = "e4m3", device=None) -> "QuantizedKVCache":
+        """A pool whose every row reads as zeros. dtype: "e4m3" or "int8"."""
+        if dtype not in CACHE_DTYPES:
+            raise ValueError(f"cache dtype must be one of {sorted(CACHE_DTYPES)}; got {dtype!r}")
+        return QuantizedKVCache(
+            torch.zeros((2, num_blocks, block_size, num_kv_heads, head_dim),
+                        dtype=CACHE_DTYPES[dtype], device=device),
+            torch.full((2, num_blocks, num_kv_heads, block_size), 127, dtype=torch.uint8,
+                       device=device))
+
+
+def _pool(cache: QuantizedKVCache):
+    """(pointers, element type, Hkv, D, num_blocks, block_size, strides) of a cache."""
+    data, scales = cache.data, cache.scales
+    if data.dim() != 5 or data.shape[0] != 2:
+        raise ValueError("cache.data must have shape (2, num_blocks, block_size, Hkv, D); "
+                         f"got {tuple(data.shape)}")
+    _, nb, bs, hkv, D = data.shape
+    code = _CODES.get(data.dtype)
+    if code is None:
+        raise ValueError(f"The dtype of `cache.data` must be float8_e4m3fn or int8. Got {data.dtype}")
+    require_dtype(scales, torch.uint8, "cache.scales")
+    if scales.shape != (2, nb, hkv, bs):
+        raise ValueError(f"cache.scales must have shape (2, num_blocks, Hkv, block_size) = "
+                         f"{(2, nb, hkv, bs)}; got {tuple(scales.shape)}")
+    s2, sb, st, sh, s1 = data.stride()
+    c2, cb, ch, c1 = scales.stride()
+    if s1 != 1 or c1 != 1:
+        raise ValueError("cache.data's head_dim and cache.scales' block_size must be contiguous")
+    d, s = data.data_ptr(), scales.data_ptr()
+    return (d, d + s2, s, s + c2), code, hkv, D, nb, bs, (sb, st, sh, cb, ch)
+
+
+def _device(dev: torch.device):
+    """The C entries launch on the current device: make it the tensors'."""
+    if dev.index is None or dev.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(dev)
+
+
+def _rows(t: torch.Tensor, name: str, T: int, D: int) -> None:
+    require_dtype(t, torch.bfloat16, name)
+    if t.dim() != 3 or t.shape[0] != T or t.shape[2] != D or t.stride(2) != 1 \
+            or (t.shape[1] > 1 and t.stride(1) != D):
+        raise ValueError(f"`{name}` must be a [num_tokens, H, head_dim] tensor with packed heads")
+
+
+def _indices(t: torch.Tensor, name: str, T: int) -> None:
+    require_dtype(t, torch.int32, name)
+    if t.shape != (T,) or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous [{T}] tensor; got shape {tuple(t.shape)}")
+
+
+def kv_store_quantized(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor,
+                       cache: QuantizedKVCache, slot_mapping: torch.Tensor,
+                       positions: torch.Tensor | None = None,
+                       q_norm_weight: torch.Tensor | None = None,
+                       k_norm_weight: torch.Tensor | None = None, *, eps: float = 1e-6,
+                       rope_theta: float = 1e6, norm: bool = True, rope: bool = True,
+                       q_out: torch.Tensor | None = None,
+                       table: torch.Tensor | None = None) -> torch.Tensor | None:
+    """One launch: q_out = rope(norm(q)), cache[slot] = 8 bits of (rope(norm(k)), v).
+
+    The arguments are kv_store_qknorm_rope's. q is rounded to bf16 once, k and
+    v to 8 bits once (kv_store_qknorm_rope rounds after every step, as the
+    reference does). Slots outside the pool store nothing (there is no wrap of
+    negative ones); the others must differ from each other within a call."""
+    dev = require_cuda(k, v, cache.data, cache.scales, slot_mapping, q, positions, q_norm_weight,
+                       k_norm_weight, q_out, table)
+    ptrs, code, Hkv, D, nb, bs, strides = _pool(cache)
+    T = k.shape[0]
+    if v.shape != k.shape:
+        raise ValueError(f"k and v must have the same shape. Got {tuple(k.shape)} and {tuple(v.shape)}")
+    _rows(k, "k", T, D)
+    _rows(v, "v", T, D)
+    if k.shape[1] != Hkv:
+        raise ValueError("cache heads/head_dim do not match k")
+    _indices(slot_mapping, "slot_mapping", T)
+    Hq = 0
+    if q is not None:
+        _rows(q, "q", T, D)
+        Hq = q.shape[1]
+        if q_out is None:
+            q_out = torch.empty((T, Hq, D), dtype=q.dtype, device=dev)
+        else:
+            _rows(q_out, "q_out", T, D)
+            if q_out.shape != q.shape:
+                raise ValueError("q_out must have q's shape")
+    elif q_out is not None:
+        raise ValueError("q_out needs q")
+    flags = 0
+    if norm:
+        flags |= _native.VJ_KV_NORM
+        if k_norm_weight is None or (q is not None and q_norm_weight is None):
+            raise ValueError("norm=True needs q_norm_weight and k_norm_weight")
+        for name, w in (("k_norm_weight", k_norm_weight), ("q_norm_weight", q_norm_weight)):
+            if w is not None:
+                require_dtype(w, torch.bfloat16, name)
+                if w.shape != (D,) or not w.is_contiguous():
+                    raise ValueError(f"{name} must be a contiguous [head_dim] tensor")
+    tab_len = 0
+    if rope:
+        flags |= _native.VJ_KV_ROPE
+        if positions is None:
+            raise ValueError("rope=True needs positions")
+        _indices(positions, "positions", T)
+        if table is None:
+            table = rope_table(dev, rope_theta)
+        require_dtype(table, torch.int32, "table")
+        if not table.is_contiguous():
+            raise ValueError("table must be contiguous")
+        tab_len = table.numel() // 64
+    with _device(dev):
+        _native.call("vj_kv_store_quantized", ptr(q), k.data_ptr(), v.data_ptr(),
+                     ptr(q_norm_weight if norm else None), ptr(k_norm_weight if norm else None),
+                     ptr(positions if rope else None), slot_mapping.data_ptr(), ptr(q_out), *ptrs,
+                     code, T, Hq, Hkv, D, nb, bs, *strides, q.stride(0) if q is not None else 0,
+                     k.stride(0), v.stride(0), q_out.stride(0) if q is not None else 0,
+                     ptr(table) if tab_len else None, tab_len, float(eps), float(rope_theta),
+                     flags, stream_ptr(dev))
+    return q_out
+
+
+def _tables(block_tables: torch.Tensor, context_lens: torch.Tensor, B: int) -> None:
+    require_dtype(block_tables, torch.int32, "block_tables")
+    if block_tables.dim() != 2 or block_tables.shape[0] != B:
+        raise ValueError("`block_tables` must have one row per sequence")
+    if block_tables.shape[1] > 1 and block_tables.stride(1) != 1:
+        raise ValueError("block_tables rows must be contiguous")
+    if B > 1 and block_tables.stride(0) < block_tables.shape[1]:
+        raise ValueError("block_tables rows must not overlap")
+    _indices(context_lens, "context_lens", B)
+
+
+def _table_stride(block_tables: torch.Tensor) -> int:
+    return max(block_tables.stride(0), block_tables.shape[1])
+
+
+def paged_decode_quantized(q: torch.Tensor, cache: QuantizedKVCache, block_tables: torch.Tensor,
+                           context_lens: torch.Tensor, scale: float | None = None,
+                           out: torch.Tensor | None = None,
+                           workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """paged_decode over a quantised cache: q [B, Hq, D] bf16, at most 16 query
+    heads per KV head; rows with no context come out 0. Cached rows past a
+    sequence's context are not used, whatever they hold. `workspace` (uint8,
+    decode_quantized_workspace_bytes(...) long): the split's scratch; by
+    default a fresh allocation of the call's own."""
+    dev = require_cuda(q, cache.data, cache.scales, block_tables, context_lens, out, workspace)
+    ptrs, code, Hkv, D, nb, bs, strides = _pool(cache)
+    require_dtype(q, torch.bfloat16, "q")
+    if q.dim() != 3 or not q.is_contiguous():
+        raise ValueError("q must be a contiguous [batch, Hq, head_dim] tensor")
+    B, Hq, Dq = q.shape
+    if Dq != D or Hq % Hkv:
+        raise ValueError("q heads/head_dim do not match the cache")
+    _tables(block_tables, context_lens, B)
+    if out is None:
+        out = torch.empty_like(q)
+    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
+        raise ValueError("out must be a contiguous bf16 tensor of q's shape")
+    if scale is None:
+        scale = 1.0 / math.sqrt(D)
+    with _device(dev):
+        need = decode_quantized_workspace_bytes(B, Hq, Hkv, D)
+        if workspace is None:
+            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+        elif workspace.dtype != torch.uint8 or workspace.numel() < need \
+                or not workspace.is_contiguous():
+            raise ValueError(f"decode workspace must be contiguous uint8 with >= {need} bytes")
+        _native.call("vj_paged_decode_quantized", q.data_ptr(), *ptrs, code,
+                     block_tables.data_ptr(), context_lens.data_ptr(), out.data_ptr(), B, Hq, Hkv,
+                     D, nb, bs, block_tables.shape[1], _table_stride(block_tables), *strides,
+                     float(scale), workspace.data_ptr(), workspace.numel(),
+                     _err_flag(dev).data_ptr(), stream_ptr(dev))
+    return out
+
+
+def decode_quantized_workspace_bytes(batch: int, num_q_heads: int, num_kv_heads: int,
+                                     head_dim: int = 128) -> int:
+    """Scratch of one paged_decode_quantized call on the current device."""
+    return int(_native.load().vj_paged_decode_quantized_workspace_size(
+        batch, num_q_heads, num_kv_heads, head_dim))
+
+
+def _read(cache, pool, block_tables, context_lens, out, B, max_len, zero_to, dev):
+    ptrs, code, Hkv, D, nb, bs, strides = pool
+    _native.call("vj_kv_read_quantized", *ptrs, code, block_tables.data_ptr(),
+                 context_lens.data_ptr(), out[0].data_ptr(), out[1].data_ptr(), B, max_len,
+                 zero_to, Hkv, D, nb, bs, block_tables.shape[1], _table_stride(block_tables),
+                 *strides, stream_ptr(dev))
+
+
+def read_kv_cache(cache: QuantizedKVCache, block_tables: torch.Tensor,
+                  context_lens: torch.Tensor, max_context_len: int = 0,
+                  out: torch.Tensor | None = None) -> torch.Tensor:
+    """The K and V of a batch as bf16, (2, B, max_context_len, Hkv, D): row t of
+    sequence b is its cached position t, exactly (a scale is a power of two),
+    and zeros from context_lens[b] on. max_context_len: rows per sequence
+    (default: what a block table row holds); longer contexts are cut there."""
+    dev = require_cuda(cache.data, cache.scales, block_tables, context_lens, out)
+    pool = _pool(cache)
+    _, _, Hkv, D, _, bs, _ = pool
+    B = block_tables.shape[0]
+    _tables(block_tables, context_lens, B)
+    if max_context_len < 0:
+        raise ValueError("max_context_len must not be negative")
+    L = int(max_context_len) or block_tables.shape[1] * bs
+    shape = (2, B, L, Hkv, D)
+    if out is None:
+        out = torch.empty(shape, dtype=torch.bfloat16, device=dev)
+    elif out.shape != shape or out.dtype != torch.bfloat16 or not out.is_contiguous():
+        raise ValueError(f"out must be a contiguous bf16 tensor of shape {shape}")
+    with _device(dev):
+        _read(cache, pool, block_tables, context_lens, out, B, L, 0, dev)
+    return out
+
+
+# bf16 rows (token x KV head) of one read-back inside paged_prefill_quantized:
+# 1 GiB of K and V. Batches that need more run in groups of sequences.
+PREFILL_SCRATCH_ROWS = 1 << 21
+_KEY_TILE = 128      # keys a prefill tile reads at once
+
+
+def paged_prefill_quantized(q: torch.Tensor, cache: QuantizedKVCache, block_tables: torch.Tensor,
+                            cu_seqlens_q: torch.Tensor, context_lens: torch.Tensor | None = None,
+                            max_seqlen_q: int = 0, scale: float | None = None,
+                            out: torch.Tensor | None = None,
+                            max_context_len: int = 0) -> torch.Tensor:
+    """paged_prefill over a quantised cache: causal attention of the new tokens
+    (rows [cu_seqlens_q[s], cu_seqlens_q[s+1]) of q) of each sequence over its
+    cached context, theirs included. The contexts are read back to bf16, which
+    is exact, and attended to from there: a prompt's attention does far more
+    work per key than reading it back, and the conversion is done once instead
+    of once per query tile. max_context_len: a bound on context_lens (default:
+    what a block table row holds); it sizes the scratch, as max_seqlen_q sizes
+    the grid."""
+    dev = require_cuda(q, cache.data, cache.scales, block_tables, cu_seqlens_q, context_lens, out)
+    pool = _pool(cache)
+    _, _, Hkv, D, _, bs, _ = pool
+    require_dtype(q, torch.bfloat16, "q")
+    require_dtype(cu_seqlens_q, torch.int32, "cu_seqlens_q")
+    if q.dim() != 3 or not q.is_contiguous():
+        raise ValueError("q must be a contiguous [num_tokens, Hq, head_dim] tensor")
+    if cu_seqlens_q.dim() != 1 or cu_seqlens_q.shape[0] < 1 or not cu_seqlens_q.is_contiguous():
+        raise ValueError("cu_seqlens_q must be a contiguous [num_seqs + 1] tensor")
+    if q.shape[2] != D or q.shape[1] % Hkv:
+        raise ValueError("q heads/head_dim do not match the cache")
+    S = cu_seqlens_q.shape[0] - 1
+    if context_lens is None:
+        context_lens = cu_seqlens_q[1:] - cu_seqlens_q[:-1]
+    _tables(block_tables, context_lens, S)
+    if max_context_len < 0:
+        raise ValueError("max_context_len must not be negative")
+    capacity = block_tables.shape[1] * bs
+    L = min(int(max_context_len) or capacity, capacity)
+    L = max(-(-L // 16) * 16, 16)
+    if out is None:
+        out = torch.empty_like(q)
+    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
+        raise ValueError("out must be a contiguous bf16 tensor of q's shape")
+    group = max(1, min(S, PREFILL_SCRATCH_ROWS // (L * Hkv)))
+    with _device(dev):
+        # page p of the group's sequence b is row block b * L/16 + p of the scratch
+        pages = torch.arange(group * (L // 16), dtype=torch.int32, device=dev).view(group, -1)
+        scratch = torch.empty((2, group, L, Hkv, D), dtype=torch.bfloat16, device=dev)
+        kv = scratch.view(2, group * (L // 16), 16, Hkv, D)
+        for s in range(0, max(S, 1), group):
+            n = min(group, S - s)
+            if n > 0:
+                _read(cache, pool, block_tables[s:s + n], context_lens[s:s + n], scratch, n, L,
+                      _KEY_TILE, dev)
+            paged_prefill(q, kv, pages[:n], cu_seqlens_q[s:s + n + 1], context_lens[s:s + n],
+                          max_seqlen_q, scale, out)
+    return out
