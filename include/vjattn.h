@@ -472,8 +472,8 @@ VJ_API vj_status vj_allreduce_add_rmsnorm(
  * A cached row (one token, one KV head, K or V) is D = 128 elements of 8 bits
  * and one scale byte; it stands for element * 2^(byte - 127) (E8M0). The scale
  * is the smallest power of two that brings the row's largest magnitude to at
- * most 448 (e4m3) or 127 (int8), never below 2^-126; a row of zeros has byte
- * 127, a row holding an infinity or NaN has byte 255 and zero elements, and
+ * most 448 (e4m3) or 127 (int8), never below 2^-126 (a row of zeros has that
+ * one); a row holding an infinity or NaN has byte 255 and zero elements, and
  * reads as NaN everywhere. A power of two times an element is a bf16 number,
  * so reading the cache back rounds nothing.
  *

@@ -30,7 +30,6 @@ def quantise_rows(x: np.ndarray, dtype: str) -> tuple[np.ndarray, np.ndarray]:
     e = np.full(amax.shape, -126)
     for step in (128, 64, 32, 16, 8, 4, 2, 1):
         e = np.where(amax > LARGEST[dtype] * np.exp2(e + step - 1.0), e + step, e)
-    e = np.where(amax > 0, e, 0)
     y = x * np.exp2(-e.astype(np.float64))[..., None]
     mids = (pos[1:] + pos[:-1]) / 2
     lo, hi = np.searchsorted(mids, np.abs(y), "left"), np.searchsorted(mids, np.abs(y), "right")

@@ -25,7 +25,7 @@ def test_quantise_rows_properties(dtype):
     x[4] = 0
     x[4, 0] = np.nextafter(oq.LARGEST[dtype], 1e9)
     codes, b = oq.quantise_rows(x, dtype)
-    assert b[0] == 127 and b[1] == b[2] == 255 and b[3] == 127 and b[4] == 128
+    assert b[0] == 1 and b[1] == b[2] == 255 and b[3] == 127 and b[4] == 128
     assert not codes[:3].any()
     y = oq.element_values(codes, dtype) * np.exp2(b.astype(float) - 127)[:, None]
     ok = np.isfinite(x).all(-1)

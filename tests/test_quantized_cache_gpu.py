@@ -299,13 +299,14 @@ def test_decode_large_and_small_queries():
 
 
 def test_decode_zero_value_rows_keep_their_weight():
-    """A zero row of V has scale 1 while its neighbours' scales are tiny."""
+    """A zero row of V counts in the softmax's sum, whatever its neighbours' scales."""
     from vllm_b200.kernels.quantized_cache import paged_decode_quantized
     for tiny in (120, 60, 2):
         codes = np.zeros((2, 2, 16, 1, D), np.uint8)
         codes[1] = 1                                    # int8 ones
         scales = np.full((2, 2, 1, 16), tiny, np.uint8)
-        codes[1, 0, 3], scales[1, 0, 0, 3] = 0, 127     # one zero row, byte 127
+        zero, byte = oq.quantise_rows(np.zeros(D), "int8")
+        codes[1, 0, 3], scales[1, 0, 0, 3] = zero, byte
         out = paged_decode_quantized(_t(np.ones((1, 4, D))), _cache(codes, scales, "int8"),
                                      _i([[0, 1]]), _i([20]))
         ref = 19 / 20 * 2.0 ** (tiny - 127)

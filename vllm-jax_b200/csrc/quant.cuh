@@ -32,13 +32,16 @@ struct Pool {
   int block_size;
 };
 
-// 2^(b - 127); byte 0 is 2^-127 (a subnormal), byte 255 comes out as infinity,
-// which times a row's zero elements is the NaN that byte stands for.
-VJ_DEV float scale_of(uint32_t b) { return __uint_as_float(b == 0u ? 0x00400000u : b << 23); }
+// 2^(b - 127); byte 0 is 2^-127 (a subnormal), byte 255 NaN.
+VJ_DEV float scale_of(uint32_t b) {
+  return __uint_as_float(b == 0u ? 0x00400000u : b == 255u ? 0x7fffffffu : b << 23);
+}
 
 // Scale exponent of a row from the bit pattern of its largest magnitude: the
 // smallest e with amax <= 448 * 2^e (448 = 1.75 * 2^8) or 127 * 2^e
-// (127 = 1.984375 * 2^6), at least -126. amax is finite and not 0.
+// (127 = 1.984375 * 2^6), at least -126 (and so for a row of zeros, whose
+// scale must not tower over its neighbours': the decode kernel weighs rows by
+// their scales). amax is finite.
 template <bool kInt8>
 VJ_DEV int scale_exponent(uint32_t amax_bits) {
   const int x = static_cast<int>(amax_bits >> 23) - 127;   // subnormals: far below the clamp

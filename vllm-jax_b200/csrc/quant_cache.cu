@@ -153,7 +153,7 @@ __global__ void __launch_bounds__(kStoreThreads) kv_store_quantized_kernel(const
     for (int j = 0; j < 16; ++j) amax = max(amax, __float_as_uint(y[j]) & 0x7fffffffu);
     amax = group_max(mask, amax);
     const bool bad = amax >= 0x7f800000u;              // an infinity or NaN in the row
-    const int e = amax == 0u || bad ? 0 : scale_exponent<kInt8>(amax);
+    const int e = bad ? 0 : scale_exponent<kInt8>(amax);
     const float f = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);   // 2^-e
     uint32_t o[4];
 #pragma unroll

@@ -30,10 +30,10 @@ int check_launch(const char *what) {
 static PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
 static std::once_flag g_encode_once;
 
-int encode_tmap_3d(CUtensorMap *map, const void *base, uint64_t dim0,
-                   uint64_t dim1, uint64_t dim2, uint64_t stride1_bytes,
-                   uint64_t stride2_bytes, uint32_t box0, uint32_t box1,
-                   uint32_t box2, bool swizzle128) {
+static int encode_3d(CUtensorMap *map, CUtensorMapDataType type, const void *base, uint64_t dim0,
+                     uint64_t dim1, uint64_t dim2, uint64_t stride1_bytes,
+                     uint64_t stride2_bytes, uint32_t box0, uint32_t box1, uint32_t box2,
+                     bool swizzle128) {
   std::call_once(g_encode_once, []() {
     void *fn = nullptr;
     cudaDriverEntryPointQueryResult q;
@@ -50,7 +50,7 @@ int encode_tmap_3d(CUtensorMap *map, const void *base, uint64_t dim0,
   cuuint64_t strides[2] = {stride1_bytes, stride2_bytes};
   cuuint32_t box[3] = {box0, box1, box2};
   cuuint32_t estr[3] = {1, 1, 1};
-  CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+  CUresult r = g_encode(map, type, 3,
                         const_cast<void *>(base), dims, strides, box, estr,
                         CU_TENSOR_MAP_INTERLEAVE_NONE,
                         swizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B
@@ -63,6 +63,22 @@ int encode_tmap_3d(CUtensorMap *map, const void *base, uint64_t dim0,
                          "): base/strides must be 16-byte aligned");
   }
   return VJ_OK;
+}
+
+int encode_tmap_3d(CUtensorMap *map, const void *base, uint64_t dim0,
+                   uint64_t dim1, uint64_t dim2, uint64_t stride1_bytes,
+                   uint64_t stride2_bytes, uint32_t box0, uint32_t box1,
+                   uint32_t box2, bool swizzle128) {
+  return encode_3d(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, base, dim0, dim1, dim2, stride1_bytes,
+                   stride2_bytes, box0, box1, box2, swizzle128);
+}
+
+int encode_tmap_3d_u8(CUtensorMap *map, const void *base, uint64_t dim0,
+                      uint64_t dim1, uint64_t dim2, uint64_t stride1_bytes,
+                      uint64_t stride2_bytes, uint32_t box0, uint32_t box1,
+                      uint32_t box2, bool swizzle128) {
+  return encode_3d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, dim0, dim1, dim2, stride1_bytes,
+                   stride2_bytes, box0, box1, box2, swizzle128);
 }
 
 int num_sms() {

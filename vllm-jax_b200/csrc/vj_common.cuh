@@ -24,6 +24,11 @@ int encode_tmap_3d(CUtensorMap *map, const void *base, uint64_t dim0,
                    uint64_t dim1, uint64_t dim2, uint64_t stride1_bytes,
                    uint64_t stride2_bytes, uint32_t box0, uint32_t box1,
                    uint32_t box2, bool swizzle128);
+// The same for 8-bit elements.
+int encode_tmap_3d_u8(CUtensorMap *map, const void *base, uint64_t dim0,
+                      uint64_t dim1, uint64_t dim2, uint64_t stride1_bytes,
+                      uint64_t stride2_bytes, uint32_t box0, uint32_t box1,
+                      uint32_t box2, bool swizzle128);
 int num_sms();
 
 // ----------------------------------------------------------------------------
