@@ -523,12 +523,13 @@ VJ_API vj_status vj_kv_read_quantized(
 /* vj_paged_decode over the quantised cache: q, out [B,Hq,D] bf16, at most 16
  * query heads per KV head. stride_block must equal block_size*stride_token.
  * Cached rows past a sequence's context are never used, whatever they hold.
- *   workspace: vj_paged_decode_quantized_workspace_size(B, Hq, Hkv, D) bytes,
- *   16-byte aligned, need not be initialised; calls whose kernels may overlap
+ *   workspace: vj_paged_decode_quantized_workspace_size(B, Hq, Hkv, D, bt_width,
+ *   block_size) bytes on the current device, 16-byte aligned, need not be initialised; calls whose kernels may overlap
  *   need one each
  *   error_flag: device int32 (may be NULL), set to 1 if a wait timed out */
 VJ_API size_t vj_paged_decode_quantized_workspace_size(int32_t batch, int32_t num_q_heads,
-                                                       int32_t num_kv_heads, int32_t head_dim);
+                                                       int32_t num_kv_heads, int32_t head_dim,
+                                                       int32_t bt_width, int32_t block_size);
 VJ_API vj_status vj_paged_decode_quantized(
     const void *q, const void *k_cache, const void *v_cache, const void *k_scales,
     const void *v_scales, int32_t cache_dtype, const int32_t *block_tables,

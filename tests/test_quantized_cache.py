@@ -154,8 +154,9 @@ def test_empty_calls_need_no_memory():
     assert _store(lib, T=0, **none) == 0
     assert _decode(lib, B=0, **none) == 0
     assert _read(lib, B=0, **none) == 0
-    assert lib.vj_paged_decode_quantized_workspace_size(4, 8, 2, 64) == 0
-    assert lib.vj_paged_decode_quantized_workspace_size(4, 8, 2, 128) >= 16
+    size = lib.vj_paged_decode_quantized_workspace_size
+    assert size(4, 8, 2, 64, 4, 16) == size(4, 8, 2, 128, 4, 0) == size(4, 0, 2, 128, 4, 16) == 0
+    assert 16 <= size(4, 8, 2, 128, 4, 16) <= size(400, 8, 2, 128, 4000, 16)
 
 
 def test_wrapper_refuses_cpu_tensors_and_unknown_types():

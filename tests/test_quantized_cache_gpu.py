@@ -280,6 +280,54 @@ def test_decode_batch_larger_than_a_block_of_threads():
     _decode_case(2500, 2, 1, 16, lens, "int8", 10)
 
 
+@pytest.mark.parametrize("Hq,Hkv,dtype", [(74, 37, "e4m3"), (8 * 37, 37, "int8"),
+                                          (370, 37, "e4m3"), (64, 64, "int8")])
+def test_decode_of_so_many_pages_that_a_part_is_dealt(Hq, Hkv, dtype):
+    """Enough work (32 pages a warp and KV head) that a fifth of it is dealt in pieces:
+    against 64 bits, the same bits every time, and on two streams at once."""
+    from vllm_b200.kernels.quantized_cache import QuantizedKVCache, paged_decode_quantized
+    lens = [9001, 17, 0, 1, 12000, 3, 333, 300, 16, 11000, 8000, 700, 90, 32]
+    bs, B = 32, len(lens)
+    gen = torch.Generator(device="cuda").manual_seed(Hq)
+    need = [-(-n // bs) for n in lens]
+    nb, width = sum(need) + 1, max(need)
+    x = torch.randn((2, nb, bs, Hkv, D), generator=gen, device="cuda")
+    data = ((x * 100).clamp(-448, 448).to(torch.float8_e4m3fn) if dtype == "e4m3"
+            else (x * 36).round().clamp(-127, 127).to(torch.int8))
+    scales = torch.randint(119, 122, (2, nb, Hkv, bs), generator=gen, device="cuda",
+                           dtype=torch.uint8)
+    del x
+    perm = torch.randperm(nb, generator=gen, device="cuda").to(torch.int32)
+    bt = torch.full((B, width), -1, dtype=torch.int32, device="cuda")
+    at = 0
+    for b, n in enumerate(need):
+        bt[b, :n] = perm[at:at + n]
+        at += n
+    q = torch.randn((B, Hq, D), generator=gen, device="cuda", dtype=torch.bfloat16)
+    cache, ln = QuantizedKVCache(data, scales), _i(lens)
+    out = paged_decode_quantized(q, cache, bt, ln)
+    ref, mag = torch.zeros((2, B, Hq, D), dtype=torch.float64, device="cuda")
+    for b, n in enumerate(lens):
+        if n:
+            t = bt[b, :need[b]].long()
+            k, v = (data[i].view(torch.uint8)[t].view(data.dtype).double()
+                    * torch.exp2(scales[i][t].double() - 127).transpose(1, 2)[..., None]
+                    for i in range(2))
+            k, v = (y.flatten(0, 1)[:n].permute(1, 0, 2) for y in (k, v))     # [Hkv, n, D]
+            p = torch.softmax(q[b].double().view(Hkv, -1, D) @ k.transpose(1, 2) / math.sqrt(D), -1)
+            ref[b], mag[b] = (p @ v).view(Hq, D), (p @ v.abs()).view(Hq, D)
+    _check(out, ref.cpu().numpy(), mag.cpu().numpy(), DECODE)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    again = []
+    for _ in range(3):
+        for s in streams:
+            with torch.cuda.stream(s):
+                again.append(paged_decode_quantized(q, cache, bt, ln))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, out) for o in again)
+
+
 def test_decode_context_longer_than_the_table_is_cut():
     _decode_case(2, 8, 2, 16, [400, 37], "e4m3", 11, width=5)
 

@@ -77,9 +77,14 @@ VJ_DEV uint32_t dequant_f16x2(uint32_t w) {
         : "=r"(d)
         : "r"(w ^ 0x80808080u), "r"(0x64646464u), "r"(kHi ? 0x4342u : 0x4140u));
     asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(d), "r"(0x64806480u));   // - 1152
+  } else if constexpr (kHi) {
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, h;\n\t}"
+        : "=r"(d)
+        : "r"(w));
   } else {
-    const uint16_t h = static_cast<uint16_t>(kHi ? w >> 16 : w);
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(d) : "h"(h));
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\t}"
+        : "=r"(d)
+        : "r"(w));
   }
   return d;
 }

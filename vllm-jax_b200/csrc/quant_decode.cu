@@ -6,20 +6,33 @@
 // query heads of its KV head together.
 //
 // The work is cut into pages of 16 tokens. All sequences' pages in a row,
-// numbered 0..T-1, are split evenly over groups of Hkv warps; the warps of a
-// group walk the same pages, each for its own KV head, so a page's rows (which
-// lie side by side) are read at about the same time. Every CTA finds its
-// warps' ranges from the context lengths by itself, so there is no planning
-// launch, no work counter and nothing to reset between calls. A sequence whose
-// pages fall to one group is finished there; otherwise each group leaves a
-// partial result (its output in 32 bits, maximum and sum), at most two per
-// warp, and quant_combine_kernel joins them.
+// numbered 0..T-1, are split evenly over the warps that serve a KV head; the
+// warps of the other heads walk the same pages at the same time, so a page's
+// rows, which lie side by side, are read together. Every CTA finds its warps'
+// ranges from the context lengths by itself: there is no planning launch.
+//   Little work (below kDealt pages a warp): eight warps with neighbouring
+// ranges form a unit and join the sequences they share in shared memory; a
+// sequence that more than one unit shares leaves a partial result in each (its
+// output in 32 bits, maximum and sum).
+//   Much work: SMs do not get equal shares of a saturated memory (even ranges
+// of 157 pages a warp ended between 212 and 281 us), so a warp keeps only the
+// first 4/5 of its range for sure. The rest is three pieces, which a warp takes
+// one by one from its own range, and then from ranges of warps that are behind,
+// by counting up the range's word. A range's warp sets that word to 0 before
+// anything else; one that looks at a word before that takes no piece, or one
+// that will be done twice with the same result, so the words need no launch of
+// their own to be cleared. Pieces depend on the lengths alone and each leaves
+// its own partial results: who does which changes no result.
+//   quant_combine_kernel joins the partial results, at most two of a unit,
+// range or piece, in the order of the pages.
 //
-// A warp streams its pages through a ring of its own in shared memory (TMA
-// boxes of 16 rows x 128 bytes, 128-byte swizzle, and the rows' scale bytes).
-// Products run on mma.sync m16n8k16 in f16 with 32-bit sums, with the tokens,
-// then the dimensions, as the 16 rows and the query heads of the group as the 8
-// columns:
+// A warp streams its pages through a ring of its own in shared memory: TMA
+// boxes of 16 rows x 128 bytes (128-byte swizzle) and the rows' scale bytes.
+// Where a page lies is looked up for 32 pages at once, a page a lane, and that
+// lane issues its copies; so the walk (sequence ends, block tables, addresses)
+// costs a page next to nothing. Products run on mma.sync m16n8k16 in f16 with
+// 32-bit sums, with the tokens, then the dimensions, as the 16 rows and the
+// query heads of the group as the 8 columns:
 //   S^T[tok][head] = K[tok][d] Q^T[d][head]     (8 steps of 16 dims)
 //   O^T[d][head]  += V^T[d][tok] W^T[tok][head]  (8 tiles of 16 dims)
 // The elements of both types are exact in f16. Which 16 dims make a step is
@@ -39,6 +52,7 @@
 #include "quant.cuh"
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 
 namespace vj {
@@ -48,32 +62,82 @@ using namespace qn;
 constexpr int kTok = 16;                      // tokens per page
 constexpr int kHalf = kTok * kD;              // bytes of a page's K (or V) rows
 constexpr int kStage = 2 * kHalf;
-constexpr int kMinPages = 4;                  // pages of a group, at least
+constexpr int kDealt = 32;                    // pages a warp from which on a part is dealt
 constexpr float kSlack = 11.0f;               // log2 of what a score may pass the maximum by
 constexpr float kUp = 4.0f;                   // log2 of the weight at the maximum
 
+// A page: what its lane looked up.
+struct Page {
+  int b;             // sequence
+  int valid_flags;   // tokens inside the context (1..16), and kFirst.. below << 8
+  int tok;           // first token's place in the pool
+  int64_t scale;     // offset of its scale bytes
+};
+// What the consumer of a stage needs to know of it.
+struct Info {
+  int b, valid_flags, h, segment;
+};
+constexpr int kFirst = 1;      // first page of its segment (the part of a sequence in a range)
+constexpr int kLast = 2;       // last page of its segment
+constexpr int kHead = 4;       // the segment starts with the sequence
+constexpr int kTail = 8;       // the segment ends with the sequence
+constexpr int kEnd = 16;       // last page of the range
+
+// What a warp leaves for its unit to join.
+struct Left {
+  int b0;         // sequence of a segment that began before the range, or -1
+  int ends0;      // whether that sequence ends in it
+  int far0;       // whether the record is in the workspace (pages came after it) or the ring
+  int b1;         // sequence of a segment that began in the range and goes on behind it, or -1
+};
+
+// How `total` pages are split: n ranges of neighbouring pages. Where pieces are
+// dealt, a range is cut in kCuts parts.
+constexpr int kCuts = 4;
+struct Split {
+  int total, n, dealt;
+};
+
 template <int NT>
 struct Shape {                                // NT tiles of 8 query heads
+  static constexpr int kUnit = 8;                             // warps that join their results
   static constexpr int kWarps = NT == 1 ? 16 : 8;
   static constexpr int kStages = NT == 1 ? 3 : 6;
-  static constexpr int kThreads = kWarps * 32;
+  static constexpr int kThreads = kWarps * 32;                // a power of two
   static constexpr int kRing = kWarps * kStages;
-  // pages, scale bytes, page infos, barriers, scan
-  static constexpr size_t kSmem =
-      1024 + (size_t)kRing * (kStage + 32 + 16 + 8) + (kThreads + 1 + kWarps) * 4;
+  static constexpr int kUnits = kWarps / kUnit;
+  static constexpr int kHeads = NT * 8;
+  // pages, scale bytes, barriers, left records, scan
+  static constexpr size_t kSmem = 1024 + (size_t)kRing * (kStage + 32 + sizeof(Info) + 8) +
+                                  kWarps * sizeof(Left) + sizeof(Split) + (kThreads + kWarps) * 4;
+  // a record in a warp's ring: kHeads x 128 outputs, kHeads (maximum, sum)
+  static_assert(kHeads * (kD + 2) * 4 <= kStages * kStage, "a record fits the ring");
 };
 
 struct Scratch {
-  int32_t *prefix;    // [B + 1] first page of each sequence
-  float2 *ml;         // [2 * groups][Hq] maximum (log2), sum
-  float *o;           // [2 * groups][Hq][128]
+  int32_t *taken;     // [groups][Hkv] pieces of a range that are taken
+  int2 *segments;     // [B] first unit (or range or piece) of a sequence, and how many hold it
+  float2 *ml;         // [records][Hq] maximum (log2), sum
+  float *o;           // [records][Hq][128]
 };
 
 inline size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
-inline size_t scratch_bytes(int64_t B, int64_t Hq, int64_t groups) {
-  return up256(4 * (B + 1)) + up256(2 * groups * Hq * sizeof(float2)) +
-         2 * groups * Hq * kD * sizeof(float);
+// Records: with units, two of each and one of each warp (a sequence that ends
+// in the middle of a warp's range); else two of each part of each range.
+inline size_t carve(Scratch *s, void *base, size_t B, size_t Hq, size_t Hkv, size_t groups,
+                    size_t unit, bool may_deal) {
+  const size_t records = may_deal ? 2 * kCuts * groups : 2 * (groups / unit) + groups;
+  char *p = static_cast<char *>(base);
+  size_t off = 0;
+  auto take = [&](size_t n) { char *at = p + off; off += up256(n); return at; };
+  Scratch t;
+  t.taken = reinterpret_cast<int32_t *>(take(may_deal ? groups * Hkv * sizeof(int32_t) : 0));
+  t.segments = reinterpret_cast<int2 *>(take(B * sizeof(int2)));
+  t.ml = reinterpret_cast<float2 *>(take(records * Hq * sizeof(float2)));
+  t.o = reinterpret_cast<float *>(take(records * Hq * kD * sizeof(float)));
+  if (s) *s = t;
+  return off;
 }
 
 struct QDecodeArgs {
@@ -83,21 +147,37 @@ struct QDecodeArgs {
   const uint8_t *ks, *vs;
   int64_t ssb, ssh;
   int B, Hq, Hkv, g, bt_stride, pages_per_block, block_size, max_pages, num_blocks, head_major;
-  int groups;         // warps of the grid / Hkv
+  int unit;           // warps of a unit
+  int groups;         // warps that serve a KV head, a multiple of unit
+  int may_deal;       // whether the tables could hold enough to deal pieces
   float scale_log2;
   Scratch ws;
   int32_t *err;
 };
 
-// Groups in use, and the page range of group G: [first(G), first(G + 1)).
-VJ_DEV int groups_of(int total, int groups) {
-  return min(groups, (total + kMinPages - 1) / kMinPages);
+VJ_DEV Split split_pages(int total, int groups, int may_deal) {
+  return {total, min(groups, total), may_deal && total / groups >= kDealt ? 1 : 0};
 }
-VJ_DEV int first_page(int G, int total, int n) {
-  return static_cast<int>(static_cast<int64_t>(G) * total / n);
+// First page of range G.
+VJ_DEV int first_page(int G, const Split &t) {
+  return static_cast<int>(static_cast<int64_t>(G) * t.total / t.n);
 }
-VJ_DEV int group_of(int page, int total, int n) {
-  return static_cast<int>((static_cast<int64_t>(page + 1) * n - 1) / total);
+VJ_DEV int range_of(int page, const Split &t) {
+  return static_cast<int>((static_cast<int64_t>(page + 1) * t.n - 1) / t.total);
+}
+// First page of part i (0..kCuts) of a range of `pages`: 4/5 of it, 3/25, 1/25, 1/25.
+VJ_DEV int part_page(int i, int pages) {
+  const int a = pages * 4 / 5, b = a + (pages - a) * 3 / 5, c = b + (pages - b) / 2;
+  return i == 0 ? 0 : i == 1 ? a : i == 2 ? b : i == 3 ? c : pages;
+}
+VJ_DEV int range_id(int G, int h, int Hkv) { return G * Hkv + h; }
+// The range, or the part of one (kCuts of a range), that holds a page.
+VJ_DEV int segment_of(int page, const Split &t) {
+  const int G = range_of(page, t);
+  if (!t.dealt) return G;
+  const int at = page - first_page(G, t), pages = first_page(G + 1, t) - first_page(G, t);
+  return G * kCuts + (at >= part_page(1, pages)) + (at >= part_page(2, pages)) +
+         (at >= part_page(3, pages));
 }
 
 VJ_DEV int pages_of(int len, int max_pages) {
@@ -112,6 +192,14 @@ VJ_DEV void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32
       "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+VJ_DEV void mma_f16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                          uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
+      "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 VJ_DEV uint32_t transpose8x8(uint32_t x) {
   uint32_t d;
@@ -135,71 +223,68 @@ VJ_DEV uint4 lds128(uint32_t addr) {
                : "r"(addr));
   return v;
 }
-VJ_DEV float max3_over_rows(float v) {        // over the lanes that share lane & 3
+VJ_DEV uint32_t lds8(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(addr));
+  return v;
+}
+VJ_DEV float max_over_rows(float v) {        // over the lanes that share lane & 3
 #pragma unroll
   for (int o = 4; o <= 16; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
 }
 
-// The pages of a warp's range in order. Every lane holds the same state but
-// the two windows: 32 sequences' lengths, and 32 entries of the current
-// sequence's block table.
-struct Walk {
-  int base, len_w;        // window: lane i has sequence base + i
-  int b, p, np;           // current sequence, next page, its pages
-  int left;               // pages left in the range
-  int start;              // first page of the current segment
-  int entry, blk_w;       // table window: lane i has entry + i
+// Sequence and page-in-sequence of page s of all pages; scan[i] = pages before
+// sequence i * per.
+struct Place {
+  int b, p, np, len;
 };
-
-VJ_DEV int walk_len(const QDecodeArgs &a, int base, int lane) {
-  return base + lane < a.B ? __ldg(a.lens + base + lane) : 0;
-}
-VJ_DEV void walk_enter(Walk &w, const QDecodeArgs &a, int b, int p) {
-  w.b = b;
-  w.p = w.start = p;
-  w.np = pages_of(__shfl_sync(0xffffffffu, w.len_w, b - w.base), a.max_pages);
-  w.entry = -64;
-}
-// Next sequence that has pages; there is one while pages are left.
-VJ_DEV void walk_next(Walk &w, const QDecodeArgs &a, int lane) {
-  int from = w.b + 1 - w.base;
-  while (true) {
-    const unsigned have = __ballot_sync(
-        0xffffffffu, lane >= from && pages_of(w.len_w, a.max_pages) > 0);
-    if (have) {
-      walk_enter(w, a, w.base + __ffs(have) - 1, 0);
-      return;
-    }
-    w.base += 32;
-    if (w.base >= a.B) { w.left = 0; return; }
-    w.len_w = walk_len(a, w.base, lane);
-    from = 0;
+template <int kRuns>
+VJ_DEV Place locate(const QDecodeArgs &a, const int *scan, int per, int s) {
+  int lo = 0;                               // last run that starts at or before s
+#pragma unroll
+  for (int step = kRuns / 2; step >= 1; step >>= 1) {
+    if (scan[lo + step] <= s) lo += step;
   }
+  Place w;
+  int cum = scan[lo];
+  for (w.b = lo * per;; ++w.b) {            // s lies in this run
+    w.len = __ldg(a.lens + w.b);
+    w.np = pages_of(w.len, a.max_pages);
+    if (s < cum + w.np || w.b + 1 >= a.B) break;
+    cum += w.np;
+  }
+  w.p = s - cum;
+  return w;
 }
-
-// What a stage holds. flags: 1 first page of its segment, 2 last page of its
-// segment, 4 the segment starts at the sequence's first page, 8 it ends at
-// its last one.
-struct PageInfo {
-  int b, page, len, flags;
-};
 
 template <bool kInt8, int NT>
 __global__ void __launch_bounds__(Shape<NT>::kThreads, 1)
 quant_decode_kernel(const __grid_constant__ CUtensorMap tmk,
                     const __grid_constant__ CUtensorMap tmv, const QDecodeArgs a) {
   using S = Shape<NT>;
+  constexpr int kStages = S::kStages, kUnit = S::kUnit;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                               ~uintptr_t(1023));
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   uint8_t *scales = smem + S::kRing * kStage;
-  PageInfo *infos = reinterpret_cast<PageInfo *>(scales + S::kRing * 32);
-  uint64_t *bars = reinterpret_cast<uint64_t *>(infos + S::kRing);
-  int *scan = reinterpret_cast<int *>(bars + S::kRing);       // [kThreads + 1]
-  int *warp_sum = scan + S::kThreads + 1;                     // [kWarps]
+  Info *infos = reinterpret_cast<Info *>(scales + S::kRing * 32);
+  uint64_t *full = reinterpret_cast<uint64_t *>(infos + S::kRing);
+  Left *lefts = reinterpret_cast<Left *>(full + S::kRing);
+  Split &split = *reinterpret_cast<Split *>(lefts + S::kWarps);
+  int *scan = reinterpret_cast<int *>(&split + 1);            // [kThreads]
+  int *warp_sum = scan + S::kThreads;                         // [kWarps]
 
+  if (lane == 0) {
+    for (int s = 0; s < kStages; ++s) mbar_init(&full[warp * kStages + s], 1);
+    fence_mbar_init();
+    if (warp == 0) { tma_prefetch_desc(&tmk); tma_prefetch_desc(&tmv); }
+  }
+  // nothing of the caller's is read before the kernel ahead is done; the
+  // combine kernel may be made ready as soon as every CTA of this one runs
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;");
   // ---- pages before each run of `per` sequences
   const int per = (a.B + S::kThreads - 1) / S::kThreads;
   int mine = 0;
@@ -214,10 +299,6 @@ quant_decode_kernel(const __grid_constant__ CUtensorMap tmk,
     if (lane >= o) incl += v;
   }
   if (lane == 31) warp_sum[warp] = incl;
-  if (lane == 0) {
-    for (int s = 0; s < S::kStages; ++s) mbar_init(&bars[warp * S::kStages + s], 1);
-    fence_mbar_init();
-  }
   __syncthreads();
   int before = 0, total = 0;
 #pragma unroll
@@ -227,153 +308,184 @@ quant_decode_kernel(const __grid_constant__ CUtensorMap tmk,
     total += v;
   }
   scan[tid] = before + incl - mine;
+  if (tid == 0) split = split_pages(total, a.groups, a.may_deal);
   __syncthreads();
-  if (blockIdx.x == 0) {                      // for the combine kernel
+  const bool dealt = split.dealt != 0;
+  const int unit = (warp / kUnit) * gridDim.x + blockIdx.x;
+  const int SG = unit / a.Hkv, h = unit - SG * a.Hkv;
+  // where each sequence's results will lie, for the combine kernel: a run of
+  // sequences a thread, spread over the CTAs
+  auto tell_combine = [&]() {
+    if (tid % gridDim.x != blockIdx.x) return;
     int run = scan[tid];
     for (int i = 0; i < per; ++i) {
       const int b = tid * per + i;
       if (b >= a.B) break;
-      a.ws.prefix[b] = run;
-      run += pages_of(__ldg(a.lens + b), a.max_pages);
-    }
-    if (tid == 0) a.ws.prefix[a.B] = total;
-  }
-
-  // ---- this warp's KV head and pages
-  const int id = warp * gridDim.x + blockIdx.x;
-  const int G = id / a.Hkv, h = id - G * a.Hkv;
-  const int n_groups = groups_of(total, a.groups);
-  if (G >= n_groups) return;
-  const int s0 = first_page(G, total, n_groups);
-  Walk w;
-  w.left = first_page(G + 1, total, n_groups) - s0;
-  const int n_pages = w.left;
-  {
-    int lo = 0;                               // last run that starts at or before s0
-#pragma unroll
-    for (int step = S::kThreads / 2; step >= 1; step >>= 1) {
-      if (scan[lo + step] <= s0) lo += step;
-    }
-    int cum = scan[lo];
-    w.base = lo * per;
-    while (true) {
-      w.len_w = walk_len(a, w.base, lane);
-      const int pg = pages_of(w.len_w, a.max_pages);
-      int in = pg;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, in, o);
-        if (lane >= o) in += v;
+      const int pages = pages_of(__ldg(a.lens + b), a.max_pages);
+      int2 in = make_int2(0, 0);
+      if (pages > 0) {
+        const int of = dealt ? 1 : kUnit;
+        in.x = segment_of(run, split) / of;
+        in.y = segment_of(run + pages - 1, split) / of - in.x + 1;
       }
-      const unsigned past = __ballot_sync(0xffffffffu, cum + in > s0);
-      if (past) {
-        const int i = __ffs(past) - 1;
-        walk_enter(w, a, w.base + i, s0 - cum - __shfl_sync(0xffffffffu, in - pg, i));
-        break;
-      }
-      cum += __shfl_sync(0xffffffffu, in, 31);
-      w.base += 32;
-      if (w.base >= a.B) return;              // cannot happen: s0 < total
+      a.ws.segments[b] = in;
+      run += pages;
     }
+  };
+  if (SG * kUnit >= split.n && !dealt) {      // the whole unit has nothing to do
+    tell_combine();
+    return;
   }
+  const int G = SG * kUnit + warp % kUnit;
+  const int r = lane >> 2, qd = lane & 3;
+  uint8_t *const my_ring = smem + warp * kStages * kStage;
+  uint8_t *const my_scales = scales + warp * kStages * 32;
+  Info *const my_info = infos + warp * kStages;
+  uint64_t *const my_full = full + warp * kStages;
 
-  uint8_t *ring = smem + warp * S::kStages * kStage;
-  uint8_t *sc_ring = scales + warp * S::kStages * 32;
-  PageInfo *info = infos + warp * S::kStages;
-  uint64_t *full = bars + warp * S::kStages;
-
-  // issue the walk's next page into stage s
-  auto produce = [&](int s) {
-    if (w.left == 0) return;
-    const int e = w.p / a.pages_per_block;
-    if (e >= w.entry + 32 || e < w.entry) {
-      w.entry = e;
-      const int last = (w.np - 1) / a.pages_per_block;
-      int blk = __ldg(a.bt + static_cast<int64_t>(w.b) * a.bt_stride + min(e + lane, last));
-      w.blk_w = blk < 0 || blk >= a.num_blocks ? 0 : blk;
+  // the range or piece whose pages are being issued
+  int seg = dealt ? G * kCuts : G, seg_h = h, seg_first = 0, seg_pages = 0, seg_at = 0;
+  if (G < split.n) {
+    if (dealt && lane == 0) atomicExch(a.ws.taken + range_id(G, h, a.Hkv), 0);
+    seg_first = first_page(G, split);
+    seg_pages = first_page(G + 1, split) - seg_first;
+    if (dealt) seg_pages = part_page(1, seg_pages);
+  }
+  Page page = {0, 0, 0, 0};             // lane i: page i of the 32 around seg_at
+  int issued = 0;
+  int own = dealt && G < split.n ? 1 : 0, misses = 0;
+  auto issue = [&](int s) {             // the next page, if there is one, into stage s
+    while (seg_at == seg_pages) {
+      if (!dealt || misses >= 3) return;
+      const int ranges = split.n * a.Hkv;
+      int range = range_id(G, h, a.Hkv);
+      if (!own) {
+        // look at 32 ranges' words, a lane each, and choose one with the least taken
+        range = static_cast<int>((static_cast<uint32_t>(unit * kUnit + warp + 97 * issued) * 61u +
+                                  (lane + 32 * misses) * 73u) % static_cast<uint32_t>(ranges));
+        const uint32_t taken = static_cast<uint32_t>(__ldcg(a.ws.taken + range));
+        unsigned who = 0;
+#pragma unroll
+        for (uint32_t i = 0; i + 1 < kCuts; ++i) {
+          const unsigned at = __ballot_sync(0xffffffffu, taken == i);
+          if (who == 0) who = at;
+        }
+        if (who == 0) { ++misses; continue; }
+        range = __shfl_sync(0xffffffffu, range, __ffs(who) - 1);
+      }
+      uint32_t i = 0;
+      if (lane == 0) i = static_cast<uint32_t>(atomicAdd(a.ws.taken + range, 1));
+      i = __shfl_sync(0xffffffffu, i, 0);
+      if (i + 1 >= kCuts) {                      // none left
+        if (own) own = 0; else ++misses;
+        continue;
+      }
+      const int g = range / a.Hkv, part = static_cast<int>(i) + 1;
+      seg = g * kCuts + part;
+      seg_h = range - g * a.Hkv;
+      const int at = first_page(g, split), pages = first_page(g + 1, split) - at;
+      seg_first = at + part_page(part, pages);
+      seg_pages = part_page(part + 1, pages) - part_page(part, pages);
+      seg_at = 0;
     }
-    const int blk = __shfl_sync(0xffffffffu, w.blk_w, e - w.entry);
-    const int len = __shfl_sync(0xffffffffu, w.len_w, w.b - w.base);
-    if (lane == 0) {
-      const int off = (w.p - e * a.pages_per_block) * kTok;
-      const int flags = (w.p == w.start ? 1 : 0) | (w.p + 1 == w.np || w.left == 1 ? 2 : 0) |
-                        (w.start == 0 ? 4 : 0) | (w.p + 1 == w.np ? 8 : 0);
-      info[s] = {w.b, w.p, len, flags};
-      uint8_t *dst = ring + s * kStage;
-      mbar_arrive_expect_tx(&full[s], kStage + 32);
-      const int tok = blk * a.block_size + off;
-      const int c1 = a.head_major ? h : tok, c2 = a.head_major ? tok : h;
-      tma_load_3d(dst, &tmk, &full[s], 0, c1, c2);
-      tma_load_3d(dst + kHalf, &tmv, &full[s], 0, c1, c2);
-      const int64_t so = blk * a.ssb + h * a.ssh + off;
-      bulk_g2s(sc_ring + s * 32, a.ks + so, 16, &full[s]);
-      bulk_g2s(sc_ring + s * 32 + 16, a.vs + so, 16, &full[s]);
+    if ((seg_at & 31) == 0 && seg_at + lane < seg_pages) {
+      const int k = seg_at + lane, at = seg_first + k;
+      const Place w = locate<S::kThreads>(a, scan, per, at);
+      const int entry = w.p / a.pages_per_block, off = (w.p - entry * a.pages_per_block) * kTok;
+      int blk = __ldg(a.bt + static_cast<int64_t>(w.b) * a.bt_stride + entry);
+      if (blk < 0 || blk >= a.num_blocks) blk = 0;   // as the other attention kernels read it
+      const bool seq_end = w.p + 1 == w.np, end = k + 1 == seg_pages;
+      page.b = w.b;
+      page.valid_flags =
+          min(w.len - w.p * kTok, kTok) |
+          ((w.p == 0 || k == 0 ? kFirst : 0) | (seq_end || end ? kLast : 0) |
+           (at - w.p >= seg_first ? kHead : 0) | (seq_end ? kTail : 0) | (end ? kEnd : 0)) << 8;
+      page.tok = blk * a.block_size + off;
+      page.scale = blk * a.ssb + seg_h * a.ssh + off;
     }
-    ++w.p;
-    --w.left;
-    if (w.left > 0 && w.p == w.np) walk_next(w, a, lane);
+    if (lane == (seg_at & 31)) {
+      my_info[s] = {page.b, page.valid_flags, seg_h, seg};
+      uint8_t *dst = my_ring + s * kStage;
+      mbar_arrive_expect_tx(&my_full[s], kStage + 32);
+      const int c1 = a.head_major ? seg_h : page.tok, c2 = a.head_major ? page.tok : seg_h;
+      tma_load_3d(dst, &tmk, &my_full[s], 0, c1, c2);
+      tma_load_3d(dst + kHalf, &tmv, &my_full[s], 0, c1, c2);
+      bulk_g2s(my_scales + s * 32, a.ks + page.scale, 16, &my_full[s]);
+      bulk_g2s(my_scales + s * 32 + 16, a.vs + page.scale, 16, &my_full[s]);
+    }
+    ++seg_at;
+    ++issued;
   };
 #pragma unroll
-  for (int s = 0; s < S::kStages; ++s) produce(s);
+  for (int s = 0; s < kStages; ++s) issue(s);
+  tell_combine();                       // while the pages travel
 
-  const int r = lane >> 2, qd = lane & 3;
+  const uint32_t ring = smem_u32(my_ring), sc_ring = smem_u32(my_scales);
   uint32_t qf[NT][16];                  // Q^T fragments: dims 32*qd + 4*j + {0,1}, {2,3}
   float qs[NT][2];                      // score factor of heads 2*qd, 2*qd + 1
   float acc[NT][8][4];                  // O^T: dims 16*r + 2*i, + 1; heads 2*qd, 2*qd + 1
-  float m[NT][2], mw[NT][2], l[NT][2];  // log2: maximum of s, of s + ev; sum of p
-  bool fail = false;
-  int it = 0;
-  for (; it < n_pages; ++it) {
-    const int s = it % S::kStages;
-    if (!mbar_wait(&full[s], (it / S::kStages) & 1)) { fail = true; break; }
-    const PageInfo pi = info[s];
-    if (pi.flags & 1) {
+  // log2, negated: maximum of s; of s + ev, less kUp. Sum of p (this lane's tokens)
+  float nm[NT][2], nw[NT][2], l[NT][2];
+  // q of a segment's query heads (head 8*t + r, dims 32*qd .. + 31), nothing summed yet
+  auto begin = [&](int b, int h) {
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const int head = t * 8 + r;
-        uint4 x[4] = {};
-        if (head < a.g) {
-          const uint4 *row = reinterpret_cast<const uint4 *>(
-              a.q + (static_cast<int64_t>(pi.b) * a.Hq + h * a.g + head) * kD + qd * 32);
+    for (int t = 0; t < NT; ++t) {
+      const int head = t * 8 + r;
+      uint4 x[4] = {};
+      if (head < a.g) {
+        const uint4 *src = reinterpret_cast<const uint4 *>(
+            a.q + (static_cast<int64_t>(b) * a.Hq + h * a.g + head) * kD + qd * 32);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) x[j] = __ldg(row + j);
-        }
-        const uint32_t *xw = reinterpret_cast<const uint32_t *>(x);
-        uint32_t amax = 0;
+        for (int j = 0; j < 4; ++j) x[j] = __ldg(src + j);
+      }
+      const uint32_t *xw = reinterpret_cast<const uint32_t *>(x);
+      uint32_t amax = 0;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          amax = max(amax, max((xw[j] << 16) & 0x7fffffffu, xw[j] & 0x7fff0000u));
-        }
-        amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-        amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-        const int ex = min(max(static_cast<int>(amax >> 23) - 127, -126), 126);
-        const float down = __uint_as_float(static_cast<uint32_t>(127 - ex) << 23);
-        const float up = a.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 + ex) << 23);
+      for (int j = 0; j < 16; ++j) {
+        amax = max(amax, max((xw[j] << 16) & 0x7fffffffu, xw[j] & 0x7fff0000u));
+      }
+      amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+      amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+      const int ex = min(max(static_cast<int>(amax >> 23) - 127, -126), 126);
+      const float down = __uint_as_float(static_cast<uint32_t>(127 - ex) << 23);
+      const float up = a.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 + ex) << 23);
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          qf[t][j] = pack_f16(bf16_lo(xw[j]) * down, bf16_hi(xw[j]) * down);
-        }
-        qs[t][0] = __shfl_sync(0xffffffffu, up, 8 * qd);
-        qs[t][1] = __shfl_sync(0xffffffffu, up, 8 * qd + 4);
+      for (int j = 0; j < 16; ++j) {
+        qf[t][j] = pack_f16(bf16_lo(xw[j]) * down, bf16_hi(xw[j]) * down);
+      }
+      qs[t][0] = __shfl_sync(0xffffffffu, up, 8 * qd);
+      qs[t][1] = __shfl_sync(0xffffffffu, up, 8 * qd + 4);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) { m[t][j] = mw[t][j] = -INFINITY; l[t][j] = 0.f; }
+      for (int j = 0; j < 2; ++j) { nm[t][j] = nw[t][j] = INFINITY; l[t][j] = 0.f; }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < 8; ++i) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) acc[t][i][j] = 0.f;
-        }
+        for (int j = 0; j < 4; ++j) acc[t][i][j] = 0.f;
       }
     }
-    const uint32_t kb = smem_u32(ring + s * kStage), vb = kb + kHalf;
-    // ---- S^T = K Q^T
+  };
+  __syncwarp();
+  if (issued > 0) begin(my_info[0].b, my_info[0].h);      // while the pages travel
+  Left mine_left = {-1, 0, 0, -1};
+  int stage = 0;
+  uint32_t parity = 0;
+  for (int it = 0; it < issued; ++it) {
+    if (!mbar_wait(&my_full[stage], parity)) {
+      // bounded: the copies still in flight must land before the CTA ends
+      for (int k = it + 1; k < issued; ++k) {
+        mbar_wait(&my_full[k % kStages], (k / kStages) & 1);
+      }
+      if (lane == 0 && a.err != nullptr) atomicExch(a.err, 1);
+      break;
+    }
+    const Info info = my_info[stage];
+    const int seq = info.b, valid = info.valid_flags & 0xff, flags = info.valid_flags >> 8;
+    const uint32_t kb = ring + stage * kStage, vb = kb + kHalf, sb = sc_ring + stage * 32;
+    if (it > 0 && (flags & kFirst)) begin(seq, info.h);
+    // ---- S^T = K Q^T, two chains of sums
     float sc[NT][4];
     {
-      float s0a[NT][4], s1a[NT][4];
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) s0a[t][j] = s1a[t][j] = 0.f;
-      }
+      float sa[NT][4], sz[NT][4];
 #pragma unroll
       for (int c = 0; c < 2; ++c) {         // 16-byte chunk 2*qd + c of rows r and r + 8
         const uint4 lo = lds128(kb + sw128(r, 2 * qd + c));
@@ -387,88 +499,103 @@ quant_decode_kernel(const __grid_constant__ CUtensorMap tmk,
           const uint32_t a3 = dequant_f16x2<kInt8, true>(hw[j]);
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
-            mma_f16(j & 1 ? s1a[t] : s0a[t], a0, a1, a2, a3, qf[t][8 * c + 2 * j],
-                    qf[t][8 * c + 2 * j + 1]);
+            const uint32_t b0 = qf[t][8 * c + 2 * j], b1 = qf[t][8 * c + 2 * j + 1];
+            if (c == 0 && j < 2) mma_f16_first(j ? sz[t] : sa[t], a0, a1, a2, a3, b0, b1);
+            else mma_f16(j & 1 ? sz[t] : sa[t], a0, a1, a2, a3, b0, b1);
           }
         }
       }
+      // tokens r, r + 8 (heads 2*qd, + 1 each), times the rows' scales
+      const float ks0 = __uint_as_float(max(lds8(sb + r) << 23, 0x00400000u));
+      const float ks1 = __uint_as_float(max(lds8(sb + r + 8) << 23, 0x00400000u));
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) sc[t][j] = s0a[t][j] + s1a[t][j];
+        for (int j = 0; j < 4; ++j) sc[t][j] = (sa[t][j] + sz[t][j]) * (j < 2 ? ks0 : ks1);
       }
     }
-    // ---- scores of tokens r, r + 8 and heads 2*qd, 2*qd + 1
-    const uint8_t *sb = sc_ring + s * 32;
-    const bool in0 = pi.page * kTok + r < pi.len, in1 = pi.page * kTok + r + 8 < pi.len;
-    const float ks0 = scale_of(sb[r]), ks1 = scale_of(sb[r + 8]);
-    const uint32_t vb0 = sb[16 + r], vb1 = sb[24 + r];
-    const float ev0 = vb0 == 255u ? __uint_as_float(0x7fffffffu) : static_cast<float>(static_cast<int>(vb0) - 127);
-    const float ev1 = vb1 == 255u ? __uint_as_float(0x7fffffffu) : static_cast<float>(static_cast<int>(vb1) - 127);
-    bool moves = false;
+    const uint32_t vb0 = lds8(sb + 16 + r), vb1 = lds8(sb + 24 + r);
+    const float ev0 = vb0 == 255u ? __uint_as_float(0x7fffffffu)
+                                  : __uint_as_float(0x4b000000u | vb0) - 8388735.0f;   // vb0 - 127
+    const float ev1 = vb1 == 255u ? __uint_as_float(0x7fffffffu)
+                                  : __uint_as_float(0x4b000000u | vb1) - 8388735.0f;
+    // ---- arguments of the exponentials, against the running maxima
+    float ap[NT][4], aw[NT][4];
+    auto arguments = [&]() {
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          ap[t][j] = fmaf(sc[t][j], qs[t][j & 1], nm[t][j & 1]);
+          aw[t][j] = fmaf(sc[t][j], qs[t][j & 1], (j < 2 ? ev0 : ev1) + nw[t][j & 1]);
+        }
+      }
+      if (valid < kTok) {            // what lies past the context may be anything
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (r + (j < 2 ? 0 : 8) >= valid) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t) ap[t][j] = aw[t][j] = -INFINITY;
+          }
+        }
+      }
+    };
+    arguments();
+    float over = -INFINITY, over_w = -INFINITY;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        sc[t][j] = in0 ? sc[t][j] * ks0 * qs[t][j] : -INFINITY;
-        sc[t][2 + j] = in1 ? sc[t][2 + j] * ks1 * qs[t][j] : -INFINITY;
-        const float most = fmaxf(sc[t][j], sc[t][2 + j]);
-        const float most_w = fmaxf(in0 ? sc[t][j] + ev0 : -INFINITY,
-                                   in1 ? sc[t][2 + j] + ev1 : -INFINITY);
-        moves |= most > m[t][j] + kSlack || most_w > mw[t][j] + kSlack;
+      for (int j = 0; j < 4; ++j) {
+        over = fmaxf(over, ap[t][j]);
+        over_w = fmaxf(over_w, aw[t][j]);
       }
     }
-    if (__any_sync(0xffffffffu, moves)) {
+    if (__any_sync(0xffffffffu, over > kSlack || over_w > kSlack + kUp)) {
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const float top = fmaxf(m[t][j], max3_over_rows(fmaxf(sc[t][j], sc[t][2 + j])));
-          const float top_w =
-              fmaxf(mw[t][j], max3_over_rows(fmaxf(in0 ? sc[t][j] + ev0 : -INFINITY,
-                                                   in1 ? sc[t][2 + j] + ev1 : -INFINITY)));
-          if (top > m[t][j]) {
-            l[t][j] *= exp2f(m[t][j] - top);
-            m[t][j] = top;
+          float s0 = sc[t][j] * qs[t][j], s1 = sc[t][2 + j] * qs[t][j];
+          float w0 = s0 + ev0, w1 = s1 + ev1;
+          if (r >= valid) s0 = w0 = -INFINITY;
+          if (r + 8 >= valid) s1 = w1 = -INFINITY;
+          const float top = max_over_rows(fmaxf(s0, s1)), top_w = max_over_rows(fmaxf(w0, w1));
+          if (-top < nm[t][j]) {
+            l[t][j] *= exp2f(-top - nm[t][j]);
+            nm[t][j] = -top;
           }
-          if (top_w > mw[t][j]) {
-            const float f = exp2f(mw[t][j] - top_w);
+          if (kUp - top_w < nw[t][j]) {
+            const float f = exp2f(kUp - top_w - nw[t][j]);
 #pragma unroll
             for (int i = 0; i < 8; ++i) { acc[t][i][j] *= f; acc[t][i][2 + j] *= f; }
-            mw[t][j] = top_w;
+            nw[t][j] = kUp - top_w;
           }
         }
       }
+      arguments();
     }
     // ---- weights
     uint32_t wb[NT][2];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      float p[4];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        l[t][j] += fast_exp2(sc[t][j] - m[t][j]) + fast_exp2(sc[t][2 + j] - m[t][j]);
-        const float d = mw[t][j] - kUp;
-        p[j] = in0 ? fast_exp2(sc[t][j] + ev0 - d) : 0.f;
-        p[2 + j] = in1 ? fast_exp2(sc[t][2 + j] + ev1 - d) : 0.f;
-      }
-      wb[t][0] = transpose8x8(pack_f16(p[0], p[1]));
-      wb[t][1] = transpose8x8(pack_f16(p[2], p[3]));
+      for (int j = 0; j < 2; ++j) l[t][j] += fast_exp2(ap[t][j]) + fast_exp2(ap[t][2 + j]);
+      wb[t][0] = transpose8x8(pack_f16(fast_exp2(aw[t][0]), fast_exp2(aw[t][1])));
+      wb[t][1] = transpose8x8(pack_f16(fast_exp2(aw[t][2]), fast_exp2(aw[t][3])));
     }
     // ---- O^T += V^T W^T: tokens 2*qd, + 1, + 8, + 9; dims 16*r .. + 15
     {
       uint4 v[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int row = 2 * qd + (j & 1) + (j >> 1) * 8;
-        v[j] = lds128(vb + sw128(row, r));
-      }
-      if (pi.page * kTok + kTok > pi.len) {      // rows past the context hold anything
+      for (int j = 0; j < 4; ++j) v[j] = lds128(vb + sw128(2 * qd + (j & 1) + (j >> 1) * 8, r));
+      if (valid < kTok) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          if (pi.page * kTok + 2 * qd + (j & 1) + (j >> 1) * 8 >= pi.len) v[j] = make_uint4(0, 0, 0, 0);
+          if (2 * qd + (j & 1) + (j >> 1) * 8 >= valid) v[j] = make_uint4(0, 0, 0, 0);
         }
       }
+      __syncwarp();            // every lane has read the stage: refill it
+      issue(stage);
       const uint32_t *w0 = reinterpret_cast<const uint32_t *>(&v[0]);
       const uint32_t *w1 = reinterpret_cast<const uint32_t *>(&v[1]);
       const uint32_t *w2 = reinterpret_cast<const uint32_t *>(&v[2]);
@@ -476,126 +603,204 @@ quant_decode_kernel(const __grid_constant__ CUtensorMap tmk,
 #pragma unroll
       for (int i = 0; i < 8; ++i) {              // dims 16*r + 2*i, + 1
         const uint32_t sel = i & 1 ? 0x7362u : 0x5140u;
-        const uint32_t x = bytes(w0[i >> 1], w1[i >> 1], sel);
-        const uint32_t y = bytes(w2[i >> 1], w3[i >> 1], sel);
-        const uint32_t a0 = dequant_f16x2<kInt8, false>(x), a1 = dequant_f16x2<kInt8, true>(x);
-        const uint32_t a2 = dequant_f16x2<kInt8, false>(y), a3 = dequant_f16x2<kInt8, true>(y);
+        const uint32_t y = bytes(w0[i >> 1], w1[i >> 1], sel);
+        const uint32_t z = bytes(w2[i >> 1], w3[i >> 1], sel);
+        const uint32_t a0 = dequant_f16x2<kInt8, false>(y), a1 = dequant_f16x2<kInt8, true>(y);
+        const uint32_t a2 = dequant_f16x2<kInt8, false>(z), a3 = dequant_f16x2<kInt8, true>(z);
 #pragma unroll
         for (int t = 0; t < NT; ++t) mma_f16(acc[t][i], a0, a1, a2, a3, wb[t][0], wb[t][1]);
       }
     }
-    __syncwarp();
-    produce(s);                // refill: every lane has read the stage
+    if (++stage == kStages) { stage = 0; parity ^= 1; }
 
-    if (pi.flags & 2) {
-      const bool whole = (pi.flags & 12) == 12;
-      const int64_t slot = 2ll * G + (pi.flags & 4 ? 1 : 0);
+    if (flags & kLast) {
+      const bool whole = (flags & (kHead | kTail)) == (kHead | kTail);
+      const bool end = (flags & kEnd) != 0;
+      float2 *ml = nullptr;
+      float *o = nullptr;
+      if (!whole) {
+        int64_t record = 2ll * info.segment + (flags & kHead ? 1 : 0);
+        if (!dealt) {
+          if (flags & kHead) {
+            mine_left.b1 = seq;          // goes on behind the range: its end
+          } else {
+            mine_left.b0 = seq;
+            mine_left.ends0 = flags & kTail;
+            mine_left.far0 = !end;
+          }
+          record = 2ll * (a.groups / kUnit) + G;
+        }
+        if (!dealt && end) {             // into the ring, whose pages are all read
+          o = reinterpret_cast<float *>(my_ring);
+          ml = reinterpret_cast<float2 *>(o + S::kHeads * kD);
+        } else {
+          o = a.ws.o + (record * a.Hq + info.h * a.g) * kD;
+          ml = a.ws.ml + record * a.Hq + info.h * a.g;
+        }
+        __syncwarp();
+      }
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           float sum = l[t][j];
 #pragma unroll
-          for (int o = 4; o <= 16; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+          for (int d = 4; d <= 16; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
           const int head = t * 8 + 2 * qd + j;
           if (head >= a.g) continue;
-          float f = exp2f(mw[t][j] - m[t][j] - kUp);
-          float o[16];
+          // maximum of s + ev less that of s, and the 2^kUp taken off
+          float f = exp2f(nm[t][j] - nw[t][j]);
           if (whole) f /= sum;
+          float y[16];
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            o[2 * i] = acc[t][i][j] * f;
-            o[2 * i + 1] = acc[t][i][2 + j] * f;
+            y[2 * i] = acc[t][i][j] * f;
+            y[2 * i + 1] = acc[t][i][2 + j] * f;
           }
-          const int hq = h * a.g + head;
           if (whole) {
             uint4 *dst = reinterpret_cast<uint4 *>(
-                a.out + (static_cast<int64_t>(pi.b) * a.Hq + hq) * kD + 16 * r);
+                a.out + (static_cast<int64_t>(seq) * a.Hq + info.h * a.g + head) * kD + 16 * r);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-              dst[i] = make_uint4(pack_bf16(o[8 * i], o[8 * i + 1]),
-                                  pack_bf16(o[8 * i + 2], o[8 * i + 3]),
-                                  pack_bf16(o[8 * i + 4], o[8 * i + 5]),
-                                  pack_bf16(o[8 * i + 6], o[8 * i + 7]));
+              dst[i] = make_uint4(pack_bf16(y[8 * i], y[8 * i + 1]),
+                                  pack_bf16(y[8 * i + 2], y[8 * i + 3]),
+                                  pack_bf16(y[8 * i + 4], y[8 * i + 5]),
+                                  pack_bf16(y[8 * i + 6], y[8 * i + 7]));
             }
           } else {
-            float4 *dst =
-                reinterpret_cast<float4 *>(a.ws.o + (slot * a.Hq + hq) * kD + 16 * r);
+            float4 *dst = reinterpret_cast<float4 *>(o + head * kD + 16 * r);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              dst[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+              dst[i] = make_float4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
             }
-            if (r == 0) a.ws.ml[slot * a.Hq + hq] = make_float2(m[t][j], sum);
+            if (r == 0) ml[head] = make_float2(-nm[t][j], sum);
           }
         }
       }
     }
   }
-  if (fail) {
-    // the ring's copies still in flight must land before the CTA ends
-    for (int k = it; k < n_pages - w.left; ++k) {
-      mbar_wait(&full[k % S::kStages], (k / S::kStages) & 1);
+
+  if (dealt) return;
+  // ---- the unit joins what its warps left, in the order of the pages
+  if (lane == 0) lefts[warp] = mine_left;
+  named_bar_sync(1 + warp / kUnit, kUnit * 32);
+  const int w0 = warp / kUnit * kUnit;
+  for (int i = tid - w0 * 32; i < a.g * (kD / 4); i += kUnit * 32) {
+    const int head = i / (kD / 4), d = i % (kD / 4);
+    const int hq = h * a.g + head;
+    bool open = false, before_unit = false;
+    int b = 0;
+    float m = 0.f, sum = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [&](float2 ml, float4 y) {
+      const float top = fmaxf(m, ml.x);
+      const float base = top == -INFINITY ? 0.f : top;
+      const float f0 = exp2f(m - base), f1 = exp2f(ml.x - base);
+      m = top;
+      sum = sum * f0 + ml.y * f1;
+      o.x = o.x * f0 + y.x * f1; o.y = o.y * f0 + y.y * f1;
+      o.z = o.z * f0 + y.z * f1; o.w = o.w * f0 + y.w * f1;
+    };
+    auto begin = [&](int seq, bool earlier) {
+      open = true;
+      before_unit = earlier;
+      b = seq;
+      m = -INFINITY;
+      sum = 0.f;
+      o = make_float4(0.f, 0.f, 0.f, 0.f);
+    };
+    auto partial = [&]() {
+      const int64_t at = (2ll * SG + (before_unit ? 0 : 1)) * a.Hq + hq;
+      if (d == 0) a.ws.ml[at] = make_float2(m, sum);
+      reinterpret_cast<float4 *>(a.ws.o + at * kD)[d] = o;
+    };
+    for (int w = w0; w < w0 + kUnit; ++w) {
+      const Left lf = lefts[w];
+      const float *near_o = reinterpret_cast<const float *>(smem + w * kStages * kStage);
+      const float2 *near_ml = reinterpret_cast<const float2 *>(near_o + S::kHeads * kD);
+      if (lf.b0 >= 0) {
+        if (!open) begin(lf.b0, true);
+        const int64_t far = (2ll * (a.groups / kUnit) + SG * kUnit + w - w0) * a.Hq + hq;
+        if (lf.far0) {
+          add(a.ws.ml[far], reinterpret_cast<const float4 *>(a.ws.o + far * kD)[d]);
+        } else {
+          add(near_ml[head], reinterpret_cast<const float4 *>(near_o + head * kD)[d]);
+        }
+        if (lf.ends0) {
+          if (before_unit) {
+            partial();
+          } else {
+            const float inv = 1.f / sum;
+            reinterpret_cast<uint2 *>(a.out + (static_cast<int64_t>(b) * a.Hq + hq) * kD)[d] =
+                make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
+          }
+          open = false;
+        }
+      }
+      if (lf.b1 >= 0) {
+        begin(lf.b1, false);
+        add(near_ml[head], reinterpret_cast<const float4 *>(near_o + head * kD)[d]);
+      }
     }
-    if (lane == 0 && a.err != nullptr) atomicExch(a.err, 1);
+    if (open) partial();
   }
 }
 
-// Joins the partial results of split sequences and writes the zeros of empty
-// ones. kSplit warps share a (sequence, query head), each taking every
-// kSplit-th partial; 8 of them for small batches, whose sequences have many
-// partials, one where there are enough rows to fill the GPU.
+// Joins the partial results of sequences that several units (or ranges and
+// pieces) shared, and writes
+// the zeros of empty ones. kSplit warps take a (sequence, query head), each
+// every kSplit-th partial, 8 of them in flight: as many warps as fit the GPU at
+// once, since a row's time is its chain of memory round trips. Launched while
+// the decode kernel runs and held by griddepcontrol until that is done.
 constexpr int kCombineWarps = 8;
 
 template <int kSplit>
 __global__ void __launch_bounds__(kCombineWarps * 32) quant_combine_kernel(const QDecodeArgs a) {
-  constexpr int kRows = kCombineWarps / kSplit;
+  constexpr int kRows = kCombineWarps / kSplit, kFly = 8;
   __shared__ float4 so[kCombineWarps][32];
   __shared__ float sm[kCombineWarps], sl[kCombineWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int part = warp % kSplit;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + warp / kSplit;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
   const bool live = row < static_cast<int64_t>(a.B) * a.Hq;
   const int b = live ? static_cast<int>(row / a.Hq) : 0;
   const int head = static_cast<int>(row - static_cast<int64_t>(b) * a.Hq);
-  const int p0 = a.ws.prefix[b], p1 = live ? a.ws.prefix[b + 1] : p0;
-  const int total = a.ws.prefix[a.B];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int2 in = live ? a.ws.segments[b] : make_int2(0, 1);
+  const int first = in.x, count = in.y;      // records: 2 * first + 1, then 2 * (first + i)
   uint2 *dst = reinterpret_cast<uint2 *>(a.out + row * kD) + lane;
-  int first = 0, count = 0;      // slots: 2 * first + 1, then 2 * (first + i)
-  if (p1 > p0) {
-    const int n = groups_of(total, a.groups);
-    first = group_of(p0, total, n);
-    count = group_of(p1 - 1, total, n) - first + 1;
-  } else if (live && part == 0) {
-    *dst = make_uint2(0u, 0u);
-  }
+  if (count == 0 && part == 0) *dst = make_uint2(0u, 0u);
   float m = -INFINITY, l = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (count > 1) {
-    auto at = [&](int i) { return (2ll * (first + i) + (i == 0 ? 1 : 0)) * a.Hq + head; };
-    for (int i = part + lane * kSplit; i < count; i += 32 * kSplit) m = fmaxf(m, a.ws.ml[at(i)].x);
+  if (count > 1) {               // 1: finished in one place
+    for (int i0 = part; i0 < count; i0 += kFly * kSplit) {
+      float4 x[kFly];
+      float2 ml[kFly];
 #pragma unroll
-    for (int d = 16; d >= 1; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-    const float mu = m == -INFINITY ? 0.f : m;
-    for (int i0 = part; i0 < count; i0 += 4 * kSplit) {
-      float4 x[4];
-      float2 ml[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < kFly; ++j) {
         const int i = i0 + j * kSplit;
+        ml[j] = make_float2(-INFINITY, 0.f);
+        x[j] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (i < count) {
-          ml[j] = a.ws.ml[at(i)];
-          x[j] = reinterpret_cast<const float4 *>(a.ws.o + at(i) * kD)[lane];
+          const int64_t at = (2ll * (first + i) + (i == 0 ? 1 : 0)) * a.Hq + head;
+          ml[j] = a.ws.ml[at];
+          x[j] = reinterpret_cast<const float4 *>(a.ws.o + at * kD)[lane];
         }
       }
+      float top = m;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (i0 + j * kSplit < count) {
-          const float f = exp2f(ml[j].x - mu);
-          l = fmaf(f, ml[j].y, l);
-          o.x = fmaf(f, x[j].x, o.x); o.y = fmaf(f, x[j].y, o.y);
-          o.z = fmaf(f, x[j].z, o.z); o.w = fmaf(f, x[j].w, o.w);
-        }
+      for (int j = 0; j < kFly; ++j) top = fmaxf(top, ml[j].x);
+      const float base = top == -INFINITY ? 0.f : top;
+      const float c = exp2f(m - base);
+      m = top;
+      l *= c;
+      o.x *= c; o.y *= c; o.z *= c; o.w *= c;
+#pragma unroll
+      for (int j = 0; j < kFly; ++j) {
+        const float f = exp2f(ml[j].x - base);
+        l = fmaf(f, ml[j].y, l);
+        o.x = fmaf(f, x[j].x, o.x); o.y = fmaf(f, x[j].y, o.y);
+        o.z = fmaf(f, x[j].z, o.z); o.w = fmaf(f, x[j].w, o.w);
       }
     }
   }
@@ -604,21 +809,55 @@ __global__ void __launch_bounds__(kCombineWarps * 32) quant_combine_kernel(const
     if (lane == 0) { sm[warp] = m; sl[warp] = l; }
     __syncthreads();
     if (part != 0 || count < 2) return;
+#pragma unroll
     for (int i = 1; i < kSplit; ++i) m = fmaxf(m, sm[warp + i]);
-    const float mu = m == -INFINITY ? 0.f : m;
+    const float base = m == -INFINITY ? 0.f : m;
     l = 0.f;
     o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
     for (int i = 0; i < kSplit; ++i) {
-      const float f = exp2f(sm[warp + i] - mu);
+      const float f = exp2f(sm[warp + i] - base);
       const float4 x = so[warp + i][lane];
       l = fmaf(f, sl[warp + i], l);
       o.x = fmaf(f, x.x, o.x); o.y = fmaf(f, x.y, o.y);
       o.z = fmaf(f, x.z, o.z); o.w = fmaf(f, x.w, o.w);
     }
   }
-  if (count < 2) return;          // finished by its group
+  if (count < 2) return;
   const float inv = 1.f / l;
   *dst = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
+}
+
+// Launch that may begin before the kernel ahead of it on the stream is done;
+// the kernel waits for that itself (griddepcontrol.wait).
+template <typename... K, typename... A>
+int launch_dependent(void (*kernel)(K...), unsigned grid, unsigned threads, size_t smem,
+                     cudaStream_t stream, const A &...args) {
+  cudaLaunchConfig_t c = {};
+  c.gridDim = dim3(grid);
+  c.blockDim = dim3(threads);
+  c.dynamicSmemBytes = smem;
+  c.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  c.attrs = at;
+  c.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&c, kernel, args...);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return set_error(VJ_ERR_CUDA,
+                     std::string("vj_paged_decode_quantized: ") + cudaGetErrorString(e));
+  }
+  return VJ_OK;
+}
+
+template <int kSplit>
+int launch_combine(const QDecodeArgs &a, int64_t rows, cudaStream_t stream) {
+  constexpr int kRows = kCombineWarps / kSplit;
+  return launch_dependent(quant_combine_kernel<kSplit>,
+                          static_cast<unsigned>((rows + kRows - 1) / kRows), kCombineWarps * 32, 0,
+                          stream, a);
 }
 
 template <bool kInt8, int NT>
@@ -626,22 +865,35 @@ int launch_decode(const CUtensorMap &tmk, const CUtensorMap &tmv, const QDecodeA
                   cudaStream_t stream) {
   using S = Shape<NT>;
   static_assert(S::kSmem <= 227 * 1024, "shared memory");
-  const char *what = "vj_paged_decode_quantized";
-  cudaError_t e = cudaFuncSetAttribute(quant_decode_kernel<kInt8, NT>,
-                                       cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       static_cast<int>(S::kSmem));
-  if (e != cudaSuccess) {
-    return set_error(VJ_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
+  // the shared-memory opt-in is a per-device attribute of the kernel
+  static std::atomic<bool> opted[64];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && (dev >= 64 || !opted[dev].load(std::memory_order_acquire))) {
+    e = cudaFuncSetAttribute(quant_decode_kernel<kInt8, NT>,
+                             cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             static_cast<int>(S::kSmem));
+    if (e == cudaSuccess && dev < 64) opted[dev].store(true, std::memory_order_release);
   }
-  quant_decode_kernel<kInt8, NT><<<grid, S::kThreads, S::kSmem, stream>>>(tmk, tmv, a);
-  return check_launch(what);
+  if (e != cudaSuccess) {
+    return set_error(VJ_ERR_CUDA,
+                     std::string("vj_paged_decode_quantized: ") + cudaGetErrorString(e));
+  }
+  return launch_dependent(quant_decode_kernel<kInt8, NT>, static_cast<unsigned>(grid),
+                          S::kThreads, S::kSmem, stream, tmk, tmv, a);
 }
 
-// Grid and groups of a shape, from head counts and the GPU's size alone.
-void decode_grid(int g, int num_kv_heads, int *grid, int *groups) {
-  const int warps = g <= 8 ? Shape<1>::kWarps : Shape<2>::kWarps;
-  *grid = std::max(num_sms(), (num_kv_heads + warps - 1) / warps);
-  *groups = *grid * warps / num_kv_heads;
+// Grid, warps of a unit and groups, from head counts and the GPU's size alone.
+void decode_grid(int g, int num_kv_heads, int *grid, int *unit, int *groups) {
+  const int units = g <= 8 ? Shape<1>::kUnits : Shape<2>::kUnits;      // of a CTA
+  *unit = g <= 8 ? Shape<1>::kUnit : Shape<2>::kUnit;
+  *grid = std::max(num_sms(), (num_kv_heads + units - 1) / units);
+  *groups = *grid * units / num_kv_heads * *unit;
+}
+
+// Whether block tables this large could hold enough pages to deal pieces.
+bool may_deal(int64_t batch, int64_t bt_width, int64_t block_size, int64_t groups) {
+  return batch * (bt_width * block_size / kTok) / groups >= kDealt;
 }
 
 }  // namespace
@@ -649,11 +901,17 @@ void decode_grid(int g, int num_kv_heads, int *grid, int *groups) {
 
 extern "C" size_t vj_paged_decode_quantized_workspace_size(int32_t batch, int32_t num_q_heads,
                                                            int32_t num_kv_heads,
-                                                           int32_t head_dim) {
-  if (batch < 0 || num_q_heads <= 0 || num_kv_heads <= 0 || head_dim != vj::kD) return 0;
-  int grid, groups;
-  vj::decode_grid((num_q_heads + num_kv_heads - 1) / num_kv_heads, num_kv_heads, &grid, &groups);
-  return vj::scratch_bytes(batch, num_q_heads, groups);
+                                                           int32_t head_dim, int32_t bt_width,
+                                                           int32_t block_size) {
+  if (batch < 0 || num_q_heads <= 0 || num_kv_heads <= 0 || head_dim != vj::kD || bt_width < 0 ||
+      block_size <= 0) {
+    return 0;
+  }
+  int grid, unit, groups;
+  vj::decode_grid((num_q_heads + num_kv_heads - 1) / num_kv_heads, num_kv_heads, &grid, &unit,
+                  &groups);
+  return vj::carve(nullptr, nullptr, batch, num_q_heads, num_kv_heads, groups, unit,
+                   vj::may_deal(batch, bt_width, block_size, groups));
 }
 
 extern "C" vj_status vj_paged_decode_quantized(
@@ -709,7 +967,8 @@ extern "C" vj_status vj_paged_decode_quantized(
     return set_error(VJ_ERR_INVALID_ARGUMENT, what + ": q and out must be 16-byte aligned");
   }
   const size_t need =
-      vj_paged_decode_quantized_workspace_size(batch, num_q_heads, num_kv_heads, head_dim);
+      vj_paged_decode_quantized_workspace_size(batch, num_q_heads, num_kv_heads, head_dim, bt_width,
+                                               block_size);
   if (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16 != 0) {
     return set_error(VJ_ERR_WORKSPACE, what + ": workspace needs " + std::to_string(need) +
                                            " bytes, 16-byte aligned");
@@ -748,13 +1007,9 @@ extern "C" vj_status vj_paged_decode_quantized(
   a.scale_log2 = scale * 1.4426950408889634f;
   a.err = error_flag;
   int grid;
-  decode_grid(a.g, num_kv_heads, &grid, &a.groups);
-  char *w = static_cast<char *>(workspace);
-  a.ws.prefix = reinterpret_cast<int32_t *>(w);
-  w += up256(4 * (static_cast<size_t>(batch) + 1));
-  a.ws.ml = reinterpret_cast<float2 *>(w);
-  w += up256(2 * static_cast<size_t>(a.groups) * num_q_heads * sizeof(float2));
-  a.ws.o = reinterpret_cast<float *>(w);
+  decode_grid(a.g, num_kv_heads, &grid, &a.unit, &a.groups);
+  a.may_deal = may_deal(batch, bt_width, block_size, a.groups) ? 1 : 0;
+  carve(&a.ws, workspace, batch, num_q_heads, num_kv_heads, a.groups, a.unit, a.may_deal != 0);
   const bool i8 = cache_dtype == VJ_CACHE_INT8;
   if (a.g <= 8) {
     rc = i8 ? launch_decode<true, 1>(tmk, tmv, a, grid, stream)
@@ -765,12 +1020,12 @@ extern "C" vj_status vj_paged_decode_quantized(
   }
   if (rc) return rc;
   const int64_t rows = static_cast<int64_t>(batch) * num_q_heads;
-  if (rows < 4 * kCombineWarps * num_sms()) {
-    quant_combine_kernel<kCombineWarps>
-        <<<static_cast<unsigned>(rows), kCombineWarps * 32, 0, stream>>>(a);
-  } else {
-    quant_combine_kernel<1><<<static_cast<unsigned>((rows + kCombineWarps - 1) / kCombineWarps),
-                              kCombineWarps * 32, 0, stream>>>(a);
-  }
+  // warps that can be resident at once: 32 an SM at this kernel's registers
+  const int64_t room = 32ll * num_sms();
+  rc = rows * 8 <= room ? launch_combine<8>(a, rows, stream)
+       : rows * 4 <= room ? launch_combine<4>(a, rows, stream)
+       : rows * 2 <= room ? launch_combine<2>(a, rows, stream)
+                          : launch_combine<1>(a, rows, stream);
+  if (rc) return rc;
   return check_launch("vj_paged_decode_quantized");
 }

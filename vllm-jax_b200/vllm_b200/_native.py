@@ -113,7 +113,7 @@ PROTOTYPES: dict[str, tuple] = {
         c_i32, c_i32, c_i32, c_i32, c_i32,          # B, max_len, zero_to, Hkv, D
         c_i64, c_i32, c_i32, c_i32,                 # nb, bs, bt_width, bt_stride
         c_i64, c_i64, c_i64, c_i64, c_i64, c_vp]),  # strides, scale strides, stream
-    "vj_paged_decode_quantized_workspace_size": (c_sz, [c_i32, c_i32, c_i32, c_i32]),
+    "vj_paged_decode_quantized_workspace_size": (c_sz, [c_i32, c_i32, c_i32, c_i32, c_i32, c_i32]),
     "vj_paged_decode_quantized": (c_int, [
         c_vp, c_vp, c_vp, c_vp, c_vp, c_i32,        # q, k, v, k_scales, v_scales, cache_dtype
         c_vp, c_vp, c_vp,                           # bt, lens, out

@@ -17,6 +17,7 @@ include/vjattn.h) has no counterpart there.
 from __future__ import annotations
 
 import contextlib
+import functools
 import math
 from dataclasses import dataclass
 
@@ -77,10 +78,13 @@ def _pool(cache: QuantizedKVCache):
     return (d, d + s2, s, s + c2), code, hkv, D, nb, bs, (sb, st, sh, cb, ch)
 
 
+_HERE = contextlib.nullcontext()
+
+
 def _device(dev: torch.device):
     """The C entries launch on the current device: make it the tensors'."""
-    if dev.index is None or dev.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
+    if dev.index is None or dev.index == torch._C._cuda_getDevice():
+        return _HERE
     return torch.cuda.device(dev)
 
 
@@ -207,7 +211,7 @@ def paged_decode_quantized(q: torch.Tensor, cache: QuantizedKVCache, block_table
     if scale is None:
         scale = 1.0 / math.sqrt(D)
     with _device(dev):
-        need = decode_quantized_workspace_bytes(B, Hq, Hkv, D)
+        need = _decode_workspace_bytes(dev.index, B, Hq, Hkv, D, block_tables.shape[1], bs)
         if workspace is None:
             workspace = torch.empty(need, dtype=torch.uint8, device=dev)
         elif workspace.dtype != torch.uint8 or workspace.numel() < need \
@@ -221,11 +225,18 @@ def paged_decode_quantized(q: torch.Tensor, cache: QuantizedKVCache, block_table
     return out
 
 
+@functools.lru_cache(maxsize=1024)
+def _decode_workspace_bytes(device_index, *sizes: int) -> int:
+    return int(_native.load().vj_paged_decode_quantized_workspace_size(*sizes))
+
+
 def decode_quantized_workspace_bytes(batch: int, num_q_heads: int, num_kv_heads: int,
+                                     table_width: int, block_size: int,
                                      head_dim: int = 128) -> int:
-    """Scratch of one paged_decode_quantized call on the current device."""
-    return int(_native.load().vj_paged_decode_quantized_workspace_size(
-        batch, num_q_heads, num_kv_heads, head_dim))
+    """Scratch of one paged_decode_quantized call, on the current device, with
+    block tables of table_width entries."""
+    return _decode_workspace_bytes(torch.cuda.current_device(), batch, num_q_heads, num_kv_heads,
+                                   head_dim, table_width, block_size)
 
 
 def _read(cache, pool, block_tables, context_lens, out, B, max_len, zero_to, dev):
