@@ -494,7 +494,8 @@ VJ_API vj_status vj_allreduce_add_rmsnorm(
  * nothing (their q is still written). Slots that are stored must differ from
  * each other within a call. q_out may equal q_in with the same row stride.
  *   q_out [T,Hq,D] with row stride q_out_row_stride (0: packed); num_q_heads
- *   may be 0 (q_in, q_out unused). Other flags are rejected. */
+ *   may be 0 (q_in, q_out unused). Other flags are rejected.
+ *   error_flag: device int32 (may be NULL), set to 1 if a wait timed out */
 VJ_API vj_status vj_kv_store_quantized(
     const void *q_in, const void *k_in, const void *v_in, const void *q_norm_w,
     const void *k_norm_w, const int32_t *positions, const int32_t *slot_mapping, void *q_out,
@@ -504,7 +505,7 @@ VJ_API vj_status vj_kv_store_quantized(
     int64_t stride_head, int64_t scale_stride_block, int64_t scale_stride_head,
     int64_t q_row_stride, int64_t k_row_stride, int64_t v_row_stride, int64_t q_out_row_stride,
     const void *rope_table, int32_t rope_table_len, double eps, float rope_theta, int32_t flags,
-    cudaStream_t stream);
+    int32_t *error_flag, cudaStream_t stream);
 
 /* Read a batch's cache back: k_out/v_out [B, max_len, Hkv, D] bf16, packed, row
  * t of sequence b = its cached position t for t < min(context_lens[b],

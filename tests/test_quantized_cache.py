@@ -53,7 +53,7 @@ def test_products_are_bf16_numbers():
 def _store(lib, **kw):
     a = dict(q=16, k=16, v=16, qw=16, kw=16, pos=16, slots=16, qo=16, kc=16, vc=16, ks=16, vs=16,
              dt=1, T=4, Hq=8, Hkv=2, D=128, nb=4, bs=16, sb=4096, st=256, sh=128, cb=32, ch=16,
-             qrs=0, krs=0, vrs=0, qors=0, tab=None, tl=0, eps=1e-6, th=1e6, fl=3, stream=None)
+             qrs=0, krs=0, vrs=0, qors=0, tab=None, tl=0, eps=1e-6, th=1e6, fl=3, err=None, stream=None)
     a.update(kw)
     return lib.vj_kv_store_quantized(*a.values())
 

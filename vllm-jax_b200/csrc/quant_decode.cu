@@ -828,36 +828,12 @@ __global__ void __launch_bounds__(kCombineWarps * 32) quant_combine_kernel(const
   *dst = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
 }
 
-// Launch that may begin before the kernel ahead of it on the stream is done;
-// the kernel waits for that itself (griddepcontrol.wait).
-template <typename... K, typename... A>
-int launch_dependent(void (*kernel)(K...), unsigned grid, unsigned threads, size_t smem,
-                     cudaStream_t stream, const A &...args) {
-  cudaLaunchConfig_t c = {};
-  c.gridDim = dim3(grid);
-  c.blockDim = dim3(threads);
-  c.dynamicSmemBytes = smem;
-  c.stream = stream;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  c.attrs = at;
-  c.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&c, kernel, args...);
-  if (e != cudaSuccess) {
-    cudaGetLastError();
-    return set_error(VJ_ERR_CUDA,
-                     std::string("vj_paged_decode_quantized: ") + cudaGetErrorString(e));
-  }
-  return VJ_OK;
-}
-
 template <int kSplit>
 int launch_combine(const QDecodeArgs &a, int64_t rows, cudaStream_t stream) {
   constexpr int kRows = kCombineWarps / kSplit;
-  return launch_dependent(quant_combine_kernel<kSplit>,
-                          static_cast<unsigned>((rows + kRows - 1) / kRows), kCombineWarps * 32, 0,
-                          stream, a);
+  return launch_dependent("vj_paged_decode_quantized", quant_combine_kernel<kSplit>,
+                          dim3(static_cast<unsigned>((rows + kRows - 1) / kRows)),
+                          kCombineWarps * 32, 0, stream, a);
 }
 
 template <bool kInt8, int NT>
@@ -879,8 +855,9 @@ int launch_decode(const CUtensorMap &tmk, const CUtensorMap &tmv, const QDecodeA
     return set_error(VJ_ERR_CUDA,
                      std::string("vj_paged_decode_quantized: ") + cudaGetErrorString(e));
   }
-  return launch_dependent(quant_decode_kernel<kInt8, NT>, static_cast<unsigned>(grid),
-                          S::kThreads, S::kSmem, stream, tmk, tmv, a);
+  return launch_dependent("vj_paged_decode_quantized", quant_decode_kernel<kInt8, NT>,
+                          dim3(static_cast<unsigned>(grid)), S::kThreads, S::kSmem, stream, tmk,
+                          tmv, a);
 }
 
 // Grid, warps of a unit and groups, from head counts and the GPU's size alone.

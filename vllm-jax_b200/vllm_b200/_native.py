@@ -106,7 +106,7 @@ PROTOTYPES: dict[str, tuple] = {
         c_i64, c_i32, c_i32, c_i32, c_i64, c_i32,   # T, Hq, Hkv, D, nb, bs
         c_i64, c_i64, c_i64, c_i64, c_i64,          # strides (block, token, head), scale (block, head)
         c_i64, c_i64, c_i64, c_i64,                 # q/k/v/q_out row strides (0 = packed)
-        c_vp, c_i32, ctypes.c_double, c_f32, c_i32, c_vp]),   # table, len, eps, theta, flags, stream
+        c_vp, c_i32, ctypes.c_double, c_f32, c_i32, c_vp, c_vp]),   # table, len, eps, theta, flags, err, stream
     "vj_kv_read_quantized": (c_int, [
         c_vp, c_vp, c_vp, c_vp, c_i32,              # k, v, k_scales, v_scales, cache_dtype
         c_vp, c_vp, c_vp, c_vp,                     # bt, lens, k_out, v_out

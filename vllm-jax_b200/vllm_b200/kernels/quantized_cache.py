@@ -167,7 +167,7 @@ def kv_store_quantized(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor,
                      code, T, Hq, Hkv, D, nb, bs, *strides, q.stride(0) if q is not None else 0,
                      k.stride(0), v.stride(0), q_out.stride(0) if q is not None else 0,
                      ptr(table) if tab_len else None, tab_len, float(eps), float(rope_theta),
-                     flags, stream_ptr(dev))
+                     flags, _err_flag(dev).data_ptr(), stream_ptr(dev))
     return q_out
 
 
@@ -272,6 +272,28 @@ def read_kv_cache(cache: QuantizedKVCache, block_tables: torch.Tensor,
     return out
 
 
+_identity: dict[int, torch.Tensor] = {}
+_retired_identity: list[torch.Tensor] = []
+
+
+def _identity_pages(dev: torch.device, n: int) -> torch.Tensor:
+    """0, 1, .., the block tables of a scratch whose pages lie in order, kept per
+    device and only grown. An outgrown tensor is kept too: a captured graph may
+    read it. What a capture makes is the graph's own."""
+    if torch.cuda.is_current_stream_capturing():
+        t = _identity.get(dev.index)
+        return t[:n] if t is not None and t.numel() >= n else \
+            torch.arange(n, dtype=torch.int32, device=dev)
+    t = _identity.get(dev.index)
+    if t is None or t.numel() < n:
+        if t is not None:
+            _retired_identity.append(t)
+        # a blocking copy: complete for every stream when it returns
+        t = torch.arange(max(n, 1 << 16), dtype=torch.int32).to(dev)
+        _identity[dev.index] = t
+    return t[:n]
+
+
 # bf16 rows (token x KV head) of one read-back inside paged_prefill_quantized:
 # 1 GiB of K and V. Batches that need more run in groups of sequences.
 PREFILL_SCRATCH_ROWS = 1 << 21
@@ -318,7 +340,7 @@ def paged_prefill_quantized(q: torch.Tensor, cache: QuantizedKVCache, block_tabl
     group = max(1, min(S, PREFILL_SCRATCH_ROWS // (L * Hkv)))
     with _device(dev):
         # page p of the group's sequence b is row block b * L/16 + p of the scratch
-        pages = torch.arange(group * (L // 16), dtype=torch.int32, device=dev).view(group, -1)
+        pages = _identity_pages(dev, group * (L // 16)).view(group, -1)
         scratch = torch.empty((2, group, L, Hkv, D), dtype=torch.bfloat16, device=dev)
         kv = scratch.view(2, group * (L // 16), 16, Hkv, D)
         for s in range(0, max(S, 1), group):
