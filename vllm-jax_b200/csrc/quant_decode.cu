@@ -25,6 +25,10 @@
 // its own partial results: who does which changes no result.
 //   quant_combine_kernel joins the partial results, at most two of a unit,
 // range or piece, in the order of the pages.
+//   Where the block tables hold at most kWhole pages a row and there is a unit for
+// every sequence and KV head, a unit takes a whole sequence: nothing is left to
+// join, and there is one launch (17 tokens: 5.7 us against 7.5; at 125 pages, 16 a
+// warp, it would be 21 against 11).
 //
 // A warp streams its pages through a ring of its own in shared memory: TMA
 // boxes of 16 rows x 128 bytes (128-byte swizzle) and the rows' scale bytes.
@@ -62,6 +66,7 @@ using namespace qn;
 constexpr int kTok = 16;                      // tokens per page
 constexpr int kHalf = kTok * kD;              // bytes of a page's K (or V) rows
 constexpr int kStage = 2 * kHalf;
+constexpr int kWhole = 32;                    // pages up to which a unit takes a sequence
 constexpr int kDealt = 32;                    // pages a warp from which on a part is dealt
 constexpr float kSlack = 11.0f;               // log2 of what a score may pass the maximum by
 constexpr float kUp = 4.0f;                   // log2 of the weight at the maximum
@@ -91,11 +96,17 @@ struct Left {
   int b1;         // sequence of a segment that began in the range and goes on behind it, or -1
 };
 
-// How `total` pages are split: n ranges of neighbouring pages. Where pieces are
-// dealt, a range is cut in kCuts parts.
+// A sequence and a page of it.
+struct Place {
+  int b, p, np, len;      // p of np pages, of a context of len tokens
+};
+
+// How all pages are split: n ranges of neighbouring pages, the first `more` of
+// them of pages + 1, the others of `pages`. Where pieces are dealt, a range is
+// cut in kCuts parts.
 constexpr int kCuts = 4;
 struct Split {
-  int total, n, dealt;
+  int n, pages, more, dealt;
 };
 
 template <int NT>
@@ -109,7 +120,8 @@ struct Shape {                                // NT tiles of 8 query heads
   static constexpr int kHeads = NT * 8;
   // pages, scale bytes, barriers, left records, scan
   static constexpr size_t kSmem = 1024 + (size_t)kRing * (kStage + 32 + sizeof(Info) + 8) +
-                                  kWarps * sizeof(Left) + sizeof(Split) + (kThreads + kWarps) * 4;
+                                  kWarps * sizeof(Left) + kUnits * (sizeof(Split) + sizeof(Place)) +
+                                  (kThreads + kWarps) * 4;
   // a record in a warp's ring: kHeads x 128 outputs, kHeads (maximum, sum)
   static_assert(kHeads * (kD + 2) * 4 <= kStages * kStage, "a record fits the ring");
 };
@@ -146,9 +158,10 @@ struct QDecodeArgs {
   const int32_t *bt, *lens;
   const uint8_t *ks, *vs;
   int64_t ssb, ssh;
-  int B, Hq, Hkv, g, bt_stride, pages_per_block, block_size, max_pages, num_blocks, head_major;
+  int B, Hq, Hkv, g, bt_stride, pages_per_block, ppb_shift, block_size, max_pages, num_blocks, head_major;
   int unit;           // warps of a unit
   int groups;         // warps that serve a KV head, a multiple of unit
+  int whole;          // whether a unit takes a whole sequence
   int may_deal;       // whether the tables could hold enough to deal pieces
   float scale_log2;
   Scratch ws;
@@ -156,14 +169,14 @@ struct QDecodeArgs {
 };
 
 VJ_DEV Split split_pages(int total, int groups, int may_deal) {
-  return {total, min(groups, total), may_deal && total / groups >= kDealt ? 1 : 0};
+  const int n = max(min(groups, total), 1);
+  return {total > 0 ? n : 0, total / n, total % n, may_deal && total / groups >= kDealt ? 1 : 0};
 }
-// First page of range G.
-VJ_DEV int first_page(int G, const Split &t) {
-  return static_cast<int>(static_cast<int64_t>(G) * t.total / t.n);
-}
+// First page of range G (no division: every warp waits for it).
+VJ_DEV int first_page(int G, const Split &t) { return G * t.pages + min(G, t.more); }
 VJ_DEV int range_of(int page, const Split &t) {
-  return static_cast<int>((static_cast<int64_t>(page + 1) * t.n - 1) / t.total);
+  const int longer = t.more * (t.pages + 1);
+  return page < longer ? page / (t.pages + 1) : t.more + (page - longer) / t.pages;
 }
 // First page of part i (0..kCuts) of a range of `pages`: 4/5 of it, 3/25, 1/25, 1/25.
 VJ_DEV int part_page(int i, int pages) {
@@ -234,11 +247,7 @@ VJ_DEV float max_over_rows(float v) {        // over the lanes that share lane &
   return v;
 }
 
-// Sequence and page-in-sequence of page s of all pages; scan[i] = pages before
-// sequence i * per.
-struct Place {
-  int b, p, np, len;
-};
+// The place of page s of all pages; scan[i] = pages before sequence i * per.
 template <int kRuns>
 VJ_DEV Place locate(const QDecodeArgs &a, const int *scan, int per, int s) {
   int lo = 0;                               // last run that starts at or before s
@@ -272,9 +281,10 @@ quant_decode_kernel(const __grid_constant__ CUtensorMap tmk,
   Info *infos = reinterpret_cast<Info *>(scales + S::kRing * 32);
   uint64_t *full = reinterpret_cast<uint64_t *>(infos + S::kRing);
   Left *lefts = reinterpret_cast<Left *>(full + S::kRing);
-  Split &split = *reinterpret_cast<Split *>(lefts + S::kWarps);
-  int *scan = reinterpret_cast<int *>(&split + 1);            // [kThreads]
-  int *warp_sum = scan + S::kThreads;                         // [kWarps]
+  Split *splits = reinterpret_cast<Split *>(lefts + S::kWarps);     // [kUnits]
+  Place *wholes = reinterpret_cast<Place *>(splits + S::kUnits);    // [kUnits]
+  int *scan = reinterpret_cast<int *>(wholes + S::kUnits);          // [kThreads]
+  int *warp_sum = scan + S::kThreads;                               // [kWarps]
 
   if (lane == 0) {
     for (int s = 0; s < kStages; ++s) mbar_init(&full[warp * kStages + s], 1);
@@ -285,34 +295,56 @@ quant_decode_kernel(const __grid_constant__ CUtensorMap tmk,
   // combine kernel may be made ready as soon as every CTA of this one runs
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;");
-  // ---- pages before each run of `per` sequences
-  const int per = (a.B + S::kThreads - 1) / S::kThreads;
-  int mine = 0;
-  for (int i = 0; i < per; ++i) {
-    const int b = tid * per + i;
-    if (b < a.B) mine += pages_of(__ldg(a.lens + b), a.max_pages);
-  }
-  int incl = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int v = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += v;
-  }
-  if (lane == 31) warp_sum[warp] = incl;
-  __syncthreads();
-  int before = 0, total = 0;
-#pragma unroll
-  for (int w = 0; w < S::kWarps; ++w) {
-    const int v = warp_sum[w];
-    before += w < warp ? v : 0;
-    total += v;
-  }
-  scan[tid] = before + incl - mine;
-  if (tid == 0) split = split_pages(total, a.groups, a.may_deal);
-  __syncthreads();
-  const bool dealt = split.dealt != 0;
   const int unit = (warp / kUnit) * gridDim.x + blockIdx.x;
-  const int SG = unit / a.Hkv, h = unit - SG * a.Hkv;
+  const int per = (a.B + S::kThreads - 1) / S::kThreads;
+  if (!a.whole) {
+    // ---- pages before each run of `per` sequences
+    int mine = 0;
+    for (int i = 0; i < per; ++i) {
+      const int b = tid * per + i;
+      if (b < a.B) mine += pages_of(__ldg(a.lens + b), a.max_pages);
+    }
+    int incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    if (lane == 31) warp_sum[warp] = incl;
+    __syncthreads();
+    int before = 0, total = 0;
+#pragma unroll
+    for (int w = 0; w < S::kWarps; ++w) {
+      const int v = warp_sum[w];
+      before += w < warp ? v : 0;
+      total += v;
+    }
+    scan[tid] = before + incl - mine;
+    if (tid < S::kUnits) splits[tid] = split_pages(total, a.groups, a.may_deal);
+    __syncthreads();
+  } else {
+    // ---- the unit's sequence, as if it were all there is
+    const int b = unit / a.Hkv;
+    const int len = b < a.B ? __ldg(a.lens + b) : 0, pages = pages_of(len, a.max_pages);
+    if (b >= a.B) return;        // the whole unit
+    if (pages == 0) {
+      const int i = tid % (kUnit * 32), h = unit - b * a.Hkv;
+      uint4 *dst = reinterpret_cast<uint4 *>(
+          a.out + (static_cast<int64_t>(b) * a.Hq + h * a.g) * kD);
+      if (i < a.g * (kD / 8)) dst[i] = make_uint4(0, 0, 0, 0);
+      return;
+    }
+    // every warp writes the same; the ranges go to the unit's first warps
+    if (lane == 0) {
+      wholes[warp / kUnit] = {b, 0, pages, len};
+      splits[warp / kUnit] = split_pages(pages, kUnit, 0);
+    }
+    __syncwarp();
+  }
+  const Split &split = splits[warp / kUnit];
+  const bool dealt = split.dealt != 0;
+  const int SG = a.whole ? 0 : unit / a.Hkv;
+  const int h = unit % a.Hkv;
   // where each sequence's results will lie, for the combine kernel: a run of
   // sequences a thread, spread over the CTAs
   auto tell_combine = [&]() {
@@ -332,7 +364,7 @@ quant_decode_kernel(const __grid_constant__ CUtensorMap tmk,
       run += pages;
     }
   };
-  if (SG * kUnit >= split.n && !dealt) {      // the whole unit has nothing to do
+  if (!a.whole && SG * kUnit >= split.n && !dealt) {      // the unit has nothing to do
     tell_combine();
     return;
   }
@@ -390,8 +422,15 @@ quant_decode_kernel(const __grid_constant__ CUtensorMap tmk,
     }
     if ((seg_at & 31) == 0 && seg_at + lane < seg_pages) {
       const int k = seg_at + lane, at = seg_first + k;
-      const Place w = locate<S::kThreads>(a, scan, per, at);
-      const int entry = w.p / a.pages_per_block, off = (w.p - entry * a.pages_per_block) * kTok;
+      Place w;
+      if (a.whole) {
+        w = wholes[warp / kUnit];
+        w.p = at;
+      } else {
+        w = locate<S::kThreads>(a, scan, per, at);
+      }
+      const int entry = a.ppb_shift >= 0 ? w.p >> a.ppb_shift : w.p / a.pages_per_block;
+      const int off = (w.p - entry * a.pages_per_block) * kTok;
       int blk = __ldg(a.bt + static_cast<int64_t>(w.b) * a.bt_stride + entry);
       if (blk < 0 || blk >= a.num_blocks) blk = 0;   // as the other attention kernels read it
       const bool seq_end = w.p + 1 == w.np, end = k + 1 == seg_pages;
@@ -418,7 +457,7 @@ quant_decode_kernel(const __grid_constant__ CUtensorMap tmk,
   };
 #pragma unroll
   for (int s = 0; s < kStages; ++s) issue(s);
-  tell_combine();                       // while the pages travel
+  if (!a.whole) tell_combine();         // while the pages travel
 
   const uint32_t ring = smem_u32(my_ring), sc_ring = smem_u32(my_scales);
   uint32_t qf[NT][16];                  // Q^T fragments: dims 32*qd + 4*j + {0,1}, {2,3}
@@ -868,6 +907,12 @@ void decode_grid(int g, int num_kv_heads, int *grid, int *unit, int *groups) {
   *groups = *grid * units / num_kv_heads * *unit;
 }
 
+// Whether a unit takes a whole sequence, so that there is nothing to join.
+bool whole_sequences(int64_t batch, int64_t num_kv_heads, int64_t table_pages, int grid, int g) {
+  const int units = g <= 8 ? Shape<1>::kUnits : Shape<2>::kUnits;
+  return table_pages <= kWhole && batch * num_kv_heads <= static_cast<int64_t>(grid) * units;
+}
+
 // Whether block tables this large could hold enough pages to deal pieces.
 bool may_deal(int64_t batch, int64_t bt_width, int64_t block_size, int64_t groups) {
   return batch * (bt_width * block_size / kTok) / groups >= kDealt;
@@ -977,6 +1022,8 @@ extern "C" vj_status vj_paged_decode_quantized(
   a.g = num_q_heads / num_kv_heads;
   a.bt_stride = bt_stride;
   a.pages_per_block = block_size / kTok;
+  a.ppb_shift = (a.pages_per_block & (a.pages_per_block - 1)) == 0
+                    ? __builtin_ctz(a.pages_per_block) : -1;
   a.block_size = block_size;
   a.max_pages = static_cast<int>(table_pages);
   a.num_blocks = static_cast<int>(num_blocks);
@@ -985,7 +1032,8 @@ extern "C" vj_status vj_paged_decode_quantized(
   a.err = error_flag;
   int grid;
   decode_grid(a.g, num_kv_heads, &grid, &a.unit, &a.groups);
-  a.may_deal = may_deal(batch, bt_width, block_size, a.groups) ? 1 : 0;
+  a.whole = whole_sequences(batch, num_kv_heads, table_pages, grid, a.g) ? 1 : 0;
+  a.may_deal = !a.whole && may_deal(batch, bt_width, block_size, a.groups) ? 1 : 0;
   carve(&a.ws, workspace, batch, num_q_heads, num_kv_heads, a.groups, a.unit, a.may_deal != 0);
   const bool i8 = cache_dtype == VJ_CACHE_INT8;
   if (a.g <= 8) {
@@ -995,7 +1043,7 @@ extern "C" vj_status vj_paged_decode_quantized(
     rc = i8 ? launch_decode<true, 2>(tmk, tmv, a, grid, stream)
             : launch_decode<false, 2>(tmk, tmv, a, grid, stream);
   }
-  if (rc) return rc;
+  if (rc || a.whole) return rc;
   const int64_t rows = static_cast<int64_t>(batch) * num_q_heads;
   // warps that can be resident at once: 32 an SM at this kernel's registers
   const int64_t room = 32ll * num_sms();

@@ -178,7 +178,7 @@ def check(status: int) -> None:
 # kernels launched by one successful call of each entry point
 KERNELS_PER_CALL = {"vj_paged_decode": 3, "vj_paged_decode_planned": 2,
                     "vj_paged_decode_noalloc": 3, "vj_paged_prefill": 2,
-                    "vj_paged_attention_mixed": 3}
+                    "vj_paged_attention_mixed": 3, "vj_paged_decode_quantized": 2}
 launch_count = 0
 
 

@@ -26,7 +26,7 @@ import torch
 from .. import _native
 from ._util import ptr, require_cuda, require_dtype, stream_ptr
 from .kv_store import rope_table
-from .prefill_paged_attention import _err_flag, paged_prefill
+from .prefill_paged_attention import _err_flag
 
 CACHE_DTYPES = {"e4m3": torch.float8_e4m3fn, "int8": torch.int8}
 _CODES = {torch.float8_e4m3fn: _native.VJ_CACHE_E4M3, torch.int8: _native.VJ_CACHE_INT8}
@@ -239,12 +239,13 @@ def decode_quantized_workspace_bytes(batch: int, num_q_heads: int, num_kv_heads:
                                    head_dim, table_width, block_size)
 
 
-def _read(cache, pool, block_tables, context_lens, out, B, max_len, zero_to, dev):
+def _read(pool, tables: int, width: int, stride: int, lens: int, out: int, B: int, max_len: int,
+          zero_to: int, stream: int) -> None:
+    """vj_kv_read_quantized into packed K, then V, at address `out`."""
     ptrs, code, Hkv, D, nb, bs, strides = pool
-    _native.call("vj_kv_read_quantized", *ptrs, code, block_tables.data_ptr(),
-                 context_lens.data_ptr(), out[0].data_ptr(), out[1].data_ptr(), B, max_len,
-                 zero_to, Hkv, D, nb, bs, block_tables.shape[1], _table_stride(block_tables),
-                 *strides, stream_ptr(dev))
+    _native.call("vj_kv_read_quantized", *ptrs, code, tables, lens, out,
+                 out + B * max_len * Hkv * D * 2, B, max_len, zero_to, Hkv, D, nb, bs, width,
+                 stride, *strides, stream)
 
 
 def read_kv_cache(cache: QuantizedKVCache, block_tables: torch.Tensor,
@@ -268,7 +269,8 @@ def read_kv_cache(cache: QuantizedKVCache, block_tables: torch.Tensor,
     elif out.shape != shape or out.dtype != torch.bfloat16 or not out.is_contiguous():
         raise ValueError(f"out must be a contiguous bf16 tensor of shape {shape}")
     with _device(dev):
-        _read(cache, pool, block_tables, context_lens, out, B, L, 0, dev)
+        _read(pool, block_tables.data_ptr(), block_tables.shape[1], _table_stride(block_tables),
+              context_lens.data_ptr(), out.data_ptr(), B, L, 0, stream_ptr(dev))
     return out
 
 
@@ -337,17 +339,25 @@ def paged_prefill_quantized(q: torch.Tensor, cache: QuantizedKVCache, block_tabl
         out = torch.empty_like(q)
     elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
         raise ValueError("out must be a contiguous bf16 tensor of q's shape")
+    if scale is None:
+        scale = 1.0 / math.sqrt(D)
     group = max(1, min(S, PREFILL_SCRATCH_ROWS // (L * Hkv)))
+    T, Hq, _ = q.shape
+    per_seq = L // 16                  # page p of the group's sequence b: block b * per_seq + p
+    half = group * L * Hkv * D         # elements of the scratch's K, and of its V
     with _device(dev):
-        # page p of the group's sequence b is row block b * L/16 + p of the scratch
-        pages = _identity_pages(dev, group * (L // 16)).view(group, -1)
-        scratch = torch.empty((2, group, L, Hkv, D), dtype=torch.bfloat16, device=dev)
-        kv = scratch.view(2, group * (L // 16), 16, Hkv, D)
+        stream = stream_ptr(dev)
+        pages = _identity_pages(dev, group * per_seq).data_ptr()
+        scratch = torch.empty(2 * half, dtype=torch.bfloat16, device=dev)
+        k_ptr = scratch.data_ptr()
+        stride = _table_stride(block_tables)
+        tables, width, lens = block_tables.data_ptr(), block_tables.shape[1], context_lens.data_ptr()
         for s in range(0, max(S, 1), group):
             n = min(group, S - s)
-            if n > 0:
-                _read(cache, pool, block_tables[s:s + n], context_lens[s:s + n], scratch, n, L,
-                      _KEY_TILE, dev)
-            paged_prefill(q, kv, pages[:n], cu_seqlens_q[s:s + n + 1], context_lens[s:s + n],
-                          max_seqlen_q, scale, out)
+            _read(pool, tables + 4 * s * stride, width, stride, lens + 4 * s, k_ptr, n, L,
+                  _KEY_TILE, stream)
+            _native.call("vj_paged_prefill", q.data_ptr(), k_ptr, k_ptr + n * L * Hkv * D * 2, pages,
+                         cu_seqlens_q.data_ptr() + 4 * s, lens + 4 * s, out.data_ptr(), T, n, Hq,
+                         Hkv, D, max(n, 1) * per_seq, 16, per_seq, per_seq, 16 * Hkv * D, Hkv * D, D,
+                         int(max_seqlen_q), float(scale), _err_flag(dev).data_ptr(), stream)
     return out
