@@ -5,10 +5,13 @@
 // HBM-bound: every cached row is read once (129 bytes a row, K and V), for all
 // query heads of its KV head together.
 //
-// The work is cut into pages of 16 tokens. All sequences' pages in a row,
-// numbered 0..T-1, are split evenly over the warps that serve a KV head; the
-// warps of the other heads walk the same pages at the same time, so a page's
-// rows, which lie side by side, are read together. Every CTA finds its warps'
+// The work is cut into pages of 16 tokens. All sequences' pages in a row are
+// split evenly over the warps that serve a KV head; the warps of the other heads
+// walk the same pages at the same time, so a page's rows, which lie side by
+// side, are read together. A sequence's start (its q, its own results) costs a
+// warp about as much as three pages, so the split counts that many places before
+// every sequence's pages: without them a warp with six short sequences among 64
+// of 1 to 8192 tokens took 26 us where most took 18. Every CTA finds its warps'
 // ranges from the context lengths by itself: there is no planning launch.
 //   Little work (below kDealt pages a warp): eight warps with neighbouring
 // ranges form a unit and join the sequences they share in shared memory; a
@@ -66,6 +69,7 @@ using namespace qn;
 constexpr int kTok = 16;                      // tokens per page
 constexpr int kHalf = kTok * kD;              // bytes of a page's K (or V) rows
 constexpr int kStage = 2 * kHalf;
+constexpr int kStart = 3;                     // places in front of a sequence's pages
 constexpr int kWhole = 32;                    // pages up to which a unit takes a sequence
 constexpr int kDealt = 32;                    // pages a warp from which on a part is dealt
 constexpr float kSlack = 11.0f;               // log2 of what a score may pass the maximum by
@@ -247,7 +251,11 @@ VJ_DEV float max_over_rows(float v) {        // over the lanes that share lane &
   return v;
 }
 
-// The place of page s of all pages; scan[i] = pages before sequence i * per.
+// Places of a sequence of `pages` pages.
+VJ_DEV int places_of(int pages) { return pages > 0 ? pages + kStart : 0; }
+
+// The sequence at place s of all places, and its page there (negative: in front
+// of its pages); scan[i] = places before sequence i * per.
 template <int kRuns>
 VJ_DEV Place locate(const QDecodeArgs &a, const int *scan, int per, int s) {
   int lo = 0;                               // last run that starts at or before s
@@ -260,10 +268,11 @@ VJ_DEV Place locate(const QDecodeArgs &a, const int *scan, int per, int s) {
   for (w.b = lo * per;; ++w.b) {            // s lies in this run
     w.len = __ldg(a.lens + w.b);
     w.np = pages_of(w.len, a.max_pages);
-    if (s < cum + w.np || w.b + 1 >= a.B) break;
-    cum += w.np;
+    const int places = places_of(w.np);
+    if (s < cum + places || w.b + 1 >= a.B) break;
+    cum += places;
   }
-  w.p = s - cum;
+  w.p = s - cum - kStart;
   return w;
 }
 
@@ -298,11 +307,11 @@ quant_decode_kernel(const __grid_constant__ CUtensorMap tmk,
   const int unit = (warp / kUnit) * gridDim.x + blockIdx.x;
   const int per = (a.B + S::kThreads - 1) / S::kThreads;
   if (!a.whole) {
-    // ---- pages before each run of `per` sequences
+    // ---- places before each run of `per` sequences
     int mine = 0;
     for (int i = 0; i < per; ++i) {
       const int b = tid * per + i;
-      if (b < a.B) mine += pages_of(__ldg(a.lens + b), a.max_pages);
+      if (b < a.B) mine += places_of(pages_of(__ldg(a.lens + b), a.max_pages));
     }
     int incl = mine;
 #pragma unroll
@@ -357,11 +366,11 @@ quant_decode_kernel(const __grid_constant__ CUtensorMap tmk,
       int2 in = make_int2(0, 0);
       if (pages > 0) {
         const int of = dealt ? 1 : kUnit;
-        in.x = segment_of(run, split) / of;
-        in.y = segment_of(run + pages - 1, split) / of - in.x + 1;
+        in.x = segment_of(run + kStart, split) / of;
+        in.y = segment_of(run + kStart + pages - 1, split) / of - in.x + 1;
       }
       a.ws.segments[b] = in;
-      run += pages;
+      run += places_of(pages);
     }
   };
   if (!a.whole && SG * kUnit >= split.n && !dealt) {      // the unit has nothing to do
@@ -376,73 +385,85 @@ quant_decode_kernel(const __grid_constant__ CUtensorMap tmk,
   uint64_t *const my_full = full + warp * kStages;
 
   // the range or piece whose pages are being issued
-  int seg = dealt ? G * kCuts : G, seg_h = h, seg_first = 0, seg_pages = 0, seg_at = 0;
+  int seg = dealt ? G * kCuts : G, seg_h = h, seg_at = 0, seg_end = 0, seg_first = 0;
   if (G < split.n) {
     if (dealt && lane == 0) atomicExch(a.ws.taken + range_id(G, h, a.Hkv), 0);
-    seg_first = first_page(G, split);
-    seg_pages = first_page(G + 1, split) - seg_first;
-    if (dealt) seg_pages = part_page(1, seg_pages);
+    seg_at = seg_first = first_page(G, split);
+    seg_end = first_page(G + 1, split);
+    if (dealt) seg_end = seg_at + part_page(1, seg_end - seg_at);
   }
-  Page page = {0, 0, 0, 0};             // lane i: page i of the 32 around seg_at
+  Page page = {};                       // lane i: the page at place i of 32
+  unsigned there = 0;                   // lanes whose places have pages yet to issue
   int issued = 0;
   int own = dealt && G < split.n ? 1 : 0, misses = 0;
   auto issue = [&](int s) {             // the next page, if there is one, into stage s
-    while (seg_at == seg_pages) {
-      if (!dealt || misses >= 3) return;
-      const int ranges = split.n * a.Hkv;
-      int range = range_id(G, h, a.Hkv);
-      if (!own) {
-        // look at 32 ranges' words, a lane each, and choose one with the least taken
-        range = static_cast<int>((static_cast<uint32_t>(unit * kUnit + warp + 97 * issued) * 61u +
-                                  (lane + 32 * misses) * 73u) % static_cast<uint32_t>(ranges));
-        const uint32_t taken = static_cast<uint32_t>(__ldcg(a.ws.taken + range));
-        unsigned who = 0;
+    while (there == 0) {
+      if (seg_at >= seg_end) {
+        if (!dealt || misses >= 3) return;
+        const int ranges = split.n * a.Hkv;
+        int range = range_id(G, h, a.Hkv);
+        if (!own) {
+          // look at 32 ranges' words, a lane each, and choose one with the least taken
+          range = static_cast<int>((static_cast<uint32_t>(unit * kUnit + warp + 97 * issued) * 61u +
+                                    (lane + 32 * misses) * 73u) % static_cast<uint32_t>(ranges));
+          const uint32_t taken = static_cast<uint32_t>(__ldcg(a.ws.taken + range));
+          unsigned who = 0;
 #pragma unroll
-        for (uint32_t i = 0; i + 1 < kCuts; ++i) {
-          const unsigned at = __ballot_sync(0xffffffffu, taken == i);
-          if (who == 0) who = at;
+          for (uint32_t i = 0; i + 1 < kCuts; ++i) {
+            const unsigned at = __ballot_sync(0xffffffffu, taken == i);
+            if (who == 0) who = at;
+          }
+          if (who == 0) { ++misses; continue; }
+          range = __shfl_sync(0xffffffffu, range, __ffs(who) - 1);
         }
-        if (who == 0) { ++misses; continue; }
-        range = __shfl_sync(0xffffffffu, range, __ffs(who) - 1);
+        uint32_t i = 0;
+        if (lane == 0) i = static_cast<uint32_t>(atomicAdd(a.ws.taken + range, 1));
+        i = __shfl_sync(0xffffffffu, i, 0);
+        if (i + 1 >= kCuts) {                      // none left
+          if (own) own = 0; else ++misses;
+          continue;
+        }
+        const int g = range / a.Hkv, part = static_cast<int>(i) + 1;
+        seg = g * kCuts + part;
+        seg_h = range - g * a.Hkv;
+        const int at = first_page(g, split), pages = first_page(g + 1, split) - at;
+        seg_at = seg_first = at + part_page(part, pages);
+        seg_end = at + part_page(part + 1, pages);
       }
-      uint32_t i = 0;
-      if (lane == 0) i = static_cast<uint32_t>(atomicAdd(a.ws.taken + range, 1));
-      i = __shfl_sync(0xffffffffu, i, 0);
-      if (i + 1 >= kCuts) {                      // none left
-        if (own) own = 0; else ++misses;
-        continue;
+      // the next 32 places, one a lane
+      const int at = seg_at + lane;
+      bool has_page = false;
+      if (at < seg_end) {
+        Place w;
+        if (a.whole) {
+          w = wholes[warp / kUnit];
+          w.p = at;
+        } else {
+          w = locate<S::kThreads>(a, scan, per, at);
+        }
+        has_page = w.p >= 0;
+        if (has_page) {
+          const int entry = a.ppb_shift >= 0 ? w.p >> a.ppb_shift : w.p / a.pages_per_block;
+          const int off = (w.p - entry * a.pages_per_block) * kTok;
+          int blk = __ldg(a.bt + static_cast<int64_t>(w.b) * a.bt_stride + entry);
+          if (blk < 0 || blk >= a.num_blocks) blk = 0;   // as the other attention kernels read it
+          const bool seq_end = w.p + 1 == w.np;
+          const bool end = at + 1 + (seq_end ? kStart : 0) >= seg_end;    // no page after it
+          page.b = w.b;
+          page.valid_flags =
+              min(w.len - w.p * kTok, kTok) |
+              ((w.p == 0 || at == seg_first ? kFirst : 0) | (seq_end || end ? kLast : 0) |
+               (at - w.p >= seg_first ? kHead : 0) | (seq_end ? kTail : 0) | (end ? kEnd : 0)) << 8;
+          page.tok = blk * a.block_size + off;
+          page.scale = blk * a.ssb + seg_h * a.ssh + off;
+        }
       }
-      const int g = range / a.Hkv, part = static_cast<int>(i) + 1;
-      seg = g * kCuts + part;
-      seg_h = range - g * a.Hkv;
-      const int at = first_page(g, split), pages = first_page(g + 1, split) - at;
-      seg_first = at + part_page(part, pages);
-      seg_pages = part_page(part + 1, pages) - part_page(part, pages);
-      seg_at = 0;
+      there = __ballot_sync(0xffffffffu, has_page);
+      seg_at += 32;
     }
-    if ((seg_at & 31) == 0 && seg_at + lane < seg_pages) {
-      const int k = seg_at + lane, at = seg_first + k;
-      Place w;
-      if (a.whole) {
-        w = wholes[warp / kUnit];
-        w.p = at;
-      } else {
-        w = locate<S::kThreads>(a, scan, per, at);
-      }
-      const int entry = a.ppb_shift >= 0 ? w.p >> a.ppb_shift : w.p / a.pages_per_block;
-      const int off = (w.p - entry * a.pages_per_block) * kTok;
-      int blk = __ldg(a.bt + static_cast<int64_t>(w.b) * a.bt_stride + entry);
-      if (blk < 0 || blk >= a.num_blocks) blk = 0;   // as the other attention kernels read it
-      const bool seq_end = w.p + 1 == w.np, end = k + 1 == seg_pages;
-      page.b = w.b;
-      page.valid_flags =
-          min(w.len - w.p * kTok, kTok) |
-          ((w.p == 0 || k == 0 ? kFirst : 0) | (seq_end || end ? kLast : 0) |
-           (at - w.p >= seg_first ? kHead : 0) | (seq_end ? kTail : 0) | (end ? kEnd : 0)) << 8;
-      page.tok = blk * a.block_size + off;
-      page.scale = blk * a.ssb + seg_h * a.ssh + off;
-    }
-    if (lane == (seg_at & 31)) {
+    const int who = __ffs(there) - 1;
+    there &= there - 1;
+    if (lane == who) {
       my_info[s] = {page.b, page.valid_flags, seg_h, seg};
       uint8_t *dst = my_ring + s * kStage;
       mbar_arrive_expect_tx(&my_full[s], kStage + 32);
@@ -452,7 +473,6 @@ quant_decode_kernel(const __grid_constant__ CUtensorMap tmk,
       bulk_g2s(my_scales + s * 32, a.ks + page.scale, 16, &my_full[s]);
       bulk_g2s(my_scales + s * 32 + 16, a.vs + page.scale, 16, &my_full[s]);
     }
-    ++seg_at;
     ++issued;
   };
 #pragma unroll
@@ -975,7 +995,7 @@ extern "C" vj_status vj_paged_decode_quantized(
                             "block_size * stride_token)");
   }
   const int64_t table_pages = static_cast<int64_t>(bt_width) * (block_size / kTok);
-  if (static_cast<int64_t>(batch) * table_pages > INT32_MAX ||
+  if (static_cast<int64_t>(batch) * (table_pages + kStart) > INT32_MAX ||
       static_cast<int64_t>(batch) * num_q_heads > INT32_MAX) {
     return set_error(VJ_ERR_UNSUPPORTED, what + ": batch or block tables too large (2^31 pages)");
   }

@@ -24,7 +24,7 @@ from dataclasses import dataclass
 import torch
 
 from .. import _native
-from ._util import ptr, require_cuda, require_dtype, stream_ptr
+from ._util import require_cuda, require_dtype, stream_ptr
 from .kv_store import rope_table
 from .prefill_paged_attention import _err_flag
 
@@ -59,14 +59,16 @@ class QuantizedKVCache:
 def _pool(cache: QuantizedKVCache):
     """(pointers, element type, Hkv, D, num_blocks, block_size, strides) of a cache."""
     data, scales = cache.data, cache.scales
-    if data.dim() != 5 or data.shape[0] != 2:
+    shape = data.shape
+    if len(shape) != 5 or shape[0] != 2:
         raise ValueError("cache.data must have shape (2, num_blocks, block_size, Hkv, D); "
-                         f"got {tuple(data.shape)}")
-    _, nb, bs, hkv, D = data.shape
+                         f"got {tuple(shape)}")
+    _, nb, bs, hkv, D = shape
     code = _CODES.get(data.dtype)
     if code is None:
         raise ValueError(f"The dtype of `cache.data` must be float8_e4m3fn or int8. Got {data.dtype}")
-    require_dtype(scales, torch.uint8, "cache.scales")
+    if scales.dtype is not torch.uint8:
+        require_dtype(scales, torch.uint8, "cache.scales")
     if scales.shape != (2, nb, hkv, bs):
         raise ValueError(f"cache.scales must have shape (2, num_blocks, Hkv, block_size) = "
                          f"{(2, nb, hkv, bs)}; got {tuple(scales.shape)}")
@@ -88,17 +90,29 @@ def _device(dev: torch.device):
     return torch.cuda.device(dev)
 
 
-def _rows(t: torch.Tensor, name: str, T: int, D: int) -> None:
+def _rows(t: torch.Tensor, name: str, T: int, D: int) -> tuple[int, int]:
+    """(heads, row stride) of a [T, H, D] tensor with packed heads."""
+    shape = t.shape
+    if len(shape) == 3 and t.dtype is torch.bfloat16:
+        rs, hs, es = t.stride()
+        if shape[0] == T and shape[2] == D and es == 1 and (hs == D or shape[1] == 1):
+            return shape[1], rs
     require_dtype(t, torch.bfloat16, name)
-    if t.dim() != 3 or t.shape[0] != T or t.shape[2] != D or t.stride(2) != 1 \
-            or (t.shape[1] > 1 and t.stride(1) != D):
-        raise ValueError(f"`{name}` must be a [num_tokens, H, head_dim] tensor with packed heads")
+    raise ValueError(f"`{name}` must be a [num_tokens, H, head_dim] tensor with packed heads")
 
 
 def _indices(t: torch.Tensor, name: str, T: int) -> None:
-    require_dtype(t, torch.int32, name)
+    if t.dtype is not torch.int32:
+        require_dtype(t, torch.int32, name)
     if t.shape != (T,) or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous [{T}] tensor; got shape {tuple(t.shape)}")
+
+
+def _weight(w: torch.Tensor, name: str, D: int) -> int:
+    require_dtype(w, torch.bfloat16, name)
+    if w.shape != (D,) or not w.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous [head_dim] tensor")
+    return w.data_ptr()
 
 
 def kv_store_quantized(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor,
@@ -121,69 +135,73 @@ def kv_store_quantized(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor,
     T = k.shape[0]
     if v.shape != k.shape:
         raise ValueError(f"k and v must have the same shape. Got {tuple(k.shape)} and {tuple(v.shape)}")
-    _rows(k, "k", T, D)
-    _rows(v, "v", T, D)
-    if k.shape[1] != Hkv:
+    heads, k_stride = _rows(k, "k", T, D)
+    _, v_stride = _rows(v, "v", T, D)
+    if heads != Hkv:
         raise ValueError("cache heads/head_dim do not match k")
     _indices(slot_mapping, "slot_mapping", T)
-    Hq = 0
+    Hq = q_stride = out_stride = 0
+    q_ptr = out_ptr = qw_ptr = kw_ptr = pos_ptr = table_ptr = None
     if q is not None:
-        _rows(q, "q", T, D)
-        Hq = q.shape[1]
+        Hq, q_stride = _rows(q, "q", T, D)
         if q_out is None:
-            q_out = torch.empty((T, Hq, D), dtype=q.dtype, device=dev)
+            q_out = torch.empty((T, Hq, D), dtype=torch.bfloat16, device=dev)
+            out_stride = Hq * D
         else:
-            _rows(q_out, "q_out", T, D)
-            if q_out.shape != q.shape:
+            out_heads, out_stride = _rows(q_out, "q_out", T, D)
+            if out_heads != Hq:
                 raise ValueError("q_out must have q's shape")
+        q_ptr, out_ptr = q.data_ptr(), q_out.data_ptr()
     elif q_out is not None:
         raise ValueError("q_out needs q")
     flags = 0
     if norm:
-        flags |= _native.VJ_KV_NORM
+        flags = _native.VJ_KV_NORM
         if k_norm_weight is None or (q is not None and q_norm_weight is None):
             raise ValueError("norm=True needs q_norm_weight and k_norm_weight")
-        for name, w in (("k_norm_weight", k_norm_weight), ("q_norm_weight", q_norm_weight)):
-            if w is not None:
-                require_dtype(w, torch.bfloat16, name)
-                if w.shape != (D,) or not w.is_contiguous():
-                    raise ValueError(f"{name} must be a contiguous [head_dim] tensor")
+        kw_ptr = _weight(k_norm_weight, "k_norm_weight", D)
+        if q is not None:
+            qw_ptr = _weight(q_norm_weight, "q_norm_weight", D)
     tab_len = 0
     if rope:
         flags |= _native.VJ_KV_ROPE
         if positions is None:
             raise ValueError("rope=True needs positions")
         _indices(positions, "positions", T)
+        pos_ptr = positions.data_ptr()
         if table is None:
             table = rope_table(dev, rope_theta)
         require_dtype(table, torch.int32, "table")
         if not table.is_contiguous():
             raise ValueError("table must be contiguous")
         tab_len = table.numel() // 64
+        if tab_len:
+            table_ptr = table.data_ptr()
     with _device(dev):
-        _native.call("vj_kv_store_quantized", ptr(q), k.data_ptr(), v.data_ptr(),
-                     ptr(q_norm_weight if norm else None), ptr(k_norm_weight if norm else None),
-                     ptr(positions if rope else None), slot_mapping.data_ptr(), ptr(q_out), *ptrs,
-                     code, T, Hq, Hkv, D, nb, bs, *strides, q.stride(0) if q is not None else 0,
-                     k.stride(0), v.stride(0), q_out.stride(0) if q is not None else 0,
-                     ptr(table) if tab_len else None, tab_len, float(eps), float(rope_theta),
-                     flags, _err_flag(dev).data_ptr(), stream_ptr(dev))
+        _native.call("vj_kv_store_quantized", q_ptr, k.data_ptr(), v.data_ptr(), qw_ptr, kw_ptr,
+                     pos_ptr, slot_mapping.data_ptr(), out_ptr, *ptrs, code, T, Hq, Hkv, D, nb, bs,
+                     *strides, q_stride, k_stride, v_stride, out_stride, table_ptr, tab_len, eps,
+                     rope_theta, flags, _err_flag(dev).data_ptr(), stream_ptr(dev))
     return q_out
 
 
-def _tables(block_tables: torch.Tensor, context_lens: torch.Tensor, B: int) -> None:
-    require_dtype(block_tables, torch.int32, "block_tables")
-    if block_tables.dim() != 2 or block_tables.shape[0] != B:
+def _tables(block_tables: torch.Tensor, context_lens: torch.Tensor, B: int) -> tuple[int, int]:
+    """(width, row stride) of the block tables."""
+    if block_tables.dtype is not torch.int32:
+        require_dtype(block_tables, torch.int32, "block_tables")
+    shape = block_tables.shape
+    if len(shape) != 2 or shape[0] != B:
         raise ValueError("`block_tables` must have one row per sequence")
-    if block_tables.shape[1] > 1 and block_tables.stride(1) != 1:
+    width = shape[1]
+    stride, s1 = block_tables.stride()
+    if s1 != 1 and width > 1:
         raise ValueError("block_tables rows must be contiguous")
-    if B > 1 and block_tables.stride(0) < block_tables.shape[1]:
-        raise ValueError("block_tables rows must not overlap")
+    if stride < width:
+        if B > 1:
+            raise ValueError("block_tables rows must not overlap")
+        stride = width
     _indices(context_lens, "context_lens", B)
-
-
-def _table_stride(block_tables: torch.Tensor) -> int:
-    return max(block_tables.stride(0), block_tables.shape[1])
+    return width, stride
 
 
 def paged_decode_quantized(q: torch.Tensor, cache: QuantizedKVCache, block_tables: torch.Tensor,
@@ -203,7 +221,7 @@ def paged_decode_quantized(q: torch.Tensor, cache: QuantizedKVCache, block_table
     B, Hq, Dq = q.shape
     if Dq != D or Hq % Hkv:
         raise ValueError("q heads/head_dim do not match the cache")
-    _tables(block_tables, context_lens, B)
+    width, stride = _tables(block_tables, context_lens, B)
     if out is None:
         out = torch.empty_like(q)
     elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
@@ -211,7 +229,7 @@ def paged_decode_quantized(q: torch.Tensor, cache: QuantizedKVCache, block_table
     if scale is None:
         scale = 1.0 / math.sqrt(D)
     with _device(dev):
-        need = _decode_workspace_bytes(dev.index, B, Hq, Hkv, D, block_tables.shape[1], bs)
+        need = _decode_workspace_bytes(dev.index, B, Hq, Hkv, D, width, bs)
         if workspace is None:
             workspace = torch.empty(need, dtype=torch.uint8, device=dev)
         elif workspace.dtype != torch.uint8 or workspace.numel() < need \
@@ -219,8 +237,7 @@ def paged_decode_quantized(q: torch.Tensor, cache: QuantizedKVCache, block_table
             raise ValueError(f"decode workspace must be contiguous uint8 with >= {need} bytes")
         _native.call("vj_paged_decode_quantized", q.data_ptr(), *ptrs, code,
                      block_tables.data_ptr(), context_lens.data_ptr(), out.data_ptr(), B, Hq, Hkv,
-                     D, nb, bs, block_tables.shape[1], _table_stride(block_tables), *strides,
-                     float(scale), workspace.data_ptr(), workspace.numel(),
+                     D, nb, bs, width, stride, *strides, scale, workspace.data_ptr(), workspace.numel(),
                      _err_flag(dev).data_ptr(), stream_ptr(dev))
     return out
 
@@ -259,18 +276,18 @@ def read_kv_cache(cache: QuantizedKVCache, block_tables: torch.Tensor,
     pool = _pool(cache)
     _, _, Hkv, D, _, bs, _ = pool
     B = block_tables.shape[0]
-    _tables(block_tables, context_lens, B)
+    width, stride = _tables(block_tables, context_lens, B)
     if max_context_len < 0:
         raise ValueError("max_context_len must not be negative")
-    L = int(max_context_len) or block_tables.shape[1] * bs
+    L = int(max_context_len) or width * bs
     shape = (2, B, L, Hkv, D)
     if out is None:
         out = torch.empty(shape, dtype=torch.bfloat16, device=dev)
     elif out.shape != shape or out.dtype != torch.bfloat16 or not out.is_contiguous():
         raise ValueError(f"out must be a contiguous bf16 tensor of shape {shape}")
     with _device(dev):
-        _read(pool, block_tables.data_ptr(), block_tables.shape[1], _table_stride(block_tables),
-              context_lens.data_ptr(), out.data_ptr(), B, L, 0, stream_ptr(dev))
+        _read(pool, block_tables.data_ptr(), width, stride, context_lens.data_ptr(),
+              out.data_ptr(), B, L, 0, stream_ptr(dev))
     return out
 
 
@@ -329,10 +346,10 @@ def paged_prefill_quantized(q: torch.Tensor, cache: QuantizedKVCache, block_tabl
     S = cu_seqlens_q.shape[0] - 1
     if context_lens is None:
         context_lens = cu_seqlens_q[1:] - cu_seqlens_q[:-1]
-    _tables(block_tables, context_lens, S)
+    width, stride = _tables(block_tables, context_lens, S)
     if max_context_len < 0:
         raise ValueError("max_context_len must not be negative")
-    capacity = block_tables.shape[1] * bs
+    capacity = width * bs
     L = min(int(max_context_len) or capacity, capacity)
     L = max(-(-L // 16) * 16, 16)
     if out is None:
@@ -350,8 +367,7 @@ def paged_prefill_quantized(q: torch.Tensor, cache: QuantizedKVCache, block_tabl
         pages = _identity_pages(dev, group * per_seq).data_ptr()
         scratch = torch.empty(2 * half, dtype=torch.bfloat16, device=dev)
         k_ptr = scratch.data_ptr()
-        stride = _table_stride(block_tables)
-        tables, width, lens = block_tables.data_ptr(), block_tables.shape[1], context_lens.data_ptr()
+        tables, lens = block_tables.data_ptr(), context_lens.data_ptr()
         for s in range(0, max(S, 1), group):
             n = min(group, S - s)
             _read(pool, tables + 4 * s * stride, width, stride, lens + 4 * s, k_ptr, n, L,
