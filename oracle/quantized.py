@@ -93,3 +93,21 @@ def attend(q: np.ndarray, k: np.ndarray, v: np.ndarray, first: int, scale: float
         p /= p.sum(-1, keepdims=True)
         out[:, h], mag[:, h] = p @ v[:, h // g], p @ np.abs(v[:, h // g])
     return out, mag
+
+
+def quantised_qwen3(cfg, W, num_blocks: int, block_size: int, dtype: str):
+    """An OracleQwen3 whose cache holds what a quantised one stands for."""
+    from .qwen3 import OracleQwen3
+
+    class Model(OracleQwen3):
+        def _layer(self, l, x, positions, slots, attn):
+            def rounded(l, q):
+                for cache in (self.kc[l], self.vc[l]):
+                    flat = cache.reshape(-1, *cache.shape[2:])
+                    at = np.asarray([s for s in slots if 0 <= s < flat.shape[0]], np.int64)
+                    codes, b = quantise_rows(flat[at].astype(np.float64), dtype)
+                    flat[at] = element_values(codes, dtype) * scale_values(b)[..., None]
+                return attn(l, q)
+            return super()._layer(l, x, positions, slots, rounded)
+
+    return Model(cfg, W, num_blocks, block_size)

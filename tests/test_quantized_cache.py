@@ -169,3 +169,16 @@ def test_wrapper_refuses_cpu_tensors_and_unknown_types():
         qc.paged_decode_quantized(torch.zeros(1, 4, 128, dtype=torch.bfloat16), cache,
                                   torch.zeros(1, 4, dtype=torch.int32),
                                   torch.ones(1, dtype=torch.int32))
+
+
+def test_config_refusals():
+    from vllm_b200 import Config
+    from vllm_b200.src.model_runner import check_kv_cache_dtype
+    base = dict(model="tiny", max_num_batched_tokens=64, max_num_seqs=2, num_blocks=8)
+    check_kv_cache_dtype(Config(**base, block_size=8))
+    check_kv_cache_dtype(Config(**base, block_size=16, compat=False, kv_cache_dtype="int8"))
+    for kw, msg in ((dict(block_size=16, compat=False, kv_cache_dtype="fp4"), "kv_cache_dtype"),
+                    (dict(block_size=16, kv_cache_dtype="e4m3"), "compat"),
+                    (dict(block_size=8, compat=False, kv_cache_dtype="e4m3"), "multiple of 16")):
+        with pytest.raises(ValueError, match=msg):
+            check_kv_cache_dtype(Config(**base, **kw))

@@ -40,6 +40,12 @@ class Config:
     # SiLU-mul in one, o_proj / down_proj plain; larger ones use cuBLAS and the
     # separate kernels. 0 turns the fused path off.
     fused_gemm_max_rows: int = 0
+    # Elements of the KV cache: "bf16", or "e4m3" / "int8" with one power-of-two
+    # scale per token and KV head (kernels/quantized_cache.py): 129 bytes a row
+    # instead of 256, so about twice the tokens in a pool and half the bytes of a
+    # decode step's attention. Needs compat=False (or enable_chunked_prefill) and
+    # a block_size that is a multiple of 16.
+    kv_cache_dtype: str = "bf16"
 
     @property
     def max_len(self) -> int:

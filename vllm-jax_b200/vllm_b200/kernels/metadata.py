@@ -62,6 +62,7 @@ class RangesMeta:
     sample_rows: torch.Tensor      # packed row of each sampled sequence's last token
     sample_slots: torch.Tensor     # their token-table rows
     sample_lens: torch.Tensor      # and lengths (the sampled token is stored there)
+    max_chunk_context: int = 1     # largest start + n of the sequences with n > 1
 
 
 class DeviceTables:
@@ -213,7 +214,8 @@ class DeviceTables:
                      pos.data_ptr(), sm.data_ptr(), tables.data_ptr(), cu.data_ptr(),
                      ctx.data_ptr(), self.error.data_ptr(), stream_ptr(dev))
         return RangesMeta(ids, pos, sm, tables, cu, ctx, S, total, max(ns), rows,
-                          s_slots, s_lens)
+                          s_slots, s_lens,
+                          max((a + n for a, n in zip(starts, ns) if n > 1), default=1))
 
     def build_decode(self, slots: list[int], lens: list[int], width: int,
                      last_block_slot: bool = True, out: DecodeMeta | None = None,

@@ -31,6 +31,8 @@ from ..kernels.fused import add_rmsnorm, silu_mul
 from ..kernels.gemm import TiledWeight, decode_gemm, gemm_workspace_bytes, qkv_gemm_kv_store
 from ..kernels.kv_store import kv_store_qknorm_rope
 from ..kernels.prefill_paged_attention import paged_attention_mixed, paged_prefill
+from ..kernels.quantized_cache import (QuantizedKVCache, kv_store_quantized,
+                                       paged_decode_quantized, paged_prefill_quantized)
 
 
 @dataclass
@@ -207,7 +209,8 @@ def rms_norm(x: torch.Tensor, w: torch.Tensor, eps: float) -> torch.Tensor:
 
 
 class Qwen3Model:
-    """Forward passes of one rank. kv_caches[l]: (2, num_blocks, bs, Hkv_l, D) bf16."""
+    """Forward passes of one rank. kv_caches[l]: (2, num_blocks, bs, Hkv_l, D) bf16,
+    or a QuantizedKVCache of that shape (reference_q_scaling must then be off)."""
 
     def __init__(self, weights: Qwen3Weights, process_group=None, tp_comm=None,
                  reference_q_scaling: bool = False):
@@ -291,7 +294,14 @@ class Qwen3Model:
         T = x.shape[0]
         fused = self._fused(T)
         tw = self.w.tiles[l] if fused else None
-        if fused:
+        if isinstance(kv_cache, QuantizedKVCache):
+            qkv = (decode_gemm(h, tw["qkv"], ws=self.gemm_workspace) if fused
+                   else F.linear(h, lw.w_qkv)).view(T, self.hq + 2 * self.hkv, self.d)
+            q = kv_store_quantized(qkv[:, :self.hq], qkv[:, self.hq:self.hq + self.hkv],
+                                   qkv[:, self.hq + self.hkv:], kv_cache, meta.slot_mapping,
+                                   meta.positions, lw.q_norm, lw.k_norm, eps=c.rms_norm_eps,
+                                   rope_theta=c.rope_theta, table=self.rope_table)
+        elif fused:
             # qkv projection + q/k norm + RoPE + KV store in one launch
             q = qkv_gemm_kv_store(h, tw["qkv"], kv_cache, meta.slot_mapping, meta.positions,
                                   lw.q_norm, lw.k_norm, self.hq, eps=c.rms_norm_eps,
@@ -344,6 +354,11 @@ class Qwen3Model:
         q_scale, scale = self._attn_scale("prefill")
 
         def attn(q, kv):
+            if isinstance(kv, QuantizedKVCache):
+                return paged_prefill_quantized(
+                    q, kv, meta.block_tables[:S], meta.cu_seqlens_q[:S + 1], meta.seq_lens[:S],
+                    max_seqlen_q=meta.max_seqlen_bucket, scale=scale,
+                    max_context_len=meta.max_seqlen_bucket)
             return paged_prefill(q, kv, meta.block_tables[:S], meta.cu_seqlens_q[:S + 1],
                                  getattr(meta, "context_lens", None),
                                  max_seqlen_q=meta.max_seqlen_bucket, scale=scale)
@@ -357,6 +372,8 @@ class Qwen3Model:
         q_scale, scale = self._attn_scale("decode")
 
         def attn(q, kv):
+            if isinstance(kv, QuantizedKVCache):
+                return paged_decode_quantized(q, kv, meta.block_tables, meta.context_lens, scale)
             out = paged_decode(q, kv, meta.block_tables, meta.context_lens, scale,
                                workspace=self.decode_workspace,
                                reuse_plan=bool(planned) and self.decode_workspace is not None)
@@ -365,6 +382,23 @@ class Qwen3Model:
 
         x = self._stack(x, kv_caches, meta, attn, q_scale)
         return F.linear(x, self.w.lm_head)           # compute_logits (qwen3.py:474-477)
+
+    def _mixed_quantized(self, q: torch.Tensor, kv: QuantizedKVCache, meta,
+                         nd: int) -> torch.Tensor:
+        """A chunked step's attention over a quantised cache: the prompt chunks
+        (which also zeroes the padding rows), then the decode rows."""
+        S = meta.num_seqs
+        out = torch.empty_like(q)
+        if nd < S:
+            paged_prefill_quantized(q, kv, meta.block_tables[nd:S], meta.cu_seqlens_q[nd:S + 1],
+                                    meta.context_lens[nd:S], meta.max_new, self.scale, out,
+                                    meta.max_chunk_context)
+        else:
+            out[nd:].zero_()
+        if nd:
+            paged_decode_quantized(q[:nd], kv, meta.block_tables[:nd], meta.context_lens[:nd],
+                                   self.scale, out[:nd])
+        return out
 
     def forward_mixed(self, meta, kv_caches: list[torch.Tensor], num_decode: int,
                       sample_rows: torch.Tensor) -> torch.Tensor:
@@ -380,6 +414,8 @@ class Qwen3Model:
         planned = []
 
         def attn(q, kv):
+            if isinstance(kv, QuantizedKVCache):
+                return self._mixed_quantized(q, kv, meta, nd)
             out = paged_attention_mixed(
                 q, kv, meta.block_tables[:S], meta.cu_seqlens_q[:S + 1], meta.context_lens[:S],
                 nd, meta.max_new, self.scale, workspace=self.decode_workspace,

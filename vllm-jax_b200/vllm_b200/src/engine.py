@@ -25,7 +25,7 @@ from ..config import Config
 from ..model.qwen3 import Qwen3Config, Qwen3Weights, get_config
 from ..sampling_params import SamplingParams
 from .kv_cache_manager import KVCacheManager
-from .model_runner import ModelRunner, kv_cache_bytes_per_block
+from .model_runner import ModelRunner, check_kv_cache_dtype, kv_cache_bytes_per_block
 from .request import Request
 from .scheduler import ChunkedScheduler, Scheduler
 
@@ -37,6 +37,9 @@ class Engine:
                  eos_token_id: int | None = 151645, process_group=None,
                  weights: Qwen3Weights | None = None, max_slots: int = 4096,
                  use_cuda_graphs: bool = True):
+        if config.enable_chunked_prefill and config.compat:
+            config = dataclasses.replace(config, compat=False)
+        check_kv_cache_dtype(config)
         self.config = config
         self.tokenizer = tokenizer
         self.eos_token_id = (tokenizer.eos_token_id if tokenizer is not None
@@ -81,7 +84,8 @@ class Engine:
         num_blocks = config.num_blocks
         if num_blocks <= 0:
             free, _ = torch.cuda.mem_get_info(device)
-            per = kv_cache_bytes_per_block(self.mcfg, config.block_size, self.tp_size)
+            per = kv_cache_bytes_per_block(self.mcfg, config.block_size, self.tp_size,
+                                           config.kv_cache_dtype)
             num_blocks = int(free * config.gpu_memory_utilization) // per
             if self.tp_size > 1:   # every rank must agree on the pool size
                 t = torch.tensor([num_blocks], device=device)
@@ -92,8 +96,6 @@ class Engine:
         if config.enable_prefix_caching and not config.enable_chunked_prefill:
             raise ValueError("enable_prefix_caching needs enable_chunked_prefill")
         if config.enable_chunked_prefill:
-            if config.compat:
-                self.config = config = dataclasses.replace(config, compat=False)
             if num_blocks < config.max_blocks_per_seq:
                 raise ValueError("chunked prefill needs a pool of at least max_model_len tokens")
         self.tp_comm = None

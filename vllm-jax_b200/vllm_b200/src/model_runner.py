@@ -22,15 +22,32 @@ from ..config import Config
 from ..kernels.decode_paged_attention import decode_workspace_bytes
 from ..kernels.kv_store import rope_table
 from ..kernels.metadata import DecodeMeta, DeviceTables, bucket_size
+from ..kernels.quantized_cache import CACHE_DTYPES, QuantizedKVCache
 from ..kernels.sampler import sample
 from ..model.qwen3 import Qwen3Config, Qwen3Model, Qwen3Weights
 from .kv_cache_manager import KVCacheManager
 from .request import Request
 
 
-def kv_cache_bytes_per_block(mcfg: Qwen3Config, block_size: int, tp_size: int) -> int:
+def kv_cache_bytes_per_block(mcfg: Qwen3Config, block_size: int, tp_size: int,
+                             kv_cache_dtype: str = "bf16") -> int:
+    row = mcfg.head_dim * 2 if kv_cache_dtype == "bf16" else mcfg.head_dim + 1   # and its scale
     return (mcfg.num_hidden_layers * 2 * block_size * (mcfg.num_key_value_heads // tp_size)
-            * mcfg.head_dim * 2)
+            * row)
+
+
+def check_kv_cache_dtype(config: Config) -> None:
+    """ValueError unless config.kv_cache_dtype can be used with its other fields."""
+    if config.kv_cache_dtype == "bf16":
+        return
+    if config.kv_cache_dtype not in CACHE_DTYPES:
+        raise ValueError(f"kv_cache_dtype must be 'bf16' or one of {sorted(CACHE_DTYPES)}; got "
+                         f"{config.kv_cache_dtype!r}")
+    if config.compat:
+        raise ValueError("a quantised KV cache needs compat=False: compat follows the "
+                         "reference's bf16 arithmetic and its wrap of negative slots")
+    if config.block_size % 16:
+        raise ValueError("a quantised KV cache needs a block_size that is a multiple of 16")
 
 
 class PendingTokens:
@@ -91,10 +108,16 @@ class ModelRunner:
         if config.fused_gemm_max_rows > 0:
             self.model.enable_fused_gemm(config.fused_gemm_max_rows)
         hkv = model_cfg.num_key_value_heads // tp_size
+        check_kv_cache_dtype(config)
         shape = (2, kv_cache_manager.num_blocks, config.block_size, hkv, model_cfg.head_dim)
         # zero-initialised like the reference's pool (model_runner.py:190-199)
-        self.kv_caches = [torch.zeros(shape, dtype=torch.bfloat16, device=device)
-                          for _ in range(model_cfg.num_hidden_layers)]
+        if config.kv_cache_dtype == "bf16":
+            self.kv_caches = [torch.zeros(shape, dtype=torch.bfloat16, device=device)
+                              for _ in range(model_cfg.num_hidden_layers)]
+        else:
+            self.kv_caches = [QuantizedKVCache.zeros(*shape[1:], dtype=config.kv_cache_dtype,
+                                                     device=device)
+                              for _ in range(model_cfg.num_hidden_layers)]
         self.tables = DeviceTables(max_slots, config.max_len, self.width, config.block_size,
                                    device)
         self.free_slots = list(range(max_slots - 1, -1, -1))
