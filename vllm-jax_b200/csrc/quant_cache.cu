@@ -640,7 +640,14 @@ extern "C" vj_status vj_kv_store_quantized(
   a.Hkv = num_kv_heads;
   a.eps = eps;
   a.err = error_flag;
-  build_rope_table(rope_theta, a.freq.inv_freq);
+  // 64 powers on the host take longer than the launch: kept for the last theta
+  static thread_local float freq_theta = -1.0f;
+  static thread_local RopeTable freq;
+  if (rope_theta != freq_theta) {
+    build_rope_table(rope_theta, freq.inv_freq);
+    freq_theta = rope_theta;
+  }
+  a.freq = freq;
   // units of 32 rows; smaller ones while those would leave half the warps without
   // one (257 tokens of 48 rows: 5.3 us; down to one for every warp 6.2)
   const int64_t warps = static_cast<int64_t>(num_sms()) * kStoreCtas * kStoreWarps;

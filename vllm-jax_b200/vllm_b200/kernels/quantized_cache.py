@@ -16,24 +16,22 @@ include/vjattn.h) has no counterpart there.
 """
 from __future__ import annotations
 
-import contextlib
 import functools
 import math
-from dataclasses import dataclass
+from typing import NamedTuple
 
 import torch
 
 from .. import _native
-from ._util import require_cuda, require_dtype, stream_ptr
+from ._util import require_cuda, require_dtype
 from .kv_store import rope_table
-from .prefill_paged_attention import _err_flag
+from .prefill_paged_attention import _err_flag, _err_flags
 
 CACHE_DTYPES = {"e4m3": torch.float8_e4m3fn, "int8": torch.int8}
 _CODES = {torch.float8_e4m3fn: _native.VJ_CACHE_E4M3, torch.int8: _native.VJ_CACHE_INT8}
 
 
-@dataclass(frozen=True)
-class QuantizedKVCache:
+class QuantizedKVCache(NamedTuple):
     """A layer's pool: `data` (2, num_blocks, block_size, Hkv, head_dim)
     float8_e4m3fn or int8, and `scales` (2, num_blocks, Hkv, block_size) uint8,
     the E8M0 byte of each row: a row stands for data * 2^(scales - 127). Any
@@ -80,14 +78,35 @@ def _pool(cache: QuantizedKVCache):
     return (d, d + s2, s, s + c2), code, hkv, D, nb, bs, (sb, st, sh, cb, ch)
 
 
-_HERE = contextlib.nullcontext()
+def _index(*tensors: torch.Tensor | None) -> int:
+    """The CUDA device all tensors are on."""
+    index = -1
+    for t in tensors:
+        if t is not None:
+            i = t.get_device()
+            if i != index or i < 0:
+                if index >= 0 or i < 0:
+                    require_cuda(*tensors)       # raises
+                index = i
+    return index
 
 
-def _device(dev: torch.device):
-    """The C entries launch on the current device: make it the tensors'."""
-    if dev.index is None or dev.index == torch._C._cuda_getDevice():
-        return _HERE
-    return torch.cuda.device(dev)
+def _call(index: int, name: str, *args) -> None:
+    """A C entry on the tensors' device (it launches on the current one)."""
+    if index == torch._C._cuda_getDevice():
+        _native.call(name, *args)
+    else:
+        with torch.cuda.device(index):
+            _native.call(name, *args)
+
+
+def _error(index: int) -> int:
+    t = _err_flags.get(index)
+    return (_err_flag(torch.device("cuda", index)) if t is None else t).data_ptr()
+
+
+def _stream(index: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def _rows(t: torch.Tensor, name: str, T: int, D: int) -> tuple[int, int]:
@@ -129,8 +148,8 @@ def kv_store_quantized(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor,
     v to 8 bits once (kv_store_qknorm_rope rounds after every step, as the
     reference does). Slots outside the pool store nothing (there is no wrap of
     negative ones); the others must differ from each other within a call."""
-    dev = require_cuda(k, v, cache.data, cache.scales, slot_mapping, q, positions, q_norm_weight,
-                       k_norm_weight, q_out, table)
+    dev = _index(k, v, cache.data, cache.scales, slot_mapping, q, positions, q_norm_weight,
+                 k_norm_weight, q_out, table)
     ptrs, code, Hkv, D, nb, bs, strides = _pool(cache)
     T = k.shape[0]
     if v.shape != k.shape:
@@ -145,7 +164,7 @@ def kv_store_quantized(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor,
     if q is not None:
         Hq, q_stride = _rows(q, "q", T, D)
         if q_out is None:
-            q_out = torch.empty((T, Hq, D), dtype=torch.bfloat16, device=dev)
+            q_out = k.new_empty((T, Hq, D))
             out_stride = Hq * D
         else:
             out_heads, out_stride = _rows(q_out, "q_out", T, D)
@@ -170,18 +189,17 @@ def kv_store_quantized(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor,
         _indices(positions, "positions", T)
         pos_ptr = positions.data_ptr()
         if table is None:
-            table = rope_table(dev, rope_theta)
+            table = rope_table(k.device, rope_theta)
         require_dtype(table, torch.int32, "table")
         if not table.is_contiguous():
             raise ValueError("table must be contiguous")
         tab_len = table.numel() // 64
         if tab_len:
             table_ptr = table.data_ptr()
-    with _device(dev):
-        _native.call("vj_kv_store_quantized", q_ptr, k.data_ptr(), v.data_ptr(), qw_ptr, kw_ptr,
-                     pos_ptr, slot_mapping.data_ptr(), out_ptr, *ptrs, code, T, Hq, Hkv, D, nb, bs,
-                     *strides, q_stride, k_stride, v_stride, out_stride, table_ptr, tab_len, eps,
-                     rope_theta, flags, _err_flag(dev).data_ptr(), stream_ptr(dev))
+    _call(dev, "vj_kv_store_quantized", q_ptr, k.data_ptr(), v.data_ptr(), qw_ptr, kw_ptr,
+          pos_ptr, slot_mapping.data_ptr(), out_ptr, *ptrs, code, T, Hq, Hkv, D, nb, bs, *strides,
+          q_stride, k_stride, v_stride, out_stride, table_ptr, tab_len, eps, rope_theta, flags,
+          _error(dev), _stream(dev))
     return q_out
 
 
@@ -213,7 +231,7 @@ def paged_decode_quantized(q: torch.Tensor, cache: QuantizedKVCache, block_table
     sequence's context are not used, whatever they hold. `workspace` (uint8,
     decode_quantized_workspace_bytes(...) long): the split's scratch; by
     default a fresh allocation of the call's own."""
-    dev = require_cuda(q, cache.data, cache.scales, block_tables, context_lens, out, workspace)
+    dev = _index(q, cache.data, cache.scales, block_tables, context_lens, out, workspace)
     ptrs, code, Hkv, D, nb, bs, strides = _pool(cache)
     require_dtype(q, torch.bfloat16, "q")
     if q.dim() != 3 or not q.is_contiguous():
@@ -228,23 +246,22 @@ def paged_decode_quantized(q: torch.Tensor, cache: QuantizedKVCache, block_table
         raise ValueError("out must be a contiguous bf16 tensor of q's shape")
     if scale is None:
         scale = 1.0 / math.sqrt(D)
-    with _device(dev):
-        need = _decode_workspace_bytes(dev.index, B, Hq, Hkv, D, width, bs)
-        if workspace is None:
-            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-        elif workspace.dtype != torch.uint8 or workspace.numel() < need \
-                or not workspace.is_contiguous():
-            raise ValueError(f"decode workspace must be contiguous uint8 with >= {need} bytes")
-        _native.call("vj_paged_decode_quantized", q.data_ptr(), *ptrs, code,
-                     block_tables.data_ptr(), context_lens.data_ptr(), out.data_ptr(), B, Hq, Hkv,
-                     D, nb, bs, width, stride, *strides, scale, workspace.data_ptr(), workspace.numel(),
-                     _err_flag(dev).data_ptr(), stream_ptr(dev))
+    need = _decode_workspace_bytes(dev, B, Hq, Hkv, D, width, bs)
+    if workspace is None:
+        workspace = q.new_empty(need, dtype=torch.uint8)
+    elif workspace.dtype != torch.uint8 or workspace.numel() < need \
+            or not workspace.is_contiguous():
+        raise ValueError(f"decode workspace must be contiguous uint8 with >= {need} bytes")
+    _call(dev, "vj_paged_decode_quantized", q.data_ptr(), *ptrs, code, block_tables.data_ptr(),
+          context_lens.data_ptr(), out.data_ptr(), B, Hq, Hkv, D, nb, bs, width, stride, *strides,
+          scale, workspace.data_ptr(), workspace.numel(), _error(dev), _stream(dev))
     return out
 
 
 @functools.lru_cache(maxsize=1024)
-def _decode_workspace_bytes(device_index, *sizes: int) -> int:
-    return int(_native.load().vj_paged_decode_quantized_workspace_size(*sizes))
+def _decode_workspace_bytes(index: int, *sizes: int) -> int:
+    with torch.cuda.device(index):       # the split goes by the device's SMs
+        return int(_native.load().vj_paged_decode_quantized_workspace_size(*sizes))
 
 
 def decode_quantized_workspace_bytes(batch: int, num_q_heads: int, num_kv_heads: int,
@@ -256,13 +273,13 @@ def decode_quantized_workspace_bytes(batch: int, num_q_heads: int, num_kv_heads:
                                    head_dim, table_width, block_size)
 
 
-def _read(pool, tables: int, width: int, stride: int, lens: int, out: int, B: int, max_len: int,
-          zero_to: int, stream: int) -> None:
+def _read(index: int, pool, tables: int, width: int, stride: int, lens: int, out: int, B: int,
+          max_len: int, zero_to: int) -> None:
     """vj_kv_read_quantized into packed K, then V, at address `out`."""
     ptrs, code, Hkv, D, nb, bs, strides = pool
-    _native.call("vj_kv_read_quantized", *ptrs, code, tables, lens, out,
-                 out + B * max_len * Hkv * D * 2, B, max_len, zero_to, Hkv, D, nb, bs, width,
-                 stride, *strides, stream)
+    _call(index, "vj_kv_read_quantized", *ptrs, code, tables, lens, out,
+          out + B * max_len * Hkv * D * 2, B, max_len, zero_to, Hkv, D, nb, bs, width, stride,
+          *strides, _stream(index))
 
 
 def read_kv_cache(cache: QuantizedKVCache, block_tables: torch.Tensor,
@@ -272,7 +289,7 @@ def read_kv_cache(cache: QuantizedKVCache, block_tables: torch.Tensor,
     sequence b is its cached position t, exactly (a scale is a power of two),
     and zeros from context_lens[b] on. max_context_len: rows per sequence
     (default: what a block table row holds); longer contexts are cut there."""
-    dev = require_cuda(cache.data, cache.scales, block_tables, context_lens, out)
+    dev = _index(cache.data, cache.scales, block_tables, context_lens, out)
     pool = _pool(cache)
     _, _, Hkv, D, _, bs, _ = pool
     B = block_tables.shape[0]
@@ -282,12 +299,11 @@ def read_kv_cache(cache: QuantizedKVCache, block_tables: torch.Tensor,
     L = int(max_context_len) or width * bs
     shape = (2, B, L, Hkv, D)
     if out is None:
-        out = torch.empty(shape, dtype=torch.bfloat16, device=dev)
+        out = cache.data.new_empty(shape, dtype=torch.bfloat16)
     elif out.shape != shape or out.dtype != torch.bfloat16 or not out.is_contiguous():
         raise ValueError(f"out must be a contiguous bf16 tensor of shape {shape}")
-    with _device(dev):
-        _read(pool, block_tables.data_ptr(), width, stride, context_lens.data_ptr(),
-              out.data_ptr(), B, L, 0, stream_ptr(dev))
+    _read(dev, pool, block_tables.data_ptr(), width, stride, context_lens.data_ptr(),
+          out.data_ptr(), B, L, 0)
     return out
 
 
@@ -332,7 +348,7 @@ def paged_prefill_quantized(q: torch.Tensor, cache: QuantizedKVCache, block_tabl
     of once per query tile. max_context_len: a bound on context_lens (default:
     what a block table row holds); it sizes the scratch, as max_seqlen_q sizes
     the grid."""
-    dev = require_cuda(q, cache.data, cache.scales, block_tables, cu_seqlens_q, context_lens, out)
+    dev = _index(q, cache.data, cache.scales, block_tables, cu_seqlens_q, context_lens, out)
     pool = _pool(cache)
     _, _, Hkv, D, _, bs, _ = pool
     require_dtype(q, torch.bfloat16, "q")
@@ -362,18 +378,16 @@ def paged_prefill_quantized(q: torch.Tensor, cache: QuantizedKVCache, block_tabl
     T, Hq, _ = q.shape
     per_seq = L // 16                  # page p of the group's sequence b: block b * per_seq + p
     half = group * L * Hkv * D         # elements of the scratch's K, and of its V
-    with _device(dev):
-        stream = stream_ptr(dev)
-        pages = _identity_pages(dev, group * per_seq).data_ptr()
-        scratch = torch.empty(2 * half, dtype=torch.bfloat16, device=dev)
-        k_ptr = scratch.data_ptr()
-        tables, lens = block_tables.data_ptr(), context_lens.data_ptr()
-        for s in range(0, max(S, 1), group):
-            n = min(group, S - s)
-            _read(pool, tables + 4 * s * stride, width, stride, lens + 4 * s, k_ptr, n, L,
-                  _KEY_TILE, stream)
-            _native.call("vj_paged_prefill", q.data_ptr(), k_ptr, k_ptr + n * L * Hkv * D * 2, pages,
-                         cu_seqlens_q.data_ptr() + 4 * s, lens + 4 * s, out.data_ptr(), T, n, Hq,
-                         Hkv, D, max(n, 1) * per_seq, 16, per_seq, per_seq, 16 * Hkv * D, Hkv * D, D,
-                         int(max_seqlen_q), float(scale), _err_flag(dev).data_ptr(), stream)
+    pages = _identity_pages(q.device, group * per_seq).data_ptr()
+    scratch = q.new_empty(2 * half)
+    k_ptr = scratch.data_ptr()
+    tables, lens = block_tables.data_ptr(), context_lens.data_ptr()
+    for s in range(0, max(S, 1), group):
+        n = min(group, S - s)
+        _read(dev, pool, tables + 4 * s * stride, width, stride, lens + 4 * s, k_ptr, n, L,
+              _KEY_TILE)
+        _call(dev, "vj_paged_prefill", q.data_ptr(), k_ptr, k_ptr + n * L * Hkv * D * 2, pages,
+              cu_seqlens_q.data_ptr() + 4 * s, lens + 4 * s, out.data_ptr(), T, n, Hq, Hkv, D,
+              max(n, 1) * per_seq, 16, per_seq, per_seq, 16 * Hkv * D, Hkv * D, D,
+              int(max_seqlen_q), scale, _error(dev), _stream(dev))
     return out

@@ -373,7 +373,8 @@ class Qwen3Model:
 
         def attn(q, kv):
             if isinstance(kv, QuantizedKVCache):
-                return paged_decode_quantized(q, kv, meta.block_tables, meta.context_lens, scale)
+                return paged_decode_quantized(q, kv, meta.block_tables, meta.context_lens, scale,
+                                              workspace=self.decode_workspace)
             out = paged_decode(q, kv, meta.block_tables, meta.context_lens, scale,
                                workspace=self.decode_workspace,
                                reuse_plan=bool(planned) and self.decode_workspace is not None)
@@ -397,7 +398,7 @@ class Qwen3Model:
             out[nd:].zero_()
         if nd:
             paged_decode_quantized(q[:nd], kv, meta.block_tables[:nd], meta.context_lens[:nd],
-                                   self.scale, out[:nd])
+                                   self.scale, out[:nd], self.decode_workspace)
         return out
 
     def forward_mixed(self, meta, kv_caches: list[torch.Tensor], num_decode: int,

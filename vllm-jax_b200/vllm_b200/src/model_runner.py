@@ -22,7 +22,8 @@ from ..config import Config
 from ..kernels.decode_paged_attention import decode_workspace_bytes
 from ..kernels.kv_store import rope_table
 from ..kernels.metadata import DecodeMeta, DeviceTables, bucket_size
-from ..kernels.quantized_cache import CACHE_DTYPES, QuantizedKVCache
+from ..kernels.quantized_cache import (CACHE_DTYPES, QuantizedKVCache,
+                                       decode_quantized_workspace_bytes)
 from ..kernels.sampler import sample
 from ..model.qwen3 import Qwen3Config, Qwen3Model, Qwen3Weights
 from .kv_cache_manager import KVCacheManager
@@ -100,15 +101,18 @@ class ModelRunner:
         self.model.rope_table = rope_table(device, model_cfg.rope_theta, config.max_len + 1)
         # one decode workspace for the largest batch bucket, allocated before
         # any graph capture and never replaced
-        self.model.decode_workspace = torch.empty(
-            max(decode_workspace_bytes(bucket_size(max(config.max_num_seqs, 1)),
-                                       model_cfg.num_attention_heads // tp_size,
-                                       model_cfg.head_dim), 16),
-            dtype=torch.uint8, device=device)
+        check_kv_cache_dtype(config)
+        rows, hq = bucket_size(max(config.max_num_seqs, 1)), model_cfg.num_attention_heads // tp_size
+        hkv = model_cfg.num_key_value_heads // tp_size
+        if config.kv_cache_dtype == "bf16":
+            ws_bytes = decode_workspace_bytes(rows, hq, model_cfg.head_dim)
+        else:
+            ws_bytes = decode_quantized_workspace_bytes(rows, hq, hkv, self.width,
+                                                        config.block_size, model_cfg.head_dim)
+        self.model.decode_workspace = torch.empty(max(ws_bytes, 16), dtype=torch.uint8,
+                                                  device=device)
         if config.fused_gemm_max_rows > 0:
             self.model.enable_fused_gemm(config.fused_gemm_max_rows)
-        hkv = model_cfg.num_key_value_heads // tp_size
-        check_kv_cache_dtype(config)
         shape = (2, kv_cache_manager.num_blocks, config.block_size, hkv, model_cfg.head_dim)
         # zero-initialised like the reference's pool (model_runner.py:190-199)
         if config.kv_cache_dtype == "bf16":
