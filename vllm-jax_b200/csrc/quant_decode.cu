@@ -808,16 +808,17 @@ quant_decode_kernel(const __grid_constant__ CUtensorMap tmk,
 // Joins the partial results of sequences that several units (or ranges and
 // pieces) shared, and writes
 // the zeros of empty ones. kSplit warps take a (sequence, query head), each
-// every kSplit-th partial, 8 of them in flight: as many warps as fit the GPU at
-// once, since a row's time is its chain of memory round trips. Launched while
+// every kSplit-th partial, several of them in flight: as many warps as fit the
+// GPU at once, since a row's time is its chain of memory round trips. Launched while
 // the decode kernel runs and held by griddepcontrol until that is done.
-constexpr int kCombineWarps = 8;
+template <int kSplit>
+constexpr int kCombineWarps = kSplit > 8 ? kSplit : 8;
 
 template <int kSplit>
-__global__ void __launch_bounds__(kCombineWarps * 32) quant_combine_kernel(const QDecodeArgs a) {
-  constexpr int kRows = kCombineWarps / kSplit, kFly = 8;
-  __shared__ float4 so[kCombineWarps][32];
-  __shared__ float sm[kCombineWarps], sl[kCombineWarps];
+__global__ void __launch_bounds__(kCombineWarps<kSplit> * 32) quant_combine_kernel(const QDecodeArgs a) {
+  constexpr int kWarps = kCombineWarps<kSplit>, kRows = kWarps / kSplit, kFly = kSplit > 8 ? 4 : 8;
+  __shared__ float4 so[kWarps][32];
+  __shared__ float sm[kWarps], sl[kWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int part = warp % kSplit;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + warp / kSplit;
@@ -889,10 +890,10 @@ __global__ void __launch_bounds__(kCombineWarps * 32) quant_combine_kernel(const
 
 template <int kSplit>
 int launch_combine(const QDecodeArgs &a, int64_t rows, cudaStream_t stream) {
-  constexpr int kRows = kCombineWarps / kSplit;
+  constexpr int kRows = kCombineWarps<kSplit> / kSplit;
   return launch_dependent("vj_paged_decode_quantized", quant_combine_kernel<kSplit>,
                           dim3(static_cast<unsigned>((rows + kRows - 1) / kRows)),
-                          kCombineWarps * 32, 0, stream, a);
+                          kCombineWarps<kSplit> * 32, 0, stream, a);
 }
 
 template <bool kInt8, int NT>
@@ -1067,7 +1068,8 @@ extern "C" vj_status vj_paged_decode_quantized(
   const int64_t rows = static_cast<int64_t>(batch) * num_q_heads;
   // warps that can be resident at once: 32 an SM at this kernel's registers
   const int64_t room = 32ll * num_sms();
-  rc = rows * 8 <= room ? launch_combine<8>(a, rows, stream)
+  rc = rows * 32 <= room  ? launch_combine<32>(a, rows, stream)
+       : rows * 8 <= room ? launch_combine<8>(a, rows, stream)
        : rows * 4 <= room ? launch_combine<4>(a, rows, stream)
        : rows * 2 <= room ? launch_combine<2>(a, rows, stream)
                           : launch_combine<1>(a, rows, stream);
