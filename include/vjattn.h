@@ -522,7 +522,8 @@ VJ_API vj_status vj_kv_read_quantized(
     int64_t scale_stride_block, int64_t scale_stride_head, cudaStream_t stream);
 
 /* vj_paged_decode over the quantised cache: q, out [B,Hq,D] bf16, at most 16
- * query heads per KV head. stride_block must equal block_size*stride_token.
+ * query heads per KV head. stride_block must equal block_size*stride_token; K
+ * and V (and their scales) may lie anywhere less than 2^40 bytes apart.
  * Cached rows past a sequence's context are never used, whatever they hold.
  *   workspace: vj_paged_decode_quantized_workspace_size(B, Hq, Hkv, D, bt_width,
  *   block_size) bytes on the current device, 16-byte aligned, need not be initialised; calls whose kernels may overlap

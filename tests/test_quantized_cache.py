@@ -132,6 +132,9 @@ def test_refusals_of_every_entry(entry, kw, status, msg):
     (_decode, dict(ws=None), "WORKSPACE", b"workspace"),
     (_decode, dict(ws=8), "WORKSPACE", b"workspace"),
     (_decode, dict(wsb=16), "WORKSPACE", b"workspace"),
+    (_decode, dict(), "INVALID_ARGUMENT", b"same memory"),
+    (_decode, dict(vc=32, vs=16), "INVALID_ARGUMENT", b"same memory"),
+    (_decode, dict(vc=16 + (1 << 40), vs=32), "UNSUPPORTED", b"2^40"),
     (_read, dict(B=-1), "INVALID_ARGUMENT", b"size"),
     (_read, dict(L=-1), "INVALID_ARGUMENT", b"size"),
     (_read, dict(z=-1), "INVALID_ARGUMENT", b"size"),

@@ -33,8 +33,10 @@
 // join, and there is one launch (17 tokens: 5.7 us against 7.5; at 125 pages, 16 a
 // warp, it would be 21 against 11).
 //
-// A warp streams its pages through a ring of its own in shared memory: TMA
-// boxes of 16 rows x 128 bytes (128-byte swizzle) and the rows' scale bytes.
+// A warp streams its pages through a ring of its own in shared memory: one TMA
+// box of 16 rows x 128 bytes of K and of V (128-byte swizzle; the distance from
+// the one to the other is the box's fourth dimension) and one of their scale
+// bytes. Issuing takes a quarter of the instructions as it is.
 // Where a page lies is looked up for 32 pages at once, a page a lane, and that
 // lane issues its copies; so the walk (sequence ends, block tables, addresses)
 // costs a page next to nothing. Products run on mma.sync m16n8k16 in f16 with
@@ -69,6 +71,7 @@ using namespace qn;
 constexpr int kTok = 16;                      // tokens per page
 constexpr int kHalf = kTok * kD;              // bytes of a page's K (or V) rows
 constexpr int kStage = 2 * kHalf;
+constexpr int kScaleStage = 128;              // 32 bytes; a TMA destination is 128-byte aligned
 constexpr int kStart = 3;                     // places in front of a sequence's pages
 constexpr int kWhole = 32;                    // pages up to which a unit takes a sequence
 constexpr int kDealt = 32;                    // pages a warp from which on a part is dealt
@@ -79,8 +82,7 @@ constexpr float kUp = 4.0f;                   // log2 of the weight at the maxim
 struct Page {
   int b;             // sequence
   int valid_flags;   // tokens inside the context (1..16), and kFirst.. below << 8
-  int tok;           // first token's place in the pool
-  int64_t scale;     // offset of its scale bytes
+  int tok, blk;      // first token's place in the pool, its block
 };
 // What the consumer of a stage needs to know of it.
 struct Info {
@@ -123,7 +125,7 @@ struct Shape {                                // NT tiles of 8 query heads
   static constexpr int kUnits = kWarps / kUnit;
   static constexpr int kHeads = NT * 8;
   // pages, scale bytes, barriers, left records, scan
-  static constexpr size_t kSmem = 1024 + (size_t)kRing * (kStage + 32 + sizeof(Info) + 8) +
+  static constexpr size_t kSmem = 1024 + (size_t)kRing * (kStage + kScaleStage + sizeof(Info) + 8) +
                                   kWarps * sizeof(Left) + kUnits * (sizeof(Split) + sizeof(Place)) +
                                   (kThreads + kWarps) * 4;
   // a record in a warp's ring: kHeads x 128 outputs, kHeads (maximum, sum)
@@ -160,9 +162,9 @@ struct QDecodeArgs {
   const __nv_bfloat16 *q;
   __nv_bfloat16 *out;
   const int32_t *bt, *lens;
-  const uint8_t *ks, *vs;
-  int64_t ssb, ssh;
-  int B, Hq, Hkv, g, bt_stride, pages_per_block, ppb_shift, block_size, max_pages, num_blocks, head_major;
+  int B, Hq, Hkv, g, bt_stride, pages_per_block, ppb_shift, block_size, max_pages, num_blocks;
+  int head_major;     // order of the pages' outer dimensions: heads, tokens
+  int v_half, v_scale_half;   // where V's rows and scales lie in a stage: 0 first, 1 second
   int unit;           // warps of a unit
   int groups;         // warps that serve a KV head, a multiple of unit
   int whole;          // whether a unit takes a whole sequence
@@ -278,8 +280,8 @@ VJ_DEV Place locate(const QDecodeArgs &a, const int *scan, int per, int s) {
 
 template <bool kInt8, int NT>
 __global__ void __launch_bounds__(Shape<NT>::kThreads, 1)
-quant_decode_kernel(const __grid_constant__ CUtensorMap tmk,
-                    const __grid_constant__ CUtensorMap tmv, const QDecodeArgs a) {
+quant_decode_kernel(const __grid_constant__ CUtensorMap tm_rows,
+                    const __grid_constant__ CUtensorMap tm_scales, const QDecodeArgs a) {
   using S = Shape<NT>;
   constexpr int kStages = S::kStages, kUnit = S::kUnit;
   extern __shared__ uint8_t smem_raw[];
@@ -287,7 +289,7 @@ quant_decode_kernel(const __grid_constant__ CUtensorMap tmk,
                                               ~uintptr_t(1023));
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   uint8_t *scales = smem + S::kRing * kStage;
-  Info *infos = reinterpret_cast<Info *>(scales + S::kRing * 32);
+  Info *infos = reinterpret_cast<Info *>(scales + S::kRing * kScaleStage);
   uint64_t *full = reinterpret_cast<uint64_t *>(infos + S::kRing);
   Left *lefts = reinterpret_cast<Left *>(full + S::kRing);
   Split *splits = reinterpret_cast<Split *>(lefts + S::kWarps);     // [kUnits]
@@ -298,7 +300,7 @@ quant_decode_kernel(const __grid_constant__ CUtensorMap tmk,
   if (lane == 0) {
     for (int s = 0; s < kStages; ++s) mbar_init(&full[warp * kStages + s], 1);
     fence_mbar_init();
-    if (warp == 0) { tma_prefetch_desc(&tmk); tma_prefetch_desc(&tmv); }
+    if (warp == 0) { tma_prefetch_desc(&tm_rows); tma_prefetch_desc(&tm_scales); }
   }
   // nothing of the caller's is read before the kernel ahead is done; the
   // combine kernel may be made ready as soon as every CTA of this one runs
@@ -380,7 +382,7 @@ quant_decode_kernel(const __grid_constant__ CUtensorMap tmk,
   const int G = SG * kUnit + warp % kUnit;
   const int r = lane >> 2, qd = lane & 3;
   uint8_t *const my_ring = smem + warp * kStages * kStage;
-  uint8_t *const my_scales = scales + warp * kStages * 32;
+  uint8_t *const my_scales = scales + warp * kStages * kScaleStage;
   Info *const my_info = infos + warp * kStages;
   uint64_t *const my_full = full + warp * kStages;
 
@@ -455,7 +457,7 @@ quant_decode_kernel(const __grid_constant__ CUtensorMap tmk,
               ((w.p == 0 || at == seg_first ? kFirst : 0) | (seq_end || end ? kLast : 0) |
                (at - w.p >= seg_first ? kHead : 0) | (seq_end ? kTail : 0) | (end ? kEnd : 0)) << 8;
           page.tok = blk * a.block_size + off;
-          page.scale = blk * a.ssb + seg_h * a.ssh + off;
+          page.blk = blk;
         }
       }
       there = __ballot_sync(0xffffffffu, has_page);
@@ -468,10 +470,9 @@ quant_decode_kernel(const __grid_constant__ CUtensorMap tmk,
       uint8_t *dst = my_ring + s * kStage;
       mbar_arrive_expect_tx(&my_full[s], kStage + 32);
       const int c1 = a.head_major ? seg_h : page.tok, c2 = a.head_major ? page.tok : seg_h;
-      tma_load_3d(dst, &tmk, &my_full[s], 0, c1, c2);
-      tma_load_3d(dst + kHalf, &tmv, &my_full[s], 0, c1, c2);
-      bulk_g2s(my_scales + s * 32, a.ks + page.scale, 16, &my_full[s]);
-      bulk_g2s(my_scales + s * 32 + 16, a.vs + page.scale, 16, &my_full[s]);
+      tma_load_4d(dst, &tm_rows, &my_full[s], 0, c1, c2, 0);
+      tma_load_4d(my_scales + s * kScaleStage, &tm_scales, &my_full[s],
+                  page.tok - page.blk * a.block_size, seg_h, page.blk, 0);
     }
     ++issued;
   };
@@ -480,6 +481,7 @@ quant_decode_kernel(const __grid_constant__ CUtensorMap tmk,
   if (!a.whole) tell_combine();         // while the pages travel
 
   const uint32_t ring = smem_u32(my_ring), sc_ring = smem_u32(my_scales);
+  const uint32_t v_rows = a.v_half ? kHalf : 0, v_scales = a.v_scale_half ? 16 : 0;
   uint32_t qf[NT][16];                  // Q^T fragments: dims 32*qd + 4*j + {0,1}, {2,3}
   float qs[NT][2];                      // score factor of heads 2*qd, 2*qd + 1
   float acc[NT][8][4];                  // O^T: dims 16*r + 2*i, + 1; heads 2*qd, 2*qd + 1
@@ -539,7 +541,9 @@ quant_decode_kernel(const __grid_constant__ CUtensorMap tmk,
     }
     const Info info = my_info[stage];
     const int seq = info.b, valid = info.valid_flags & 0xff, flags = info.valid_flags >> 8;
-    const uint32_t kb = ring + stage * kStage, vb = kb + kHalf, sb = sc_ring + stage * 32;
+    const uint32_t kb = ring + stage * kStage + (kHalf - v_rows), vb = ring + stage * kStage + v_rows;
+    const uint32_t ksb = sc_ring + stage * kScaleStage + (16 - v_scales);
+    const uint32_t vsb = sc_ring + stage * kScaleStage + v_scales;
     if (it > 0 && (flags & kFirst)) begin(seq, info.h);
     // ---- S^T = K Q^T, two chains of sums
     float sc[NT][4];
@@ -565,15 +569,15 @@ quant_decode_kernel(const __grid_constant__ CUtensorMap tmk,
         }
       }
       // tokens r, r + 8 (heads 2*qd, + 1 each), times the rows' scales
-      const float ks0 = __uint_as_float(max(lds8(sb + r) << 23, 0x00400000u));
-      const float ks1 = __uint_as_float(max(lds8(sb + r + 8) << 23, 0x00400000u));
+      const float ks0 = __uint_as_float(max(lds8(ksb + r) << 23, 0x00400000u));
+      const float ks1 = __uint_as_float(max(lds8(ksb + r + 8) << 23, 0x00400000u));
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) sc[t][j] = (sa[t][j] + sz[t][j]) * (j < 2 ? ks0 : ks1);
       }
     }
-    const uint32_t vb0 = lds8(sb + 16 + r), vb1 = lds8(sb + 24 + r);
+    const uint32_t vb0 = lds8(vsb + r), vb1 = lds8(vsb + r + 8);
     const float ev0 = vb0 == 255u ? __uint_as_float(0x7fffffffu)
                                   : __uint_as_float(0x4b000000u | vb0) - 8388735.0f;   // vb0 - 127
     const float ev1 = vb1 == 255u ? __uint_as_float(0x7fffffffu)
@@ -897,7 +901,7 @@ int launch_combine(const QDecodeArgs &a, int64_t rows, cudaStream_t stream) {
 }
 
 template <bool kInt8, int NT>
-int launch_decode(const CUtensorMap &tmk, const CUtensorMap &tmv, const QDecodeArgs &a, int grid,
+int launch_decode(const CUtensorMap &tm_rows, const CUtensorMap &tm_scales, const QDecodeArgs &a, int grid,
                   cudaStream_t stream) {
   using S = Shape<NT>;
   static_assert(S::kSmem <= 227 * 1024, "shared memory");
@@ -916,8 +920,8 @@ int launch_decode(const CUtensorMap &tmk, const CUtensorMap &tmv, const QDecodeA
                      std::string("vj_paged_decode_quantized: ") + cudaGetErrorString(e));
   }
   return launch_dependent("vj_paged_decode_quantized", quant_decode_kernel<kInt8, NT>,
-                          dim3(static_cast<unsigned>(grid)), S::kThreads, S::kSmem, stream, tmk,
-                          tmv, a);
+                          dim3(static_cast<unsigned>(grid)), S::kThreads, S::kSmem, stream, tm_rows,
+                          tm_scales, a);
 }
 
 // Grid, warps of a unit and groups, from head counts and the GPU's size alone.
@@ -1016,27 +1020,43 @@ extern "C" vj_status vj_paged_decode_quantized(
     return set_error(VJ_ERR_WORKSPACE, what + ": workspace needs " + std::to_string(need) +
                                            " bytes, 16-byte aligned");
   }
-  CUtensorMap tmk, tmv;
-  const uint64_t ntok = static_cast<uint64_t>(num_blocks) * block_size;
-  // the two outer dims in the order of their strides
-  const bool head_major = stride_head < stride_token;
-  for (int i = 0; i < 2; ++i) {
-    CUtensorMap *m = i ? &tmv : &tmk;
-    const void *base = i ? v_cache : k_cache;
-    rc = head_major ? encode_tmap_3d_u8(m, base, kD, num_kv_heads, ntok, stride_head, stride_token,
-                                        kD, 1, kTok, true)
-                    : encode_tmap_3d_u8(m, base, kD, ntok, num_kv_heads, stride_token, stride_head,
-                                        kD, kTok, 1, true);
-    if (rc) return rc;
+  // one map for the rows of K and V, one for their scales: the fourth dimension
+  // leads from the lower address to the higher one
+  CUtensorMap tm_rows, tm_scales;
+  const uint64_t ntok = static_cast<uint64_t>(num_blocks) * block_size, hkv = num_kv_heads;
+  const bool head_major = stride_head < stride_token;    // outer dims in the order of strides
+  auto apart = [](const void *x, const void *y) {
+    const auto p = reinterpret_cast<uintptr_t>(x), r = reinterpret_cast<uintptr_t>(y);
+    return static_cast<uint64_t>(p < r ? r - p : p - r);
+  };
+  const uint64_t rows_apart = apart(k_cache, v_cache), scales_apart = apart(k_scales, v_scales);
+  if (rows_apart == 0 || scales_apart == 0) {
+    return set_error(VJ_ERR_INVALID_ARGUMENT, what + ": K and V must not be the same memory");
   }
+  if (rows_apart >= (1ull << 40) || scales_apart >= (1ull << 40)) {
+    return set_error(VJ_ERR_UNSUPPORTED, what + ": K and V lie 2^40 bytes apart or more");
+  }
+  a.v_half = v_cache > k_cache ? 1 : 0;
+  a.v_scale_half = v_scales > k_scales ? 1 : 0;
+  const uint64_t st = stride_token, sh = stride_head;
+  const uint32_t box_tok = kTok;
+  rc = head_major
+           ? encode_tmap_4d_u8(&tm_rows, a.v_half ? k_cache : v_cache, {kD, hkv, ntok, 2},
+                               {sh, st, rows_apart}, {kD, 1, box_tok, 2}, true)
+           : encode_tmap_4d_u8(&tm_rows, a.v_half ? k_cache : v_cache, {kD, ntok, hkv, 2},
+                               {st, sh, rows_apart}, {kD, box_tok, 1, 2}, true);
+  if (rc) return rc;
+  rc = encode_tmap_4d_u8(
+      &tm_scales, a.v_scale_half ? k_scales : v_scales,
+      {static_cast<uint64_t>(block_size), hkv, static_cast<uint64_t>(num_blocks), 2},
+      {static_cast<uint64_t>(scale_stride_head), static_cast<uint64_t>(scale_stride_block),
+       scales_apart},
+      {box_tok, 1, 1, 2}, false);
+  if (rc) return rc;
   a.q = static_cast<const __nv_bfloat16 *>(q);
   a.out = static_cast<__nv_bfloat16 *>(out);
   a.bt = block_tables;
   a.lens = context_lens;
-  a.ks = pool.ks;
-  a.vs = pool.vs;
-  a.ssb = scale_stride_block;
-  a.ssh = scale_stride_head;
   a.B = batch;
   a.Hq = num_q_heads;
   a.Hkv = num_kv_heads;
@@ -1058,11 +1078,11 @@ extern "C" vj_status vj_paged_decode_quantized(
   carve(&a.ws, workspace, batch, num_q_heads, num_kv_heads, a.groups, a.unit, a.may_deal != 0);
   const bool i8 = cache_dtype == VJ_CACHE_INT8;
   if (a.g <= 8) {
-    rc = i8 ? launch_decode<true, 1>(tmk, tmv, a, grid, stream)
-            : launch_decode<false, 1>(tmk, tmv, a, grid, stream);
+    rc = i8 ? launch_decode<true, 1>(tm_rows, tm_scales, a, grid, stream)
+            : launch_decode<false, 1>(tm_rows, tm_scales, a, grid, stream);
   } else {
-    rc = i8 ? launch_decode<true, 2>(tmk, tmv, a, grid, stream)
-            : launch_decode<false, 2>(tmk, tmv, a, grid, stream);
+    rc = i8 ? launch_decode<true, 2>(tm_rows, tm_scales, a, grid, stream)
+            : launch_decode<false, 2>(tm_rows, tm_scales, a, grid, stream);
   }
   if (rc || a.whole) return rc;
   const int64_t rows = static_cast<int64_t>(batch) * num_q_heads;

@@ -30,10 +30,9 @@ int check_launch(const char *what) {
 static PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
 static std::once_flag g_encode_once;
 
-static int encode_3d(CUtensorMap *map, CUtensorMapDataType type, const void *base, uint64_t dim0,
-                     uint64_t dim1, uint64_t dim2, uint64_t stride1_bytes,
-                     uint64_t stride2_bytes, uint32_t box0, uint32_t box1, uint32_t box2,
-                     bool swizzle128) {
+static int encode(CUtensorMap *map, CUtensorMapDataType type, uint32_t rank, const void *base,
+                  const uint64_t *dims, const uint64_t *stride_bytes, const uint32_t *box,
+                  bool swizzle128) {
   std::call_once(g_encode_once, []() {
     void *fn = nullptr;
     cudaDriverEntryPointQueryResult q;
@@ -46,12 +45,14 @@ static int encode_3d(CUtensorMap *map, CUtensorMapDataType type, const void *bas
   if (!g_encode) {
     return set_error(VJ_ERR_CUDA, "cuTensorMapEncodeTiled entry point not found");
   }
-  cuuint64_t dims[3] = {dim0, dim1, dim2};
-  cuuint64_t strides[2] = {stride1_bytes, stride2_bytes};
-  cuuint32_t box[3] = {box0, box1, box2};
-  cuuint32_t estr[3] = {1, 1, 1};
-  CUresult r = g_encode(map, type, 3,
-                        const_cast<void *>(base), dims, strides, box, estr,
+  cuuint64_t d[4], strides[3];
+  cuuint32_t b[4], estr[4] = {1, 1, 1, 1};
+  for (uint32_t i = 0; i < rank; ++i) {
+    d[i] = dims[i];
+    b[i] = box[i];
+    if (i > 0) strides[i - 1] = stride_bytes[i - 1];
+  }
+  CUresult r = g_encode(map, type, rank, const_cast<void *>(base), d, strides, b, estr,
                         CU_TENSOR_MAP_INTERLEAVE_NONE,
                         swizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B
                                    : CU_TENSOR_MAP_SWIZZLE_NONE,
@@ -69,16 +70,15 @@ int encode_tmap_3d(CUtensorMap *map, const void *base, uint64_t dim0,
                    uint64_t dim1, uint64_t dim2, uint64_t stride1_bytes,
                    uint64_t stride2_bytes, uint32_t box0, uint32_t box1,
                    uint32_t box2, bool swizzle128) {
-  return encode_3d(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, base, dim0, dim1, dim2, stride1_bytes,
-                   stride2_bytes, box0, box1, box2, swizzle128);
+  const uint64_t dims[3] = {dim0, dim1, dim2}, strides[2] = {stride1_bytes, stride2_bytes};
+  const uint32_t box[3] = {box0, box1, box2};
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, base, dims, strides, box, swizzle128);
 }
 
-int encode_tmap_3d_u8(CUtensorMap *map, const void *base, uint64_t dim0,
-                      uint64_t dim1, uint64_t dim2, uint64_t stride1_bytes,
-                      uint64_t stride2_bytes, uint32_t box0, uint32_t box1,
-                      uint32_t box2, bool swizzle128) {
-  return encode_3d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, dim0, dim1, dim2, stride1_bytes,
-                   stride2_bytes, box0, box1, box2, swizzle128);
+int encode_tmap_4d_u8(CUtensorMap *map, const void *base, const uint64_t (&dims)[4],
+                      const uint64_t (&stride_bytes)[3], const uint32_t (&box)[4],
+                      bool swizzle128) {
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, base, dims, stride_bytes, box, swizzle128);
 }
 
 int num_sms() {

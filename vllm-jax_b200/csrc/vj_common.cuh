@@ -24,11 +24,10 @@ int encode_tmap_3d(CUtensorMap *map, const void *base, uint64_t dim0,
                    uint64_t dim1, uint64_t dim2, uint64_t stride1_bytes,
                    uint64_t stride2_bytes, uint32_t box0, uint32_t box1,
                    uint32_t box2, bool swizzle128);
-// The same for 8-bit elements.
-int encode_tmap_3d_u8(CUtensorMap *map, const void *base, uint64_t dim0,
-                      uint64_t dim1, uint64_t dim2, uint64_t stride1_bytes,
-                      uint64_t stride2_bytes, uint32_t box0, uint32_t box1,
-                      uint32_t box2, bool swizzle128);
+// The same with four dimensions, of 8-bit elements.
+int encode_tmap_4d_u8(CUtensorMap *map, const void *base, const uint64_t (&dims)[4],
+                      const uint64_t (&stride_bytes)[3], const uint32_t (&box)[4],
+                      bool swizzle128);
 int num_sms();
 
 // ----------------------------------------------------------------------------
@@ -140,6 +139,16 @@ VJ_DEV void tma_load_3d(void *dst, const CUtensorMap *map, uint64_t *bar,
       "bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0),
       "r"(c1), "r"(c2)
+      : "memory");
+}
+
+VJ_DEV void tma_load_4d(void *dst, const CUtensorMap *map, uint64_t *bar,
+                        int32_t c0, int32_t c1, int32_t c2, int32_t c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::"
+      "bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0),
+      "r"(c1), "r"(c2), "r"(c3)
       : "memory");
 }
 
