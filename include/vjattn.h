@@ -486,9 +486,9 @@ VJ_API vj_status vj_allreduce_add_rmsnorm(
 
 /* vj_kv_store_qknorm_rope for the quantised cache: per-head RMSNorm
  * (VJ_KV_NORM) and RoPE (VJ_KV_ROPE, interleaved pairs, rope_table as there)
- * of q and k; q_out in bf16, k and v into their slots. All arithmetic of a row
- * is done in 32 bits (q) or 64 bits (k) and rounded once at the end, so a
- * cached row is the correctly rounded one (q of vj_kv_store_qknorm_rope is
+ * of q and k; q_out in bf16, k and v into their slots. A row of q is computed
+ * in 32 bits and rounded once at the end; one of k in 32 bits where those
+ * decide its rounding, else in 64, so a cached row is the correctly rounded one (q of vj_kv_store_qknorm_rope is
  * rounded to bf16 after every step as the reference does, so the two differ by
  * roundings). Tokens whose slot lies outside [0, num_blocks*block_size) store
  * nothing (their q is still written). Slots that are stored must differ from
@@ -525,9 +525,12 @@ VJ_API vj_status vj_kv_read_quantized(
  * query heads per KV head. stride_block must equal block_size*stride_token; K
  * and V (and their scales) may lie anywhere less than 2^40 bytes apart.
  * Cached rows past a sequence's context are never used, whatever they hold.
+ * A row of byte 255 within it must have zero elements, as the store leaves it
+ * (its sequence's results are NaN). Contexts longer than bt_width*block_size
+ * are cut there. out must not overlap q.
  *   workspace: vj_paged_decode_quantized_workspace_size(B, Hq, Hkv, D, bt_width,
- *   block_size) bytes on the current device, 16-byte aligned, need not be initialised; calls whose kernels may overlap
- *   need one each
+ *   block_size) bytes on the current device, 16-byte aligned, need not be
+ *   initialised; calls whose kernels may overlap need one each
  *   error_flag: device int32 (may be NULL), set to 1 if a wait timed out */
 VJ_API size_t vj_paged_decode_quantized_workspace_size(int32_t batch, int32_t num_q_heads,
                                                        int32_t num_kv_heads, int32_t head_dim,

@@ -135,6 +135,9 @@ def test_refusals_of_every_entry(entry, kw, status, msg):
     (_decode, dict(), "INVALID_ARGUMENT", b"same memory"),
     (_decode, dict(vc=32, vs=16), "INVALID_ARGUMENT", b"same memory"),
     (_decode, dict(vc=16 + (1 << 40), vs=32), "UNSUPPORTED", b"2^40"),
+    (_decode, dict(vc=32, vs=32), "INVALID_ARGUMENT", b"overlap"),
+    (_decode, dict(vc=32, vs=32, q=16 + 2 * 8 * 128 * 2 - 16), "INVALID_ARGUMENT", b"overlap"),
+    (_decode, dict(vc=32, vs=32, out=16 + 2 * 8 * 128 * 2 - 16), "INVALID_ARGUMENT", b"overlap"),
     (_read, dict(B=-1), "INVALID_ARGUMENT", b"size"),
     (_read, dict(L=-1), "INVALID_ARGUMENT", b"size"),
     (_read, dict(z=-1), "INVALID_ARGUMENT", b"size"),

@@ -285,7 +285,9 @@ def test_decode_batch_larger_than_a_block_of_threads():
 def test_decode_of_so_many_pages_that_a_part_is_dealt(Hq, Hkv, dtype):
     """Enough work (32 pages a warp and KV head) that a fifth of it is dealt in pieces:
     against 64 bits, the same bits every time, and on two streams at once."""
-    from vllm_b200.kernels.quantized_cache import QuantizedKVCache, paged_decode_quantized
+    from vllm_b200.kernels.quantized_cache import (QuantizedKVCache,
+                                                   decode_quantized_workspace_bytes,
+                                                   paged_decode_quantized)
     lens = [9001, 17, 0, 1, 12000, 3, 333, 300, 16, 11000, 8000, 700, 90, 32]
     bs, B = 32, len(lens)
     gen = torch.Generator(device="cuda").manual_seed(Hq)
@@ -326,6 +328,13 @@ def test_decode_of_so_many_pages_that_a_part_is_dealt(Hq, Hkv, dtype):
                 again.append(paged_decode_quantized(q, cache, bt, ln))
     torch.cuda.synchronize()
     assert all(torch.equal(o, out) for o in again)
+    # whatever the scratch holds before the call (counts of pieces among it)
+    ws = torch.empty(decode_quantized_workspace_bytes(B, Hq, Hkv, width, bs) // 4,
+                     dtype=torch.int32, device="cuda")
+    for word in (0, 1, 2, 3, -1, 0x7fc00000):
+        ws.fill_(word)
+        assert torch.equal(paged_decode_quantized(q, cache, bt, ln, workspace=ws.view(torch.uint8)),
+                           out)
 
 
 def test_decode_context_longer_than_the_table_is_cut():
@@ -597,6 +606,7 @@ def test_wrapper_refusals():
         (lambda: qc.paged_decode_quantized(q, c, bt.t().contiguous().t(), ln), "contiguous"),
         (lambda: qc.paged_decode_quantized(q, c, bt[:1].expand(3, 4), ln), "overlap"),
         (lambda: qc.paged_decode_quantized(q, c, bt, ln, out=q.float()), "out"),
+        (lambda: qc.paged_decode_quantized(q, c, bt, ln, out=q), "overlap"),
         (lambda: qc.paged_decode_quantized(q, c, bt, ln, workspace=torch.zeros(
             1, dtype=torch.uint8, device="cuda")), "workspace"),
         (lambda: qc.paged_decode_quantized(q, qc.QuantizedKVCache(c.data, c.scales[:, :3]), bt,

@@ -98,7 +98,9 @@ VJ_DEV float2 f16x2_to_f32(uint32_t w) {
 
 // Launch that may begin before the kernel ahead of it on the stream is done;
 // the kernel waits for that itself (griddepcontrol.wait) before it touches
-// memory that others write or read.
+// memory that others write or read, and reads it by plain loads: what read-only
+// ones (ld.global.nc) return is only defined for data that does not change from
+// the launch on, and the compiler may move those above the wait.
 template <typename... K, typename... A>
 int launch_dependent(const char *what, void (*kernel)(K...), dim3 grid, unsigned threads,
                      size_t smem, cudaStream_t stream, const A &...args) {

@@ -157,7 +157,7 @@ __device__ __noinline__ Scaled k_row_64(const uint8_t *row, const __nv_bfloat16 
   const int l8 = threadIdx.x & 7;
   const RowSlice x = load_slice(row, l8);
   RowSlice w = {};
-  if (norm) w = ldg_nc_slice(kw, l8);
+  if (norm) w = load_slice(kw, l8);
   Scaled r;
   double y[16];
 #pragma unroll
@@ -328,7 +328,7 @@ kv_store_quantized_kernel(const StoreArgs a) {
   int in_part = part, sent = 0;
   auto read_at = [&]() {
     if (in_t >= a.num_tokens) return make_int2(0, 0);
-    return make_int2(a.rope ? __ldg(a.positions + in_t) : 0, __ldg(a.slots + in_t));
+    return make_int2(a.rope ? a.positions[in_t] : 0, a.slots[in_t]);
   };
   int2 at = read_at();
   auto issue = [&](int s) {
@@ -392,7 +392,7 @@ kv_store_quantized_kernel(const StoreArgs a) {
     }
     int h = r0 + grp;
     if (h < a.Hq) {
-      const Turn turn = make_turn(a.norm ? ldg_nc_slice(a.qw, l8) : ones(), cs);
+      const Turn turn = make_turn(a.norm ? load_slice(a.qw, l8) : ones(), cs);
       __nv_bfloat16 *out = a.q_out + t * a.qors;
 #pragma unroll 4
       for (; h < min(r1, a.Hq); h += 4) {
@@ -404,7 +404,7 @@ kv_store_quantized_kernel(const StoreArgs a) {
     const int blk = a.bs_shift >= 0 ? slot >> a.bs_shift : slot / a.pool.block_size;
     const int64_t off = slot - blk * a.pool.block_size;
     Turn turn = {};
-    if (stored && h < a.Hq + a.Hkv) turn = make_turn(a.norm ? ldg_nc_slice(a.kw, l8) : ones(), cs);
+    if (stored && h < a.Hq + a.Hkv) turn = make_turn(a.norm ? load_slice(a.kw, l8) : ones(), cs);
 #pragma unroll 1
     for (; stored && h < r1; h += 4) {
       const bool is_v = h >= a.Hq + a.Hkv;
@@ -499,7 +499,7 @@ __global__ void __launch_bounds__(kReadThreads) kv_read_quantized_kernel(const R
   const int b = blockIdx.y;
   const int t0 = blockIdx.x * kReadTok;
   asm volatile("griddepcontrol.wait;" ::: "memory");    // the kernel ahead is done
-  const int len = min(min(__ldg(a.lens + b), a.max_tokens), a.max_len);
+  const int len = min(min(a.lens[b], a.max_tokens), a.max_len);
   int end = a.max_len;          // rows [len, end) are zeroed
   if (a.zero_to > 0) {
     const int64_t up = (static_cast<int64_t>(max(len, 1)) + a.zero_to - 1) / a.zero_to * a.zero_to;
@@ -509,7 +509,7 @@ __global__ void __launch_bounds__(kReadThreads) kv_read_quantized_kernel(const R
   if (nt <= 0) return;
   int64_t blk = 0;
   if (t0 < len) {
-    blk = __ldg(a.bt + static_cast<int64_t>(b) * a.bt_stride + t0 / a.pool.block_size);
+    blk = a.bt[static_cast<int64_t>(b) * a.bt_stride + t0 / a.pool.block_size];
     if (blk < 0 || blk >= a.pool.num_blocks) blk = 0;
   }
   const int off0 = t0 % a.pool.block_size;
@@ -533,7 +533,7 @@ __global__ void __launch_bounds__(kReadThreads) kv_read_quantized_kernel(const R
         const int tt = a.Hkv == 1 ? r : static_cast<int>(__umulhi(r, a.Hkv_magic));
         const int h = r - tt * a.Hkv;
         w[j] = __ldcs(reinterpret_cast<const uint2 *>(src + tt * a.pool.st + h * a.pool.sh));
-        sc[j] = __ldg(scales + h * a.pool.ssh + tt);
+        sc[j] = scales[h * a.pool.ssh + tt];
       }
     }
 #pragma unroll

@@ -30,16 +30,14 @@
 // range or piece, in the order of the pages.
 //   Where the block tables hold at most kWhole pages a row and there is a unit for
 // every sequence and KV head, a unit takes a whole sequence: nothing is left to
-// join, and there is one launch (17 tokens: 5.7 us against 7.5; at 125 pages, 16 a
+// join, and there is one launch (17 tokens: 5.4 us against 7.5; at 125 pages, 16 a
 // warp, it would be 21 against 11).
 //
 // A warp streams its pages through a ring of its own in shared memory: one TMA
 // box of 16 rows x 128 bytes of K and of V (128-byte swizzle; the distance from
 // the one to the other is the box's fourth dimension) and one of their scale
-// bytes. Issuing takes a quarter of the instructions as it is.
-// Where a page lies is looked up for 32 pages at once, a page a lane, and that
-// lane issues its copies; so the walk (sequence ends, block tables, addresses)
-// costs a page next to nothing. Products run on mma.sync m16n8k16 in f16 with
+// bytes. Where a page lies (sequence ends, block tables) is looked up for 32
+// pages at once, a page a lane, and that lane issues its copies. Products run on mma.sync m16n8k16 in f16 with
 // 32-bit sums, with the tokens, then the dimensions, as the 16 rows and the
 // query heads of the group as the 8 columns:
 //   S^T[tok][head] = K[tok][d] Q^T[d][head]     (8 steps of 16 dims)
@@ -107,9 +105,9 @@ struct Place {
   int b, p, np, len;      // p of np pages, of a context of len tokens
 };
 
-// How all pages are split: n ranges of neighbouring pages, the first `more` of
-// them of pages + 1, the others of `pages`. Where pieces are dealt, a range is
-// cut in kCuts parts.
+// How all places are split: n ranges of neighbouring ones, the first `more` of
+// them of pages + 1, the others of `pages` (in both, the kStart places in front of
+// a sequence count as pages). Where pieces are dealt, a range is cut in kCuts parts.
 constexpr int kCuts = 4;
 struct Split {
   int n, pages, more, dealt;
@@ -178,7 +176,7 @@ VJ_DEV Split split_pages(int total, int groups, int may_deal) {
   const int n = max(min(groups, total), 1);
   return {total > 0 ? n : 0, total / n, total % n, may_deal && total / groups >= kDealt ? 1 : 0};
 }
-// First page of range G (no division: every warp waits for it).
+// First place of range G (no division: every warp waits for it).
 VJ_DEV int first_page(int G, const Split &t) { return G * t.pages + min(G, t.more); }
 VJ_DEV int range_of(int page, const Split &t) {
   const int longer = t.more * (t.pages + 1);
@@ -268,7 +266,7 @@ VJ_DEV Place locate(const QDecodeArgs &a, const int *scan, int per, int s) {
   Place w;
   int cum = scan[lo];
   for (w.b = lo * per;; ++w.b) {            // s lies in this run
-    w.len = __ldg(a.lens + w.b);
+    w.len = a.lens[w.b];
     w.np = pages_of(w.len, a.max_pages);
     const int places = places_of(w.np);
     if (s < cum + places || w.b + 1 >= a.B) break;
@@ -302,8 +300,9 @@ quant_decode_kernel(const __grid_constant__ CUtensorMap tm_rows,
     fence_mbar_init();
     if (warp == 0) { tma_prefetch_desc(&tm_rows); tma_prefetch_desc(&tm_scales); }
   }
-  // nothing of the caller's is read before the kernel ahead is done; the
-  // combine kernel may be made ready as soon as every CTA of this one runs
+  // nothing of the caller's is read before the kernel ahead is done (and none of
+  // it by read-only loads, which need data that stands still from the launch on);
+  // the combine kernel may be made ready as soon as every CTA of this one runs
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;");
   const int unit = (warp / kUnit) * gridDim.x + blockIdx.x;
@@ -313,7 +312,7 @@ quant_decode_kernel(const __grid_constant__ CUtensorMap tm_rows,
     int mine = 0;
     for (int i = 0; i < per; ++i) {
       const int b = tid * per + i;
-      if (b < a.B) mine += places_of(pages_of(__ldg(a.lens + b), a.max_pages));
+      if (b < a.B) mine += places_of(pages_of(a.lens[b], a.max_pages));
     }
     int incl = mine;
 #pragma unroll
@@ -336,7 +335,7 @@ quant_decode_kernel(const __grid_constant__ CUtensorMap tm_rows,
   } else {
     // ---- the unit's sequence, as if it were all there is
     const int b = unit / a.Hkv;
-    const int len = b < a.B ? __ldg(a.lens + b) : 0, pages = pages_of(len, a.max_pages);
+    const int len = b < a.B ? a.lens[b] : 0, pages = pages_of(len, a.max_pages);
     if (b >= a.B) return;        // the whole unit
     if (pages == 0) {
       const int i = tid % (kUnit * 32), h = unit - b * a.Hkv;
@@ -364,7 +363,7 @@ quant_decode_kernel(const __grid_constant__ CUtensorMap tm_rows,
     for (int i = 0; i < per; ++i) {
       const int b = tid * per + i;
       if (b >= a.B) break;
-      const int pages = pages_of(__ldg(a.lens + b), a.max_pages);
+      const int pages = pages_of(a.lens[b], a.max_pages);
       int2 in = make_int2(0, 0);
       if (pages > 0) {
         const int of = dealt ? 1 : kUnit;
@@ -447,7 +446,7 @@ quant_decode_kernel(const __grid_constant__ CUtensorMap tm_rows,
         if (has_page) {
           const int entry = a.ppb_shift >= 0 ? w.p >> a.ppb_shift : w.p / a.pages_per_block;
           const int off = (w.p - entry * a.pages_per_block) * kTok;
-          int blk = __ldg(a.bt + static_cast<int64_t>(w.b) * a.bt_stride + entry);
+          int blk = a.bt[static_cast<int64_t>(w.b) * a.bt_stride + entry];
           if (blk < 0 || blk >= a.num_blocks) blk = 0;   // as the other attention kernels read it
           const bool seq_end = w.p + 1 == w.np;
           const bool end = at + 1 + (seq_end ? kStart : 0) >= seg_end;    // no page after it
@@ -497,7 +496,7 @@ quant_decode_kernel(const __grid_constant__ CUtensorMap tm_rows,
         const uint4 *src = reinterpret_cast<const uint4 *>(
             a.q + (static_cast<int64_t>(b) * a.Hq + h * a.g + head) * kD + qd * 32);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] = __ldg(src + j);
+        for (int j = 0; j < 4; ++j) x[j] = src[j];
       }
       const uint32_t *xw = reinterpret_cast<const uint32_t *>(x);
       uint32_t amax = 0;
@@ -810,11 +809,11 @@ quant_decode_kernel(const __grid_constant__ CUtensorMap tm_rows,
 }
 
 // Joins the partial results of sequences that several units (or ranges and
-// pieces) shared, and writes
-// the zeros of empty ones. kSplit warps take a (sequence, query head), each
-// every kSplit-th partial, several of them in flight: as many warps as fit the
-// GPU at once, since a row's time is its chain of memory round trips. Launched while
-// the decode kernel runs and held by griddepcontrol until that is done.
+// pieces) shared, and writes the zeros of empty ones. kSplit warps take a
+// (sequence, query head), each every kSplit-th partial, several of them in
+// flight: as many warps as fit the GPU at once, since a row's time is its chain
+// of memory round trips. Launched while the decode kernel runs and held by
+// griddepcontrol until that is done.
 template <int kSplit>
 constexpr int kCombineWarps = kSplit > 8 ? kSplit : 8;
 
@@ -1000,7 +999,8 @@ extern "C" vj_status vj_paged_decode_quantized(
                             "block_size * stride_token)");
   }
   const int64_t table_pages = static_cast<int64_t>(bt_width) * (block_size / kTok);
-  if (static_cast<int64_t>(batch) * (table_pages + kStart) > INT32_MAX ||
+  // places are counted in 32 bits, and looked up 32 at a time
+  if (static_cast<int64_t>(batch) * (table_pages + kStart) > INT32_MAX - 64 ||
       static_cast<int64_t>(batch) * num_q_heads > INT32_MAX) {
     return set_error(VJ_ERR_UNSUPPORTED, what + ": batch or block tables too large (2^31 pages)");
   }
@@ -1035,6 +1035,11 @@ extern "C" vj_status vj_paged_decode_quantized(
   }
   if (rows_apart >= (1ull << 40) || scales_apart >= (1ull << 40)) {
     return set_error(VJ_ERR_UNSUPPORTED, what + ": K and V lie 2^40 bytes apart or more");
+  }
+  // a sequence's q is read again after another part of its results is written
+  const uint64_t rows_bytes = static_cast<uint64_t>(batch) * num_q_heads * kD * 2;
+  if (apart(q, out) < rows_bytes) {
+    return set_error(VJ_ERR_INVALID_ARGUMENT, what + ": out must not overlap q");
   }
   a.v_half = v_cache > k_cache ? 1 : 0;
   a.v_scale_half = v_scales > k_scales ? 1 : 0;
