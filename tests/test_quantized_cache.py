@@ -177,6 +177,22 @@ def test_wrapper_refuses_cpu_tensors_and_unknown_types():
                                   torch.ones(1, dtype=torch.int32))
 
 
+def test_arguments_of_other_types():
+    from vllm_b200.kernels import quantized_cache as qc
+    q, bt = torch.zeros(1, 4, 128, dtype=torch.bfloat16), torch.zeros(1, 4, dtype=torch.int32)
+    cache = qc.QuantizedKVCache.zeros(4, 16, 2)
+    for call, msg in ((lambda: qc.paged_decode_quantized(q, cache, bt, [1]), "context_lens"),
+                      (lambda: qc.paged_decode_quantized(q, cache.data, bt, bt[0]), "cache"),
+                      (lambda: qc.paged_decode_quantized(q, (None, None), bt, bt[0]), "cache.data"),
+                      (lambda: qc.paged_decode_quantized(None, cache, bt, bt[0]), "`q`"),
+                      (lambda: qc.paged_decode_quantized(q, cache, bt, bt[0], out=1), "out"),
+                      (lambda: qc.kv_store_quantized(None, None, q, cache, bt[0]), "`k`"),
+                      (lambda: qc.read_kv_cache(cache, None, bt[0]), "block_tables"),
+                      (lambda: qc.paged_prefill_quantized(q, cache, bt, "x"), "cu_seqlens_q")):
+        with pytest.raises(TypeError, match=msg):
+            call()
+
+
 def test_config_refusals():
     from vllm_b200 import Config
     from vllm_b200.src.model_runner import check_kv_cache_dtype

@@ -589,6 +589,44 @@ def test_a_step_as_it_is_used():
                 assert not got[n:].any()
 
 
+def test_calls_keep_nothing_and_count_their_launches():
+    """Refused and accepted calls leave no references and no memory behind."""
+    import sys
+
+    from vllm_b200 import _native
+    from vllm_b200.kernels import quantized_cache as qc
+    c = qc.QuantizedKVCache.zeros(4, 16, 2, device="cuda")
+    q = torch.ones((3, 4, D), dtype=torch.bfloat16, device="cuda")
+    kv = torch.ones((3, 2, D), dtype=torch.bfloat16, device="cuda")
+    bt, idx = _i(np.arange(3)[:, None]), _i([0, 17, 34])
+    ln, cu, w = _i([1, 2, 3]), _i([0, 1, 2, 3]), _t(np.ones(D))
+    out = torch.empty_like(q)
+
+    def calls():
+        qc.kv_store_quantized(q, kv, kv, c, idx, ln, w, w)
+        qc.paged_decode_quantized(q, c, bt, ln)
+        assert qc.paged_decode_quantized(q, c, bt, ln, out=out) is out
+        qc.read_kv_cache(c, bt, ln)
+        qc.paged_prefill_quantized(q, c, bt, cu)
+        for bad in (lambda: qc.paged_decode_quantized(q, c, bt, ln, out=q),
+                    lambda: qc.paged_decode_quantized(q[:2], c, bt, ln),
+                    lambda: qc.kv_store_quantized(q, kv, kv, c, idx, ln, w)):
+            with pytest.raises(ValueError):
+                bad()
+
+    calls()                          # tables, identity pages, error word
+    torch.cuda.synchronize()
+    things = (q, kv, *c, bt, idx, ln, cu, w, out, _native, torch.device("cuda", 0))
+    refs, mem = [sys.getrefcount(x) for x in things], torch.cuda.memory_allocated()
+    before = _native.launch_count
+    for _ in range(20):
+        calls()
+    torch.cuda.synchronize()
+    assert _native.launch_count - before == 20 * (1 + 2 + 2 + 1 + 3)
+    assert torch.cuda.memory_allocated() == mem
+    assert [sys.getrefcount(x) for x in things] == refs
+
+
 # ----------------------------------------------------------------------------- refusals
 def test_wrapper_refusals():
     from vllm_b200.kernels import quantized_cache as qc

@@ -6,11 +6,14 @@ raises. The C prototypes mirror include/vjattn.h one to one.
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 import os
 import threading
 from pathlib import Path
 
 _LIB_PATH = Path(__file__).resolve().parent / "libvjattn.so"
+_CALLS_PATH = _LIB_PATH.with_name("_torch_calls.so")
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
 
@@ -165,6 +168,22 @@ def load() -> ctypes.CDLL:
                 fn.argtypes = args
             _lib = lib
     return _lib
+
+
+def load_calls():
+    """The compiled calls of the quantised cache (csrc/torch_calls.cpp), not bound yet."""
+    if not _CALLS_PATH.exists():
+        raise RuntimeError(f"{_CALLS_PATH} not found: build it with `python -m vllm_b200.build`")
+    loader = importlib.machinery.ExtensionFileLoader("vllm_b200._torch_calls", str(_CALLS_PATH))
+    spec = importlib.util.spec_from_loader(loader.name, loader)
+    module = importlib.util.module_from_spec(spec)
+    loader.exec_module(module)
+    return module
+
+
+def address(name: str) -> int:
+    """Address of an entry point."""
+    return ctypes.cast(getattr(load(), name), ctypes.c_void_p).value
 
 
 def check(status: int) -> None:

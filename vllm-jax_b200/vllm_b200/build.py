@@ -1,6 +1,8 @@
-"""Build libvjattn.so (the sm_100a kernels + C ABI) in-tree with nvcc.
+"""Build libvjattn.so (the sm_100a kernels + C ABI) in-tree with nvcc, and
+_torch_calls.so (argument checks and launches of the shortest calls, against
+torch's C++ headers) with g++.
 
-The shared library is written next to this file so that it travels with the
+The shared libraries are written next to this file so that they travel with the
 source tree; nothing is installed into site-packages. Usage:
 
     python -m vllm_b200.build            # incremental
@@ -15,6 +17,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parent
@@ -23,6 +26,8 @@ INCLUDE = PKG_DIR.parent.parent / "include"
 BUILD_DIR = PKG_DIR.parent / "_build"
 LIB_NAME = "libvjattn.so"
 LIB_PATH = PKG_DIR / LIB_NAME
+CALLS_SRC = CSRC / "torch_calls.cpp"
+CALLS_PATH = PKG_DIR / "_torch_calls.so"
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = [
@@ -57,6 +62,26 @@ def _compile(src: Path, obj: Path, ptxas_v: bool) -> str:
     return r.stderr
 
 
+def _build_calls() -> None:
+    import torch
+    root = Path(torch.__file__).resolve().parent
+    cxx = shutil.which("g++") or shutil.which("c++")
+    if cxx is None:
+        raise RuntimeError("g++ not found; a C++ compiler is required to build _torch_calls")
+    cuda = Path(_nvcc()).resolve().parent.parent / "include"
+    inc = [root / "include", root / "include/torch/csrc/api/include", cuda,
+           sysconfig.get_paths()["include"]]
+    tmp = CALLS_PATH.with_suffix(".so.tmp")
+    cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-shared",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+           *(f"-I{i}" for i in inc), str(CALLS_SRC), "-o", str(tmp), f"-L{root / 'lib'}",
+           "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed for {CALLS_SRC.name}:\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, CALLS_PATH)
+
+
 def build(force: bool = False, ptxas_v: bool = False, verbose: bool = False) -> Path:
     BUILD_DIR.mkdir(exist_ok=True)
     hdr_t = _headers_mtime()
@@ -69,13 +94,20 @@ def build(force: bool = False, ptxas_v: bool = False, verbose: bool = False) -> 
                  or obj.stat().st_mtime < max(src.stat().st_mtime, hdr_t))
         if stale:
             jobs.append((src, obj))
-    if jobs:
-        with cf.ThreadPoolExecutor(max_workers=min(8, len(jobs))) as ex:
+    header = INCLUDE / "vjattn.h"
+    stale_calls = (force or not CALLS_PATH.exists()
+                   or CALLS_PATH.stat().st_mtime < max(CALLS_SRC.stat().st_mtime,
+                                                       header.stat().st_mtime))
+    with cf.ThreadPoolExecutor(max_workers=8) as ex:
+        calls = ex.submit(_build_calls) if stale_calls else None
+        if jobs:
             futs = {ex.submit(_compile, s, o, ptxas_v): s for s, o in jobs}
             for f in cf.as_completed(futs):
                 log = f.result()
                 if (verbose or ptxas_v) and log:
                     print(f"--- {futs[f].name}\n{log}", file=sys.stderr)
+        if calls is not None:
+            calls.result()
     newest = max(o.stat().st_mtime for o in objs)
     if force or jobs or not LIB_PATH.exists() or LIB_PATH.stat().st_mtime < newest:
         tmp = LIB_PATH.with_suffix(".so.tmp")
