@@ -464,6 +464,28 @@ VJ_API vj_status vj_allreduce_add_rmsnorm(
     uint32_t *flags, int32_t rank, int32_t world, const void *residual, const void *weight,
     void *residual_out, void *y, int64_t rows, int32_t hidden, float eps, cudaStream_t stream);
 
+/* vj_paged_prefill where few tile pairs of new tokens leave SMs without work: the
+ * keys of a pair are split over several CTAs, whose results a second launch joins.
+ * Arguments as there, and
+ *   max_context_len: a bound on context_lens, which with max_seqlen_q, the batch
+ *   and the heads decides how far is split (not at all: vj_paged_prefill's bits)
+ *   workspace: vj_paged_prefill_split_workspace_size(...) bytes on the current
+ *   device (0 without a split: may be NULL), 16-byte aligned, need not be
+ *   initialised; calls whose kernels may overlap need one each
+ *   scale: positive and finite */
+VJ_API size_t vj_paged_prefill_split_workspace_size(int64_t num_tokens, int32_t num_seqs,
+                                                    int32_t num_q_heads, int32_t num_kv_heads,
+                                                    int32_t head_dim, int32_t max_seqlen_q,
+                                                    int32_t max_context_len);
+VJ_API vj_status vj_paged_prefill_split(
+    const void *q, const void *k_cache, const void *v_cache, const int32_t *block_tables,
+    const int32_t *cu_seqlens_q, const int32_t *context_lens, void *out, int64_t num_tokens,
+    int32_t num_seqs, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+    int64_t num_blocks, int32_t block_size, int32_t bt_width, int32_t bt_stride,
+    int64_t stride_block, int64_t stride_token, int64_t stride_head, int32_t max_seqlen_q,
+    int32_t max_context_len, float scale, void *workspace, size_t workspace_bytes,
+    int32_t *error_flag, cudaStream_t stream);
+
 /* ---------------------------------------------------------------------------
  * Quantised KV cache. No counterpart in the reference, whose kernels name
  * quantised pages (k_scales_pages, v_scales_pages:

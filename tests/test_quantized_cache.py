@@ -74,6 +74,14 @@ def _read(lib, **kw):
     return lib.vj_kv_read_quantized(*a.values())
 
 
+def _split(lib, **kw):
+    a = dict(q=16, k=16, v=16, bt=16, cu=16, ctx=16, out=16, T=4, S=1, Hq=8, Hkv=2, D=128, nb=200,
+             bs=16, w=200, bts=200, sb=4096, st=256, sh=128, mq=4, mc=3200, scale=0.1, ws=None,
+             wsb=0, err=16, stream=None)
+    a.update(kw)
+    return lib.vj_paged_prefill_split(*a.values())
+
+
 COMMON = [
     (dict(D=64), "UNSUPPORTED", b"head_dim"),
     (dict(dt=0), "INVALID_ARGUMENT", b"cache_dtype"),
@@ -145,6 +153,17 @@ def test_refusals_of_every_entry(entry, kw, status, msg):
     (_read, dict(Hkv=5000, st=128 * 5000, sb=16 * 128 * 5000), "UNSUPPORTED", b"4096"),
     (_read, dict(ko=None), "INVALID_ARGUMENT", b"null"),
     (_read, dict(vo=8), "INVALID_ARGUMENT", b"aligned"),
+    (_split, dict(scale=0.0), "INVALID_ARGUMENT", b"positive"),
+    (_split, dict(scale=-1.0), "INVALID_ARGUMENT", b"positive"),
+    (_split, dict(scale=float("nan")), "INVALID_ARGUMENT", b"positive"),
+    (_split, dict(scale=float("inf")), "INVALID_ARGUMENT", b"positive"),
+    (_split, dict(mc=-1), "INVALID_ARGUMENT", b"size"),
+    (_split, dict(Hq=7), "INVALID_ARGUMENT", b"divisible"),
+    (_split, dict(Hq=12), "UNSUPPORTED", b"divide 128"),
+    (_split, dict(D=64), "UNSUPPORTED", b"head_dim"),
+    (_split, dict(q=None), "INVALID_ARGUMENT", b"null"),
+    (_split, dict(), "WORKSPACE", b"workspace"),
+    (_split, dict(ws=8, wsb=1 << 30), "WORKSPACE", b"workspace"),
 ])
 def test_refusals_of_one_entry(entry, kw, status, msg):
     from vllm_b200 import _native

@@ -493,6 +493,79 @@ def test_prefill_scratch_garbage_does_not_matter():
     assert torch.equal(a, qc.paged_prefill_quantized(*args)) and torch.isfinite(a).all()
 
 
+@pytest.mark.parametrize("dtype", ["e4m3", "int8"])
+@pytest.mark.parametrize("Hq,Hkv,bs,new,prefix", [
+    (8, 2, 16, [1], [2000]),
+    (4, 1, 16, [3, 0, 2], [1500, 700, 4000]),
+    (16, 8, 32, [40], [1030]),
+    (32, 4, 16, [2, 17, 5], [5000, 3, 0]),      # more parts than key tiles
+    (8, 1, 16, [300], [1400]),                  # parts that early rows see nothing of
+    (16, 1, 48, [700], [2500]),
+    (12, 3, 16, [1, 1, 1, 1], [3000, 1023, 1024, 1025]),
+])
+def test_prefill_split_over_keys_matches_oracle(Hq, Hkv, bs, new, prefix, dtype):
+    """Few new tokens after long prefixes; scratch full of NaN; the same bits again."""
+    from vllm_b200 import _native
+    from vllm_b200.kernels import quantized_cache as qc
+    rng = np.random.default_rng(sum(prefix))
+    ctx = [a + b for a, b in zip(new, prefix)]
+    nb, width = sum(-(-n // bs) for n in ctx) + 2, max(-(-n // bs) for n in ctx) + 1
+    codes, scales = _random_pool(rng, nb, bs, Hkv, dtype)
+    bt = _tables(rng, ctx, nb, bs, width)
+    cu = np.concatenate([[0], np.cumsum(new)])
+    T = int(cu[-1])
+    q = bf16(rng.standard_normal((T + 5, Hq, D)))          # five padding rows
+    args = (_t(q), _cache(codes, scales, dtype), _i(bt), _i(cu), _i(ctx), max(new))
+    assert _native.load().vj_paged_prefill_split_workspace_size(T + 5, len(new), Hq, Hkv, D,
+                                                                max(new), max(ctx)) > 0
+    junk = [torch.full((1 << 22,), float("nan"), device="cuda") for _ in range(8)]
+    torch.cuda.synchronize()
+    del junk
+    got = qc.paged_prefill_quantized(*args, max_context_len=max(ctx))
+    vals = _values(codes, scales, dtype)
+    ref, mag = np.zeros(q.shape), np.zeros(q.shape)
+    for s, (n, p) in enumerate(zip(new, prefix)):
+        if n:
+            k, v = (oq.gather(vals[i], bt[s], n + p) for i in range(2))
+            rows = slice(cu[s], cu[s + 1])
+            ref[rows], mag[rows] = oq.attend(q[rows].astype(np.float64), k, v, p, 1 / math.sqrt(D))
+    _check(got, ref, mag, PREFILL)
+    for _ in range(3):
+        assert torch.equal(got, qc.paged_prefill_quantized(*args, max_context_len=max(ctx)))
+
+
+@pytest.mark.parametrize("S,new", [(0, 0), (3, 0), (1, 2)])
+def test_prefill_rows_behind_the_last_sequence_are_zeroed(S, new):
+    """Also where there is no sequence, or none has new tokens."""
+    from vllm_b200.kernels.quantized_cache import QuantizedKVCache, paged_prefill_quantized
+    cache = QuantizedKVCache.zeros(8, 16, 2, device="cuda")
+    cache.data.view(torch.uint8).fill_(0x38)                   # ones
+    q = torch.ones((1000, 4, D), dtype=torch.bfloat16, device="cuda")
+    out = torch.full_like(q, float("nan"))
+    paged_prefill_quantized(q, cache, _i(np.zeros((S, 2))), _i(np.arange(S + 1) * new),
+                            _i(np.full(S, new)), new, out=out)
+    assert (out[:S * new] == 1).all() and not out[S * new:].any()
+
+
+@pytest.mark.parametrize("prefix", [0, 2000])
+def test_prefill_nan_row_stays_in_its_sequence(prefix):
+    """A NaN row in the first page of the first sequence, whose block every unused table
+    entry stands for."""
+    from vllm_b200.kernels.quantized_cache import paged_prefill_quantized
+    rng = np.random.default_rng(23)
+    new, ctx = [5, 7], [prefix + 5, prefix + 7]
+    need = [-(-n // 16) for n in ctx]
+    codes, scales = _random_pool(rng, sum(need), 16, 2, "e4m3")
+    codes[:, 0, 0], scales[:, 0, :, 0] = 0, 255
+    bt = np.full((2, need[1] + 3), -1, np.int32)
+    bt[0, :need[0]] = np.arange(need[0])
+    bt[1, :need[1]] = need[0] + np.arange(need[1])
+    q = _t(bf16(rng.standard_normal((12, 4, D))))
+    out = paged_prefill_quantized(q, _cache(codes, scales, "e4m3"), _i(bt), _i([0, 5, 12]),
+                                  _i(ctx), max(new))
+    assert torch.isnan(out[:5]).all() and torch.isfinite(out[5:]).all()
+
+
 # ----------------------------------------------------------------------------- streams, graphs
 def test_decode_is_deterministic_on_two_streams_at_once_and_in_graphs():
     from vllm_b200.kernels.quantized_cache import paged_decode_quantized
@@ -622,7 +695,7 @@ def test_calls_keep_nothing_and_count_their_launches():
     for _ in range(20):
         calls()
     torch.cuda.synchronize()
-    assert _native.launch_count - before == 20 * (1 + 2 + 2 + 1 + 3)
+    assert _native.launch_count - before == 20 * (1 + 2 + 2 + 1 + 2)
     assert torch.cuda.memory_allocated() == mem
     assert [sys.getrefcount(x) for x in things] == refs
 
@@ -662,6 +735,7 @@ def test_wrapper_refusals():
         (lambda: qc.kv_store_quantized(q, kv[:, :1], kv[:, :1], c, ln, ln, w, w), "do not match"),
         (lambda: qc.kv_store_quantized(q, kv, kv, c, ln, ln, w, w, q_out=q[:, :2]), "q_out"),
         (lambda: qc.paged_prefill_quantized(q, c, bt, ln, ln), "one row per sequence"),
+        (lambda: qc.paged_prefill_quantized(q, c, bt[:2], ln, ln[:2], scale=0.0), "positive"),
         (lambda: qc.paged_prefill_quantized(q, c, bt[:2], ln, ln[:2], max_context_len=-4),
          "negative"),
     ]

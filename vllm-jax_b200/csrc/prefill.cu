@@ -33,10 +33,17 @@
 //                    core works on one tile while softmax works on the other
 //   warp 10          TMA producer of V tiles
 // Tensor-core bound: FLOPs = 4 * Hq * D * (n*p + n(n+1)/2) per sequence.
+//
+// prefill_split_kernel runs the same tiles for vj_paged_prefill_split: where the
+// tile pairs leave SMs without work, a pair's key tiles are split over several
+// CTAs. Each leaves its rows' sums in 32 bits, not normalised, with their maximum
+// and sum of weights, and prefill_join_kernel joins them.
 #include "../../include/vjattn.h"
 #include "vj_common.cuh"
 
 #include <algorithm>
+#include <atomic>
+#include <cmath>
 #include <string>
 
 namespace vj {
@@ -65,6 +72,7 @@ constexpr int OFF_K = OFF_Q + 2 * kTile;
 constexpr int OFF_V = OFF_K + kKStages * kTile;
 constexpr int OFF_BAR = OFF_V + kVStages * kTile;
 constexpr uint32_t TM_S = 0, TM_O = 256;        // + tile * 128
+constexpr int kSplitTiles = 8;                  // key tiles from which on a pair may be split
 constexpr float kRescaleThreshold = 8.0f;       // log2 units
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -118,12 +126,17 @@ struct PrefillArgs {
   int num_tokens;
   float scale_log2;
   int *err;
+  // key split: parts of a tile pair's key tiles, and what they leave per (part, token, head)
+  int parts, num_seqs;
+  float *part_o;            // [parts][tokens][Hq][128]
+  float2 *part_ml;          // [parts][tokens][Hq] maximum (log2), sum
 };
+constexpr float kLowest = -1e30f;       // a maximum that no key has moved yet
 
 // Token coordinate (flat pool token index of the page's first token) of page
-// grp*32 + lane of sequence s: one coalesced block-table read per 4 KV tiles.
-VJ_DEV int page_tok0(const PrefillArgs &a, const int32_t *row, int grp, int lane) {
-  const int page = grp * 32 + lane;
+// first + grp*32 + lane of sequence s: one coalesced block-table read per 4 KV tiles.
+VJ_DEV int page_tok0(const PrefillArgs &a, const int32_t *row, int first, int grp, int lane) {
+  const int page = first + grp * 32 + lane;
   int blk = 0;
   if (page < a.max_pages) {
     blk = __ldg(row + page / a.pages_per_block);
@@ -137,16 +150,17 @@ VJ_DEV int page_tok0(const PrefillArgs &a, const int32_t *row, int grp, int lane
 // issues the copies. Returns false if a wait timed out.
 template <int kStagesT>
 VJ_DEV bool produce_kv(const CUtensorMap *tm, uint8_t *ring, uint64_t *full, uint64_t *empty,
-                       const PrefillArgs &a, int s, int h, int nkv, int lane) {
+                       const PrefillArgs &a, int s, int h, int j0, int nkv, int lane) {
   const int32_t *row = a.bt + (size_t)s * a.bt_stride;
-  int cur = page_tok0(a, row, 0, lane);
-  int nxt = nkv > 4 ? page_tok0(a, row, 1, lane) : 0;
+  const int first = j0 * kPagesPerTile;
+  int cur = page_tok0(a, row, first, 0, lane);
+  int nxt = nkv > 4 ? page_tok0(a, row, first, 1, lane) : 0;
   for (int j = 0; j < nkv; ++j) {
     const int st = j % kStagesT, jj = j & 3;
     const int use = j / kStagesT;
     if (jj == 0 && j > 0) {
       cur = nxt;
-      nxt = j + 4 < nkv ? page_tok0(a, row, (j >> 2) + 1, lane) : 0;
+      nxt = j + 4 < nkv ? page_tok0(a, row, first, (j >> 2) + 1, lane) : 0;
     }
     bool ok = true;
     if (use > 0) ok = mbar_wait(&empty[st], (use - 1) & 1);
@@ -166,20 +180,52 @@ VJ_DEV bool produce_kv(const CUtensorMap *tm, uint8_t *ring, uint64_t *full, uin
   return true;
 }
 
-// The work of one CTA: tile pair m2 of (sequence s, kv head h). All 352
-// threads of the CTA run it.
+// This CTA's share of the rows past cu_seqlens_q[num_seqs] -> 0, by n of its threads.
+VJ_DEV void zero_tail_share(const PrefillArgs &a, int i, int n) {
+  const int64_t per_row = static_cast<int64_t>(a.Hq) * (kD / 8), from = a.cu[a.num_seqs] * per_row;
+  const int64_t tail = a.num_tokens * per_row - from;
+  if (tail <= 0) return;
+  const int64_t cta = (static_cast<int64_t>(blockIdx.z) * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x;
+  const int64_t ctas = static_cast<int64_t>(gridDim.x) * gridDim.y * gridDim.z;
+  uint4 *o = reinterpret_cast<uint4 *>(a.out) + from;
+  for (int64_t k = tail * cta / ctas + i; k < tail * (cta + 1) / ctas; k += n) {
+    o[k] = make_uint4(0u, 0u, 0u, 0u);
+  }
+}
+
+// The work of one CTA: tile pair m2 of (sequence s, kv head h), and with kSplit
+// its part `part` of a.parts of the key tiles. All 352 threads of the CTA run it.
+template <bool kSplit = false>
 __device__ __forceinline__ void prefill_body(const CUtensorMap *tmq_p, const CUtensorMap *tmk_p,
                                              const CUtensorMap *tmv_p, const PrefillArgs &a,
-                                             int s, int h, int m2, uint8_t *smem_raw) {
-  const int q0 = __ldg(a.cu + s);
-  const int n = __ldg(a.cu + s + 1) - q0;
+                                             int s, int h, int m2, uint8_t *smem_raw,
+                                             int part = 0) {
+  // (plain loads where the kernel may begin before what writes these is done)
+  const int q0 = kSplit ? a.cu[s] : __ldg(a.cu + s);
+  const int n = (kSplit ? a.cu[s + 1] : __ldg(a.cu + s + 1)) - q0;
   const int tq0 = m2 * 2 * a.tt;               // first token of tile A
-  if (tq0 >= n) return;  // whole CTA, before any barrier or TMEM use
-  int ctx = a.ctx_lens ? __ldg(a.ctx_lens + s) : n;
+  if (tq0 >= n) {        // whole CTA, before any barrier or TMEM use
+    if (kSplit && a.parts == 1) zero_tail_share(a, threadIdx.x, kThreads);
+    return;
+  }
+  int ctx = a.ctx_lens ? (kSplit ? a.ctx_lens[s] : __ldg(a.ctx_lens + s)) : n;
   if (ctx < n) ctx = n;
   const int p0 = ctx - n;                          // cached prefix length
   const int kv_end = p0 + min(n, tq0 + 2 * a.tt);  // keys visible to the last row of B
-  const int nkv = (kv_end + kBN - 1) / kBN;
+  int j0 = 0, nkv = (kv_end + kBN - 1) / kBN;
+  if constexpr (kSplit) {
+    const int all = nkv;
+    j0 = static_cast<int>(static_cast<int64_t>(all) * part / a.parts);
+    nkv = static_cast<int>(static_cast<int64_t>(all) * (part + 1) / a.parts) - j0;
+    if (nkv == 0) {                                // more parts than key tiles
+      const int t = threadIdx.x / kBM, r = threadIdx.x % kBM, tq = tq0 + t * a.tt + r / a.g;
+      if (t < 2 && tq < n && q0 + tq < a.num_tokens) {
+        a.part_ml[(static_cast<int64_t>(part) * a.num_tokens + q0 + tq) * a.Hq + h * a.g + r % a.g] =
+            make_float2(kLowest, 0.f);
+      }
+      return;
+    }
+  }
 
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                               ~uintptr_t(1023));
@@ -215,10 +261,11 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap *tmq_p, const CUt
         tma_load_3d(smem + OFF_Q + t * kTile + kHalf, tmq_p, &bar.q_full, 64, h * a.g, tok);
       }
     }
-    ok = produce_kv<kKStages>(tmk_p, smem + OFF_K, bar.k_full, bar.k_empty, a, s, h, nkv, lane);
+    ok = produce_kv<kKStages>(tmk_p, smem + OFF_K, bar.k_full, bar.k_empty, a, s, h, j0, nkv, lane);
   } else if (warp == kWarpV) {
     // ------------------------------------------------------------ V producer
-    ok = produce_kv<kVStages>(tmv_p, smem + OFF_V, bar.v_full, bar.v_empty, a, s, h, nkv, lane);
+    ok = produce_kv<kVStages>(tmv_p, smem + OFF_V, bar.v_full, bar.v_empty, a, s, h, j0, nkv, lane);
+    if (kSplit && a.parts == 1) zero_tail_share(a, lane, 32);
   } else if (warp == kWarpMma) {
     // ------------------------------------------------------------ MMA issuer
     if (lane == 0) {
@@ -289,14 +336,15 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap *tmq_p, const CUt
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t tS = tmem + lane_base + TM_S + t * kBM;
     const uint32_t tO = tmem + lane_base + TM_O + t * kBM;
-    float m_run = -INFINITY, l_run = 0.f;
+    // (a part may hold no key that a row sees: the maximum stays finite all the same)
+    float m_run = kSplit ? kLowest : -INFINITY, l_run = 0.f;
     float sv[kBN];
     for (int j = 0; j < nkv; ++j) {
       ok = mbar_wait(&bar.s_full[t], j & 1);
       if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
       tc_fence_after();
       tmem_ld128(tS, sv);
-      const int kbase = j * kBN;
+      const int kbase = (j0 + j) * kBN;
       if (kbase + kBN - 1 > qpos_min) {
 #pragma unroll
         for (int i = 0; i < kBN; ++i) {
@@ -375,6 +423,23 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap *tmq_p, const CUt
       tc_fence_after();
       const float inv = 1.f / l_run;
       const bool valid = tq < n && q0 + tq < a.num_tokens;
+      if (kSplit && a.parts > 1) {
+        const int64_t at =
+            (static_cast<int64_t>(part) * a.num_tokens + q0 + tq) * a.Hq + h * a.g + r % a.g;
+        if (valid) a.part_ml[at] = make_float2(m_run, l_run);
+#pragma unroll 1
+        for (int c = 0; c < kD / 32; ++c) {
+          float o[32];
+          tmem_ld32(tO + c * 32, o);
+          if (valid) {
+            float4 *dst = reinterpret_cast<float4 *>(a.part_o + at * kD + c * 32);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              dst[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+            }
+          }
+        }
+      } else {
       __nv_bfloat16 *orow =
           a.out + ((size_t)(q0 + tq) * a.Hq + (size_t)h * a.g + (r % a.g)) * kD;
 #pragma unroll 1
@@ -392,6 +457,7 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap *tmq_p, const CUt
             *reinterpret_cast<uint4 *>(orow + c * 32 + i) = w;
           }
         }
+      }
       }
     } else {
       ok = false;
@@ -459,6 +525,83 @@ attention_mixed_kernel(const __grid_constant__ CUtensorMap tmq,
   prefill_body(&tmq, &tmk, &tmv, pa, rest / pa.Hkv, rest % pa.Hkv, mpairs - 1 - x, smem_raw);
 }
 
+// Grid: tile pairs, kv heads, (sequence, part). Launched before the kernel ahead is
+// done, and lets the join be made ready.
+__global__ void __launch_bounds__(kThreads, 1)
+prefill_split_kernel(const __grid_constant__ CUtensorMap tmq,
+                     const __grid_constant__ CUtensorMap tmk,
+                     const __grid_constant__ CUtensorMap tmv, PrefillArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (a.parts > 1) asm volatile("griddepcontrol.launch_dependents;");
+  if (a.num_seqs == 0) {
+    zero_tail_share(a, threadIdx.x, kThreads);
+    return;
+  }
+  const int s = blockIdx.z / a.parts, part = blockIdx.z - s * a.parts;
+  prefill_body<true>(&tmq, &tmk, &tmv, a, s, blockIdx.y, gridDim.x - 1 - blockIdx.x, smem_raw,
+                     part);
+}
+
+// Joins the parts of the rows [cu[0], cu[num_seqs]) and zeroes those behind. kWarps
+// warps take a (token, query head), each every kWarps-th part, four of them in flight.
+constexpr int kJoinWarps = 8;
+template <int kWarps>
+__global__ void __launch_bounds__(kJoinWarps * 32)
+prefill_join_kernel(const PrefillArgs a) {
+  __shared__ float4 so[kJoinWarps][32];
+  __shared__ float2 sml[kJoinWarps];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, w = warp % kWarps;
+  const int64_t rows = static_cast<int64_t>(a.num_tokens) * a.Hq;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kJoinWarps / kWarps) + warp / kWarps;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int64_t first = static_cast<int64_t>(a.cu[0]) * a.Hq;
+  const int64_t end = static_cast<int64_t>(a.cu[a.num_seqs]) * a.Hq;
+  uint2 *dst = reinterpret_cast<uint2 *>(a.out + row * kD) + lane;
+  const bool mine = row >= first && row < end && row < rows;
+  if (row >= end && row < rows && w == 0) *dst = make_uint2(0u, 0u);
+  float m = kLowest, l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto add = [&](float2 ml, float4 x) {
+    if (ml.y == 0.f) return;            // no key of the part: its sums may not be there
+    const float top = fmaxf(m, ml.x), f0 = exp2f(m - top), f1 = exp2f(ml.x - top);
+    m = top;
+    l = fmaf(ml.y, f1, l * f0);
+    o.x = fmaf(x.x, f1, o.x * f0); o.y = fmaf(x.y, f1, o.y * f0);
+    o.z = fmaf(x.z, f1, o.z * f0); o.w = fmaf(x.w, f1, o.w * f0);
+  };
+  if (mine) {
+    constexpr int kFly = 4;
+    for (int i0 = w; i0 < a.parts; i0 += kFly * kWarps) {
+      float2 ml[kFly];
+      float4 x[kFly];
+#pragma unroll
+      for (int k = 0; k < kFly; ++k) {
+        const int i = i0 + k * kWarps;
+        ml[k] = make_float2(kLowest, 0.f);
+        x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (i < a.parts) {
+          const int64_t at = i * rows + row;
+          ml[k] = a.part_ml[at];
+          x[k] = reinterpret_cast<const float4 *>(a.part_o + at * kD)[lane];
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kFly; ++k) add(ml[k], x[k]);
+    }
+  }
+  if constexpr (kWarps > 1) {
+    so[warp][lane] = o;
+    if (lane == 0) sml[warp] = make_float2(m, l);
+    __syncthreads();
+    if (w != 0) return;
+    for (int k = 1; k < kWarps; ++k) add(sml[warp + k], so[warp + k][lane]);
+  }
+  if (!mine) return;
+  const float inv = 1.f / l;
+  *dst = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
+}
+
 // Rows of the packed output past cu_seqlens_q[num_seqs] (bucket padding) -> 0,
 // as the reference's scatter leaves them (prefill_paged_attention.py:384-388).
 __global__ void prefill_zero_tail_kernel(__nv_bfloat16 *out, const int32_t *cu, int num_seqs,
@@ -475,6 +618,109 @@ __global__ void prefill_zero_tail_kernel(__nv_bfloat16 *out, const int32_t *cu, 
 }  // namespace
 }  // namespace vj
 
+namespace vj {
+namespace {
+
+// Checks and arguments of vj_paged_prefill and vj_paged_prefill_split. Leaves
+// *pairs = 0 where there is no tile pair to launch, -1 where nothing is.
+int prefill_setup(const std::string &what, const void *q, const void *k_cache, const void *v_cache,
+                  const int32_t *block_tables, const int32_t *cu_seqlens_q,
+                  const int32_t *context_lens, void *out, int64_t num_tokens, int32_t num_seqs,
+                  int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int64_t num_blocks,
+                  int32_t block_size, int32_t bt_width, int32_t bt_stride, int64_t stride_block,
+                  int64_t stride_token, int64_t stride_head, int32_t max_seqlen_q, float scale,
+                  int32_t *error_flag, PrefillArgs *args, int64_t *pairs) {
+  *pairs = -1;
+  if (num_tokens < 0 || num_seqs < 0 || num_q_heads <= 0 || num_kv_heads <= 0 ||
+      num_blocks <= 0 || bt_width < 0 || bt_stride < bt_width) {
+    return set_error(VJ_ERR_INVALID_ARGUMENT, what + ": negative or zero size");
+  }
+  if (num_q_heads % num_kv_heads != 0) {
+    return set_error(VJ_ERR_INVALID_ARGUMENT,
+                     what + ": Number of Q heads must be divisible by number of KV "
+                            "heads. Got " + std::to_string(num_q_heads) + " and " +
+                         std::to_string(num_kv_heads) + ".");
+  }
+  const int g = num_q_heads / num_kv_heads;
+  if (head_dim != kD) return set_error(VJ_ERR_UNSUPPORTED, what + ": head_dim must be 128");
+  if (kBM % g != 0) {
+    return set_error(VJ_ERR_UNSUPPORTED, what + ": query heads per KV head must divide 128");
+  }
+  if (block_size <= 0 || block_size % kPageTok != 0) {
+    return set_error(VJ_ERR_UNSUPPORTED, what + ": block_size must be a multiple of 16");
+  }
+  if (stride_block != (int64_t)block_size * stride_token) {
+    return set_error(VJ_ERR_UNSUPPORTED,
+                     what + ": stride_block must equal block_size * stride_token");
+  }
+  if (num_blocks * block_size > (int64_t)INT32_MAX || num_tokens > (int64_t)INT32_MAX) {
+    return set_error(VJ_ERR_UNSUPPORTED, what + ": sizes beyond 2^31");
+  }
+  if (num_tokens == 0) return VJ_OK;
+  if (!q || !k_cache || !v_cache || !cu_seqlens_q || !out || !error_flag ||
+      (num_seqs > 0 && !block_tables)) {
+    return set_error(VJ_ERR_INVALID_ARGUMENT, what + ": null pointer");
+  }
+  PrefillArgs &a = *args;
+  a.out = static_cast<__nv_bfloat16 *>(out);
+  a.bt = block_tables;
+  a.cu = cu_seqlens_q;
+  a.ctx_lens = context_lens;
+  a.Hq = num_q_heads; a.Hkv = num_kv_heads; a.g = g; a.tt = kBM / g;
+  a.bt_stride = bt_stride;
+  a.pages_per_block = block_size / kPageTok;
+  a.max_pages = bt_width * a.pages_per_block;
+  a.block_size = block_size;
+  a.num_blocks = (int)num_blocks;
+  a.head_major = stride_head < stride_token ? 1 : 0;
+  a.num_tokens = (int)num_tokens;
+  a.scale_log2 = scale * kLog2e;
+  a.err = error_flag;
+  a.parts = 1;
+  a.num_seqs = num_seqs;
+  a.part_o = nullptr;
+  a.part_ml = nullptr;
+  const int64_t maxq = max_seqlen_q > 0 ? max_seqlen_q : num_tokens;
+  *pairs = num_seqs > 0 ? (maxq + 2 * a.tt - 1) / (2 * a.tt) : 0;
+  if (*pairs > 0 && (*pairs > INT32_MAX || num_kv_heads > 65535 || num_seqs > 65535)) {
+    return set_error(VJ_ERR_UNSUPPORTED, what + ": grid too large");
+  }
+  return VJ_OK;
+}
+
+// Tensor maps of the checked arguments.
+int prefill_maps(const PrefillArgs &a, const void *q, const void *k_cache, const void *v_cache,
+                 int64_t stride_token, int64_t stride_head, CUtensorMap *tmq, CUtensorMap *tmk,
+                 CUtensorMap *tmv) {
+  // Q: dims (D, Hq, tokens); one box = the g heads of tt tokens, 64 dims
+  int rc = encode_tmap_3d(tmq, q, kD, a.Hq, a.num_tokens, (uint64_t)kD * 2,
+                          (uint64_t)a.Hq * kD * 2, 64, a.g, a.tt, true);
+  if (rc) return rc;
+  const uint64_t ntok = (uint64_t)a.num_blocks * a.block_size;
+  for (int i = 0; i < 2; ++i) {
+    CUtensorMap *mp = i ? tmv : tmk;
+    const void *base = i ? v_cache : k_cache;
+    rc = a.head_major ? encode_tmap_3d(mp, base, kD, a.Hkv, ntok, stride_head * 2,
+                                       stride_token * 2, 64, 1, kPageTok, true)
+                      : encode_tmap_3d(mp, base, kD, ntok, a.Hkv, stride_token * 2,
+                                       stride_head * 2, 64, kPageTok, 1, true);
+    if (rc) return rc;
+  }
+  return VJ_OK;
+}
+
+// Parts of a tile pair's key tiles. Splitting pays where it fills SMs that the
+// pairs leave empty and saves several key tiles' time (0.7 us each) for the 4 us
+// of a join; a part of one tile costs more than it saves.
+int prefill_parts(int64_t pairs, int64_t num_kv_heads, int64_t num_seqs, int64_t max_context_len) {
+  const int64_t ctas = pairs * num_kv_heads * num_seqs, tiles = (max_context_len + kBN - 1) / kBN;
+  if (ctas == 0 || tiles < kSplitTiles) return 1;
+  return static_cast<int>(std::max<int64_t>(1, std::min(num_sms() / ctas, tiles / 2)));
+}
+
+}  // namespace
+}  // namespace vj
+
 extern "C" vj_status vj_paged_prefill(
     const void *q, const void *k_cache, const void *v_cache, const int32_t *block_tables,
     const int32_t *cu_seqlens_q, const int32_t *context_lens, void *out, int64_t num_tokens,
@@ -483,76 +729,17 @@ extern "C" vj_status vj_paged_prefill(
     int64_t stride_block, int64_t stride_token, int64_t stride_head, int32_t max_seqlen_q,
     float scale, int32_t *error_flag, cudaStream_t stream) {
   using namespace vj;
-  if (num_tokens < 0 || num_seqs < 0 || num_q_heads <= 0 || num_kv_heads <= 0 ||
-      num_blocks <= 0 || bt_width < 0 || bt_stride < bt_width) {
-    return set_error(VJ_ERR_INVALID_ARGUMENT, "vj_paged_prefill: negative or zero size");
-  }
-  if (num_q_heads % num_kv_heads != 0) {
-    return set_error(VJ_ERR_INVALID_ARGUMENT,
-                     "vj_paged_prefill: Number of Q heads must be divisible by number of KV "
-                     "heads. Got " + std::to_string(num_q_heads) + " and " +
-                         std::to_string(num_kv_heads) + ".");
-  }
-  const int g = num_q_heads / num_kv_heads;
-  if (head_dim != kD) return set_error(VJ_ERR_UNSUPPORTED, "vj_paged_prefill: head_dim must be 128");
-  if (kBM % g != 0) {
-    return set_error(VJ_ERR_UNSUPPORTED,
-                     "vj_paged_prefill: query heads per KV head must divide 128");
-  }
-  if (block_size <= 0 || block_size % kPageTok != 0) {
-    return set_error(VJ_ERR_UNSUPPORTED, "vj_paged_prefill: block_size must be a multiple of 16");
-  }
-  if (stride_block != (int64_t)block_size * stride_token) {
-    return set_error(VJ_ERR_UNSUPPORTED,
-                     "vj_paged_prefill: stride_block must equal block_size * stride_token");
-  }
-  if (num_blocks * block_size > (int64_t)INT32_MAX || num_tokens > (int64_t)INT32_MAX) {
-    return set_error(VJ_ERR_UNSUPPORTED, "vj_paged_prefill: sizes beyond 2^31");
-  }
-  if (num_tokens == 0) return VJ_OK;
-  if (!q || !k_cache || !v_cache || !cu_seqlens_q || !out || !error_flag ||
-      (num_seqs > 0 && !block_tables)) {
-    return set_error(VJ_ERR_INVALID_ARGUMENT, "vj_paged_prefill: null pointer");
-  }
-  const int tt = kBM / g;
   CUtensorMap tmq, tmk, tmv;
-  // Q: dims (D, Hq, tokens); one box = the g heads of tt tokens, 64 dims
-  int rc = encode_tmap_3d(&tmq, q, kD, num_q_heads, num_tokens, (uint64_t)kD * 2,
-                          (uint64_t)num_q_heads * kD * 2, 64, g, tt, true);
-  if (rc) return rc;
-  const uint64_t ntok = (uint64_t)num_blocks * block_size;
-  const bool head_major = stride_head < stride_token;
-  for (int i = 0; i < 2; ++i) {
-    CUtensorMap *mp = i ? &tmv : &tmk;
-    const void *base = i ? v_cache : k_cache;
-    rc = head_major ? encode_tmap_3d(mp, base, kD, num_kv_heads, ntok, stride_head * 2,
-                                     stride_token * 2, 64, 1, kPageTok, true)
-                    : encode_tmap_3d(mp, base, kD, ntok, num_kv_heads, stride_token * 2,
-                                     stride_head * 2, 64, kPageTok, 1, true);
-    if (rc) return rc;
-  }
   PrefillArgs a;
-  a.out = static_cast<__nv_bfloat16 *>(out);
-  a.bt = block_tables;
-  a.cu = cu_seqlens_q;
-  a.ctx_lens = context_lens;
-  a.Hq = num_q_heads; a.Hkv = num_kv_heads; a.g = g; a.tt = tt;
-  a.bt_stride = bt_stride;
-  a.pages_per_block = block_size / kPageTok;
-  a.max_pages = bt_width * a.pages_per_block;
-  a.block_size = block_size;
-  a.num_blocks = (int)num_blocks;
-  a.head_major = head_major ? 1 : 0;
-  a.num_tokens = (int)num_tokens;
-  a.scale_log2 = scale * kLog2e;
-  a.err = error_flag;
-
-  const int64_t maxq = max_seqlen_q > 0 ? max_seqlen_q : num_tokens;
-  const int64_t mpairs = (maxq + 2 * tt - 1) / (2 * tt);
-  if (num_seqs > 0 && mpairs > 0) {
-    if (mpairs > INT32_MAX || num_kv_heads > 65535 || num_seqs > 65535) {
-      return set_error(VJ_ERR_UNSUPPORTED, "vj_paged_prefill: grid too large");
-    }
+  int64_t mpairs;
+  int rc = prefill_setup("vj_paged_prefill", q, k_cache, v_cache, block_tables, cu_seqlens_q,
+                         context_lens, out, num_tokens, num_seqs, num_q_heads, num_kv_heads,
+                         head_dim, num_blocks, block_size, bt_width, bt_stride, stride_block,
+                         stride_token, stride_head, max_seqlen_q, scale, error_flag, &a, &mpairs);
+  if (rc || mpairs < 0) return rc;
+  rc = prefill_maps(a, q, k_cache, v_cache, stride_token, stride_head, &tmq, &tmk, &tmv);
+  if (rc) return rc;
+  if (mpairs > 0) {
     cudaFuncSetAttribute(prefill_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                          (int)kSmemBytes);
     dim3 grid((unsigned)mpairs, num_kv_heads, num_seqs);
@@ -563,6 +750,89 @@ extern "C" vj_status vj_paged_prefill(
   prefill_zero_tail_kernel<<<num_sms() * 2, 256, 0, stream>>>(
       static_cast<__nv_bfloat16 *>(out), cu_seqlens_q, num_seqs, num_tokens, num_q_heads * kD);
   return check_launch("vj_paged_prefill(zero tail)");
+}
+
+extern "C" size_t vj_paged_prefill_split_workspace_size(int64_t num_tokens, int32_t num_seqs,
+                                                        int32_t num_q_heads, int32_t num_kv_heads,
+                                                        int32_t head_dim, int32_t max_seqlen_q,
+                                                        int32_t max_context_len) {
+  if (num_tokens <= 0 || num_seqs <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 ||
+      head_dim != vj::kD || max_context_len < 0 || num_q_heads % num_kv_heads != 0 ||
+      vj::kBM % (num_q_heads / num_kv_heads) != 0) {
+    return 0;
+  }
+  const int64_t tt2 = 2 * (vj::kBM / (num_q_heads / num_kv_heads));
+  const int64_t maxq = max_seqlen_q > 0 ? max_seqlen_q : num_tokens;
+  const int parts =
+      vj::prefill_parts((maxq + tt2 - 1) / tt2, num_kv_heads, num_seqs, max_context_len);
+  return parts == 1 ? 0
+                    : static_cast<size_t>(parts) * num_tokens * num_q_heads *
+                          (vj::kD * sizeof(float) + sizeof(float2));
+}
+
+extern "C" vj_status vj_paged_prefill_split(
+    const void *q, const void *k_cache, const void *v_cache, const int32_t *block_tables,
+    const int32_t *cu_seqlens_q, const int32_t *context_lens, void *out, int64_t num_tokens,
+    int32_t num_seqs, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+    int64_t num_blocks, int32_t block_size, int32_t bt_width, int32_t bt_stride,
+    int64_t stride_block, int64_t stride_token, int64_t stride_head, int32_t max_seqlen_q,
+    int32_t max_context_len, float scale, void *workspace, size_t workspace_bytes,
+    int32_t *error_flag, cudaStream_t stream) {
+  using namespace vj;
+  const std::string what = "vj_paged_prefill_split";
+  if (max_context_len < 0) {
+    return set_error(VJ_ERR_INVALID_ARGUMENT, what + ": negative or zero size");
+  }
+  // the row maximum is taken of q.k, before the scale; 0 times a masked key's -inf is NaN
+  if (!(scale > 0.f) || std::isinf(scale)) {
+    return set_error(VJ_ERR_INVALID_ARGUMENT, what + ": scale must be positive and finite");
+  }
+  CUtensorMap tmq, tmk, tmv;
+  PrefillArgs a;
+  int64_t mpairs;
+  int rc = prefill_setup(what, q, k_cache, v_cache, block_tables, cu_seqlens_q, context_lens, out,
+                         num_tokens, num_seqs, num_q_heads, num_kv_heads, head_dim, num_blocks,
+                         block_size, bt_width, bt_stride, stride_block, stride_token, stride_head,
+                         max_seqlen_q, scale, error_flag, &a, &mpairs);
+  if (rc || mpairs < 0) return rc;
+  a.parts = prefill_parts(mpairs, num_kv_heads, num_seqs, max_context_len);
+  const int64_t rows = num_tokens * num_q_heads;
+  if (a.parts > 1) {
+    const size_t need = vj_paged_prefill_split_workspace_size(
+        num_tokens, num_seqs, num_q_heads, num_kv_heads, head_dim, max_seqlen_q, max_context_len);
+    if (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16 != 0) {
+      return set_error(VJ_ERR_WORKSPACE, what + ": workspace needs " + std::to_string(need) +
+                                             " bytes, 16-byte aligned");
+    }
+    a.part_o = static_cast<float *>(workspace);
+    a.part_ml = reinterpret_cast<float2 *>(a.part_o + a.parts * rows * kD);
+  }
+  const int64_t z = std::max<int64_t>(static_cast<int64_t>(num_seqs) * a.parts, 1);
+  if (z > 65535 || rows > INT32_MAX) {
+    return set_error(VJ_ERR_UNSUPPORTED, what + ": grid too large");
+  }
+  rc = prefill_maps(a, q, k_cache, v_cache, stride_token, stride_head, &tmq, &tmk, &tmv);
+  if (rc) return rc;
+  // the shared-memory opt-in is a per-device attribute of the kernel
+  static std::atomic<bool> opted[64];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && (dev >= 64 || !opted[dev].load(std::memory_order_acquire))) {
+    e = cudaFuncSetAttribute(prefill_split_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             static_cast<int>(kSmemBytes));
+    if (e == cudaSuccess && dev < 64) opted[dev].store(true, std::memory_order_release);
+  }
+  if (e != cudaSuccess) return set_error(VJ_ERR_CUDA, what + ": " + cudaGetErrorString(e));
+  const dim3 grid(static_cast<unsigned>(std::max<int64_t>(mpairs, 1)),
+                  static_cast<unsigned>(num_kv_heads), static_cast<unsigned>(z));
+  rc = launch_dependent(what.c_str(), prefill_split_kernel, grid, kThreads, kSmemBytes, stream, tmq,
+                        tmk, tmv, a);
+  if (rc || a.parts == 1) return rc;
+  // few rows: eight warps each
+  const bool few = rows <= 8 * num_sms();
+  const int64_t blocks = few ? rows : (rows + kJoinWarps - 1) / kJoinWarps;
+  return launch_dependent(what.c_str(), few ? prefill_join_kernel<kJoinWarps> : prefill_join_kernel<1>,
+                          dim3(static_cast<unsigned>(blocks)), kJoinWarps * 32, 0, stream, a);
 }
 
 extern "C" size_t vj_paged_attention_mixed_workspace_size(int32_t num_decode,

@@ -96,32 +96,6 @@ VJ_DEV float2 f16x2_to_f32(uint32_t w) {
   return r;
 }
 
-// Launch that may begin before the kernel ahead of it on the stream is done;
-// the kernel waits for that itself (griddepcontrol.wait) before it touches
-// memory that others write or read, and reads it by plain loads: what read-only
-// ones (ld.global.nc) return is only defined for data that does not change from
-// the launch on, and the compiler may move those above the wait.
-template <typename... K, typename... A>
-int launch_dependent(const char *what, void (*kernel)(K...), dim3 grid, unsigned threads,
-                     size_t smem, cudaStream_t stream, const A &...args) {
-  cudaLaunchConfig_t c = {};
-  c.gridDim = grid;
-  c.blockDim = dim3(threads);
-  c.dynamicSmemBytes = smem;
-  c.stream = stream;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  c.attrs = at;
-  c.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&c, kernel, args...);
-  if (e != cudaSuccess) {
-    cudaGetLastError();
-    return set_error(VJ_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
-  }
-  return VJ_OK;
-}
-
 // Checks shared by every entry point of the quantised cache; `what` names it.
 inline int check_pool(const std::string &what, const Pool &p, int cache_dtype, int num_kv_heads,
                       int head_dim) {

@@ -28,7 +28,8 @@ decltype(&vj_kv_store_quantized) store_entry;
 decltype(&vj_paged_decode_quantized) decode_entry;
 decltype(&vj_paged_decode_quantized_workspace_size) workspace_entry;
 decltype(&vj_kv_read_quantized) read_entry;
-decltype(&vj_paged_prefill) prefill_entry;
+decltype(&vj_paged_prefill_split) prefill_entry;
+decltype(&vj_paged_prefill_split_workspace_size) prefill_workspace_entry;
 PyObject *native;             // module: check(status), launch_count
 PyObject *error_flag_of;      // (device index) -> address
 PyObject *rope_table_of;      // (device, theta) -> tensor
@@ -251,9 +252,9 @@ Tables tables(const Arg &bt, const Arg &lens, int64_t B) {
   if (bt->dim() != 2 || bt->size(0) != B) fail("`block_tables` must have one row per sequence");
   Tables t;
   t.width = i32(bt->size(1), "the width of block_tables");
-  if (bt->stride(1) != 1 && t.width > 1) fail("block_tables rows must be contiguous");
+  if (B > 0 && t.width > 1 && bt->stride(1) != 1) fail("block_tables rows must be contiguous");
   int64_t stride = bt->stride(0);
-  if (stride < t.width) {
+  if (B == 0 || stride < t.width) {
     if (B > 1) fail("block_tables rows must not overlap");
     stride = t.width;
   }
@@ -449,15 +450,22 @@ PyObject *paged_prefill(PyObject *const *args) {
   const int64_t bound = integer(args[8]), capacity = static_cast<int64_t>(t.width) * p.bs;
   if (bound < 0) fail("max_context_len must not be negative");
   const int64_t most = std::min(bound ? bound : capacity, capacity);
-  const int32_t len = i32(std::max<int64_t>((most + kPage - 1) / kPage, 1) * kPage, "max_context_len");
+  // whole key tiles: a tile's keys behind a context are zeros of its own, not another's rows
+  const int32_t len =
+      i32(std::max<int64_t>((most + kKeyTile - 1) / kKeyTile, 1) * kKeyTile, "max_context_len");
   const float scale = static_cast<float>(args[6] == Py_None ? 1.0 / std::sqrt(p.D) : number(args[6]));
   at::Tensor out = output(given, q);
-  // the scratch: page i of a group's sequence b is block b * per_seq + i
+  // the scratch: K and V, where page i of a group's sequence b is block b * per_seq
+  // + i, then what a split over keys needs
   const int64_t row = static_cast<int64_t>(p.hkv) * p.D;
   const int64_t group = std::max<int64_t>(
       1, std::min<int64_t>(S, integer(args[9]) / (static_cast<int64_t>(len) * p.hkv)));
   const int32_t per_seq = len / kPage;
-  const at::Tensor scratch = at::empty({2 * group * len * row}, q->options());
+  const int64_t T = q->size(0);
+  const size_t split_bytes = prefill_workspace_entry(T, static_cast<int32_t>(std::min<int64_t>(group, S)),
+                                                     hq, p.hkv, p.D, max_new, len);
+  const at::Tensor scratch = at::empty(
+      {2 * group * len * row + static_cast<int64_t>(split_bytes / 2)}, q->options());
   const Owned device(PyObject_GetAttrString(q.o, "device"));
   const Owned in_order(PyObject_CallFunction(pages_in_order, "OL", device.p,
                                              static_cast<long long>(group * per_seq)));
@@ -465,34 +473,40 @@ PyObject *paged_prefill(PyObject *const *args) {
   const int32_t *const cu_ptr = static_cast<const int32_t *>(cu.ptr());
   const void *q_ptr = q.ptr();
   void *const out_ptr = out.data_ptr(), *const k_ptr = scratch.data_ptr();
+  void *const ws = static_cast<uint8_t *>(k_ptr) + 4 * group * len * row;
   int32_t *const err = error_flag(dev);
   const cudaStream_t stream = stream_of(dev);
-  const int64_t T = q->size(0);
   for (int64_t s = 0; s < std::max(S, 1); s += group) {
     const int32_t n = static_cast<int32_t>(std::min<int64_t>(group, S - s));
     const Tables part = {t.ptr + s * t.stride, t.lens + s, t.width, t.stride};
     read_back(p, part, k_ptr, n, len, kKeyTile, stream);
-    enter(2, [&] {
+    // (the last group may be smaller and split further than the others)
+    const size_t need = prefill_workspace_entry(T, n, hq, p.hkv, p.D, max_new, len);
+    at::Tensor more;
+    if (need > split_bytes) more = at::empty({static_cast<int64_t>(need)}, q->options().dtype(at::kByte));
+    void *const part_ws = more.defined() ? more.data_ptr() : ws;
+    enter(need > 0 ? 2 : 1, [&] {
       return prefill_entry(q_ptr, k_ptr, static_cast<uint8_t *>(k_ptr) + n * len * row * 2, pages,
                            cu_ptr + s, part.lens, out_ptr, T, n, hq, p.hkv, p.D,
                            static_cast<int64_t>(std::max(n, 1)) * per_seq, kPage, per_seq, per_seq,
-                           kPage * row, row, p.D, max_new, scale, err, stream);
+                           kPage * row, row, p.D, max_new, len, scale, part_ws, need, err, stream);
     });
   }
   return given ? Py_NewRef(given.o) : THPVariable_Wrap(std::move(out));
 }
 
-// (addresses of the five entries in the order above, then the four objects)
+// (addresses of the six entries in the order above, then the four objects)
 PyObject *bind(PyObject *const *args) {
   store_entry = reinterpret_cast<decltype(store_entry)>(integer(args[0]));
   decode_entry = reinterpret_cast<decltype(decode_entry)>(integer(args[1]));
   workspace_entry = reinterpret_cast<decltype(workspace_entry)>(integer(args[2]));
   read_entry = reinterpret_cast<decltype(read_entry)>(integer(args[3]));
   prefill_entry = reinterpret_cast<decltype(prefill_entry)>(integer(args[4]));
-  native = Py_NewRef(args[5]);
-  error_flag_of = Py_NewRef(args[6]);
-  rope_table_of = Py_NewRef(args[7]);
-  pages_in_order = Py_NewRef(args[8]);
+  prefill_workspace_entry = reinterpret_cast<decltype(prefill_workspace_entry)>(integer(args[5]));
+  native = Py_NewRef(args[6]);
+  error_flag_of = Py_NewRef(args[7]);
+  rope_table_of = Py_NewRef(args[8]);
+  pages_in_order = Py_NewRef(args[9]);
   Py_RETURN_NONE;
 }
 
@@ -518,7 +532,7 @@ PyMethodDef entry(const char *name) {
 }
 PyMethodDef methods[] = {entry<kv_store, 14>("kv_store"), entry<paged_decode, 7>("paged_decode"),
                          entry<read_kv_cache, 5>("read_kv_cache"),
-                         entry<paged_prefill, 10>("paged_prefill"), entry<bind, 9>("bind"),
+                         entry<paged_prefill, 10>("paged_prefill"), entry<bind, 10>("bind"),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_torch_calls", nullptr, -1, methods};
 

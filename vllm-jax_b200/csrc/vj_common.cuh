@@ -10,6 +10,8 @@
 
 #include <string>
 
+#include "../../include/vjattn.h"
+
 #define VJ_DEV __device__ __forceinline__
 
 namespace vj {
@@ -29,6 +31,32 @@ int encode_tmap_4d_u8(CUtensorMap *map, const void *base, const uint64_t (&dims)
                       const uint64_t (&stride_bytes)[3], const uint32_t (&box)[4],
                       bool swizzle128);
 int num_sms();
+
+// Launch that may begin before the kernel ahead of it on the stream is done;
+// the kernel waits for that itself (griddepcontrol.wait) before it touches
+// memory that others write or read, and reads it by plain loads: what read-only
+// ones (ld.global.nc) return is only defined for data that does not change from
+// the launch on, and the compiler may move those above the wait.
+template <typename... K, typename... A>
+int launch_dependent(const char *what, void (*kernel)(K...), dim3 grid, unsigned threads,
+                     size_t smem, cudaStream_t stream, const A &...args) {
+  cudaLaunchConfig_t c = {};
+  c.gridDim = grid;
+  c.blockDim = dim3(threads);
+  c.dynamicSmemBytes = smem;
+  c.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  c.attrs = at;
+  c.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&c, kernel, args...);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return set_error(VJ_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
+  }
+  return VJ_OK;
+}
 
 // ----------------------------------------------------------------------------
 // bf16 helpers
