@@ -10,6 +10,7 @@
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/sub.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -33,7 +34,7 @@ decltype(&vj_paged_prefill_split_workspace_size) prefill_workspace_entry;
 PyObject *native;             // module: check(status), launch_count
 PyObject *error_flag_of;      // (device index) -> address
 PyObject *rope_table_of;      // (device, theta) -> tensor
-PyObject *pages_in_order;     // (device, n) -> tensor
+PyObject *pages_in_order;     // (device index, n) -> tensor
 
 struct Raised {};             // a Python error is set
 
@@ -131,6 +132,30 @@ int32_t *error_flag(int index) {
   int32_t *p = reinterpret_cast<int32_t *>(integer(address.p));
   if (index < 64) flags[index] = p;
   return p;
+}
+
+// n pages in order, or more of them. What the package keeps stays where it is for
+// good, so its address is remembered; what a capture makes is not kept.
+struct Pages {
+  const int32_t *ptr;
+  int64_t n;
+  PyObject *made;                // a reference to drop after the launches
+};
+Pages in_order(int index, int64_t n) {
+  static Pages kept[64];
+  if (index < 64 && kept[index].n >= n) return kept[index];
+  const bool capturing =
+      c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None;
+  PyObject *made = raise_if_null(
+      PyObject_CallFunction(pages_in_order, "iL", index, static_cast<long long>(n)));
+  const Arg t = tensor(made, "pages");
+  const Pages p = {static_cast<const int32_t *>(t.ptr()), t->numel(), nullptr};
+  if (!capturing && index < 64) {
+    kept[index] = p;
+    Py_DECREF(made);             // the package keeps it
+    return p;
+  }
+  return {p.ptr, p.n, made};
 }
 
 // A C entry without the interpreter's lock; counts its launches, raises its errors.
@@ -466,10 +491,12 @@ PyObject *paged_prefill(PyObject *const *args) {
                                                      hq, p.hkv, p.D, max_new, len);
   const at::Tensor scratch = at::empty(
       {2 * group * len * row + static_cast<int64_t>(split_bytes / 2)}, q->options());
-  const Owned device(PyObject_GetAttrString(q.o, "device"));
-  const Owned in_order(PyObject_CallFunction(pages_in_order, "OL", device.p,
-                                             static_cast<long long>(group * per_seq)));
-  const int32_t *const pages = static_cast<const int32_t *>(tensor(in_order.p, "pages").ptr());
+  const Pages listed = in_order(dev, group * per_seq);
+  struct Drop {
+    PyObject *p;
+    ~Drop() { Py_XDECREF(p); }
+  } const drop{listed.made};
+  const int32_t *const pages = listed.ptr;
   const int32_t *const cu_ptr = static_cast<const int32_t *>(cu.ptr());
   const void *q_ptr = q.ptr();
   void *const out_ptr = out.data_ptr(), *const k_ptr = scratch.data_ptr();

@@ -129,22 +129,22 @@ _identity: dict[int, torch.Tensor] = {}
 _retired_identity: list[torch.Tensor] = []
 
 
-def _identity_pages(dev: torch.device, n: int) -> torch.Tensor:
-    """0, 1, .., the block tables of a scratch whose pages lie in order, kept per
-    device and only grown. An outgrown tensor is kept too: a captured graph may
+def _identity_pages(index: int, n: int) -> torch.Tensor:
+    """0, 1, .., n - 1 or further, the block tables of a scratch whose pages lie in order, kept
+    per device and only grown. An outgrown tensor is kept too: a captured graph may
     read it. What a capture makes is the graph's own."""
+    t = _identity.get(index)
+    if t is not None and t.numel() >= n:
+        return t
+    dev = torch.device("cuda", index)
     if torch.cuda.is_current_stream_capturing():
-        t = _identity.get(dev.index)
-        return t[:n] if t is not None and t.numel() >= n else \
-            torch.arange(n, dtype=torch.int32, device=dev)
-    t = _identity.get(dev.index)
-    if t is None or t.numel() < n:
-        if t is not None:
-            _retired_identity.append(t)
-        # a blocking copy: complete for every stream when it returns
-        t = torch.arange(max(n, 1 << 16), dtype=torch.int32).to(dev)
-        _identity[dev.index] = t
-    return t[:n]
+        return torch.arange(n, dtype=torch.int32, device=dev)
+    if t is not None:
+        _retired_identity.append(t)
+    # a blocking copy: complete for every stream when it returns
+    t = torch.arange(max(n, 1 << 16), dtype=torch.int32).to(dev)
+    _identity[index] = t
+    return t
 
 
 # bf16 rows (token x KV head) of one read-back inside paged_prefill_quantized:
