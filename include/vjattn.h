@@ -467,6 +467,7 @@ VJ_API vj_status vj_allreduce_add_rmsnorm(
 /* vj_paged_prefill where few tile pairs of new tokens leave SMs without work: the
  * keys of a pair are split over several CTAs, whose results a second launch joins.
  * Arguments as there, and
+ *   block_tables may be NULL: entry i of sequence s is then s*bt_stride + i
  *   max_context_len: a bound on context_lens, which with max_seqlen_q, the batch
  *   and the heads decides how far is split (not at all: vj_paged_prefill's bits)
  *   workspace: vj_paged_prefill_split_workspace_size(...) bytes on the current

@@ -162,6 +162,7 @@ def test_refusals_of_every_entry(entry, kw, status, msg):
     (_split, dict(Hq=12), "UNSUPPORTED", b"divide 128"),
     (_split, dict(D=64), "UNSUPPORTED", b"head_dim"),
     (_split, dict(q=None), "INVALID_ARGUMENT", b"null"),
+    (_split, dict(bt=None, S=1 << 16, bts=1 << 16), "UNSUPPORTED", b"2^31"),
     (_split, dict(), "WORKSPACE", b"workspace"),
     (_split, dict(ws=8, wsb=1 << 30), "WORKSPACE", b"workspace"),
 ])

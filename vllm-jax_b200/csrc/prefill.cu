@@ -73,6 +73,8 @@ constexpr int OFF_V = OFF_K + kKStages * kTile;
 constexpr int OFF_BAR = OFF_V + kVStages * kTile;
 constexpr uint32_t TM_S = 0, TM_O = 256;        // + tile * 128
 constexpr int kSplitTiles = 8;                  // key tiles from which on a pair may be split
+// K and V up to which all heads' tile pairs may run side by side (L2 holds 126 MB)
+constexpr int64_t kResidentKv = 80 << 20;
 constexpr float kRescaleThreshold = 8.0f;       // log2 units
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -127,7 +129,7 @@ struct PrefillArgs {
   float scale_log2;
   int *err;
   // key split: parts of a tile pair's key tiles, and what they leave per (part, token, head)
-  int parts, num_seqs;
+  int parts, num_seqs, longest_first;
   float *part_o;            // [parts][tokens][Hq][128]
   float2 *part_ml;          // [parts][tokens][Hq] maximum (log2), sum
 };
@@ -135,11 +137,15 @@ constexpr float kLowest = -1e30f;       // a maximum that no key has moved yet
 
 // Token coordinate (flat pool token index of the page's first token) of page
 // first + grp*32 + lane of sequence s: one coalesced block-table read per 4 KV tiles.
-VJ_DEV int page_tok0(const PrefillArgs &a, const int32_t *row, int first, int grp, int lane) {
+// kSplit: with no block tables (row null), the blocks from s0 on in order.
+template <bool kSplit>
+VJ_DEV int page_tok0(const PrefillArgs &a, const int32_t *row, int s0, int first, int grp,
+                     int lane) {
   const int page = first + grp * 32 + lane;
   int blk = 0;
   if (page < a.max_pages) {
-    blk = __ldg(row + page / a.pages_per_block);
+    if (kSplit) blk = row ? row[page / a.pages_per_block] : s0 + page / a.pages_per_block;
+    else blk = __ldg(row + page / a.pages_per_block);
     if (blk < 0 || blk >= a.num_blocks) blk = 0;  // safe_block_tables
   }
   return blk * a.block_size + (page % a.pages_per_block) * kPageTok;
@@ -148,19 +154,19 @@ VJ_DEV int page_tok0(const PrefillArgs &a, const int32_t *row, int first, int gr
 // Stream the K or V tiles of one work item through a ring of `stages`
 // buffers; the whole warp runs this (lanes hold page coordinates), lane 0
 // issues the copies. Returns false if a wait timed out.
-template <int kStagesT>
+template <bool kSplit, int kStagesT>
 VJ_DEV bool produce_kv(const CUtensorMap *tm, uint8_t *ring, uint64_t *full, uint64_t *empty,
                        const PrefillArgs &a, int s, int h, int j0, int nkv, int lane) {
-  const int32_t *row = a.bt + (size_t)s * a.bt_stride;
-  const int first = j0 * kPagesPerTile;
-  int cur = page_tok0(a, row, first, 0, lane);
-  int nxt = nkv > 4 ? page_tok0(a, row, first, 1, lane) : 0;
+  const int32_t *row = kSplit && !a.bt ? nullptr : a.bt + (size_t)s * a.bt_stride;
+  const int first = j0 * kPagesPerTile, s0 = s * a.bt_stride;
+  int cur = page_tok0<kSplit>(a, row, s0, first, 0, lane);
+  int nxt = nkv > 4 ? page_tok0<kSplit>(a, row, s0, first, 1, lane) : 0;
   for (int j = 0; j < nkv; ++j) {
     const int st = j % kStagesT, jj = j & 3;
     const int use = j / kStagesT;
     if (jj == 0 && j > 0) {
       cur = nxt;
-      nxt = j + 4 < nkv ? page_tok0(a, row, first, (j >> 2) + 1, lane) : 0;
+      nxt = j + 4 < nkv ? page_tok0<kSplit>(a, row, s0, first, (j >> 2) + 1, lane) : 0;
     }
     bool ok = true;
     if (use > 0) ok = mbar_wait(&empty[st], (use - 1) & 1);
@@ -200,15 +206,49 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap *tmq_p, const CUt
                                              const CUtensorMap *tmv_p, const PrefillArgs &a,
                                              int s, int h, int m2, uint8_t *smem_raw,
                                              int part = 0) {
-  // (plain loads where the kernel may begin before what writes these is done)
+  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                              ~uintptr_t(1023));
+  Bars &bar = *reinterpret_cast<Bars *>(smem + OFF_BAR);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint32_t tmem = 0;
+  auto setup = [&]() {
+    if (threadIdx.x == 0) {
+      mbar_init(&bar.q_full, 1);
+      for (int i = 0; i < kKStages; ++i) { mbar_init(&bar.k_full[i], 1); mbar_init(&bar.k_empty[i], 1); }
+      for (int i = 0; i < kVStages; ++i) { mbar_init(&bar.v_full[i], 1); mbar_init(&bar.v_empty[i], 1); }
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&bar.s_full[i], 1);
+        mbar_init(&bar.p_full[i], kBM);
+        mbar_init(&bar.o_final[i], 1);
+      }
+      fence_mbar_init();
+    }
+    if (warp == kWarpMma) tmem_alloc(&bar.tmem_base, 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    tmem = bar.tmem_base;
+  };
+  // kSplit: plain loads, since the kernel may begin before what writes these is
+  // done; all of them, and the setup, before the first is waited for
   const int q0 = kSplit ? a.cu[s] : __ldg(a.cu + s);
-  const int n = (kSplit ? a.cu[s + 1] : __ldg(a.cu + s + 1)) - q0;
+  const int q1 = kSplit ? a.cu[s + 1] : __ldg(a.cu + s + 1);
+  int ctx = 0;
+  if constexpr (kSplit) {
+    if (a.ctx_lens) ctx = a.ctx_lens[s];
+    setup();
+  }
+  const int n = q1 - q0;
   const int tq0 = m2 * 2 * a.tt;               // first token of tile A
-  if (tq0 >= n) {        // whole CTA, before any barrier or TMEM use
-    if (kSplit && a.parts == 1) zero_tail_share(a, threadIdx.x, kThreads);
+  if (tq0 >= n) {        // whole CTA, before any barrier (kSplit: wait) or TMEM use
+    if constexpr (kSplit) {
+      if (a.parts == 1) zero_tail_share(a, threadIdx.x, kThreads);
+      __syncwarp();
+      if (warp == kWarpMma) tmem_dealloc(tmem, 512);
+    }
     return;
   }
-  int ctx = a.ctx_lens ? (kSplit ? a.ctx_lens[s] : __ldg(a.ctx_lens + s)) : n;
+  if constexpr (!kSplit) ctx = a.ctx_lens ? __ldg(a.ctx_lens + s) : n;
   if (ctx < n) ctx = n;
   const int p0 = ctx - n;                          // cached prefix length
   const int kv_end = p0 + min(n, tq0 + 2 * a.tt);  // keys visible to the last row of B
@@ -223,31 +263,13 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap *tmq_p, const CUt
         a.part_ml[(static_cast<int64_t>(part) * a.num_tokens + q0 + tq) * a.Hq + h * a.g + r % a.g] =
             make_float2(kLowest, 0.f);
       }
+      __syncwarp();
+      if (warp == kWarpMma) tmem_dealloc(tmem, 512);
       return;
     }
+  } else {
+    setup();
   }
-
-  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
-                                              ~uintptr_t(1023));
-  Bars &bar = *reinterpret_cast<Bars *>(smem + OFF_BAR);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-
-  if (threadIdx.x == 0) {
-    mbar_init(&bar.q_full, 1);
-    for (int i = 0; i < kKStages; ++i) { mbar_init(&bar.k_full[i], 1); mbar_init(&bar.k_empty[i], 1); }
-    for (int i = 0; i < kVStages; ++i) { mbar_init(&bar.v_full[i], 1); mbar_init(&bar.v_empty[i], 1); }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&bar.s_full[i], 1);
-      mbar_init(&bar.p_full[i], kBM);
-      mbar_init(&bar.o_final[i], 1);
-    }
-    fence_mbar_init();
-  }
-  if (warp == kWarpMma) tmem_alloc(&bar.tmem_base, 512);
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = bar.tmem_base;
   bool ok = true;
 
   if (warp == kWarpK) {
@@ -261,10 +283,10 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap *tmq_p, const CUt
         tma_load_3d(smem + OFF_Q + t * kTile + kHalf, tmq_p, &bar.q_full, 64, h * a.g, tok);
       }
     }
-    ok = produce_kv<kKStages>(tmk_p, smem + OFF_K, bar.k_full, bar.k_empty, a, s, h, j0, nkv, lane);
+    ok = produce_kv<kSplit, kKStages>(tmk_p, smem + OFF_K, bar.k_full, bar.k_empty, a, s, h, j0, nkv, lane);
   } else if (warp == kWarpV) {
     // ------------------------------------------------------------ V producer
-    ok = produce_kv<kVStages>(tmv_p, smem + OFF_V, bar.v_full, bar.v_empty, a, s, h, j0, nkv, lane);
+    ok = produce_kv<kSplit, kVStages>(tmv_p, smem + OFF_V, bar.v_full, bar.v_empty, a, s, h, j0, nkv, lane);
     if (kSplit && a.parts == 1) zero_tail_share(a, lane, 32);
   } else if (warp == kWarpMma) {
     // ------------------------------------------------------------ MMA issuer
@@ -526,21 +548,35 @@ attention_mixed_kernel(const __grid_constant__ CUtensorMap tmq,
 }
 
 // Grid: tile pairs, kv heads, (sequence, part). Launched before the kernel ahead is
-// done, and lets the join be made ready.
+// done, and lets the join be made ready. The grid's order is sequence by sequence
+// and head by head, the tile pairs of one side by side, so that they share its K and
+// V in L2; or, where L2 holds all K and V and no head alone fills the GPU, the pairs
+// with the most keys first, which leaves the short ones for the end (2048 tokens
+// after 4096, 32 query heads: 116 -> 96 us; 8 times that with 329 MB of K and V: 1221
+// against 1380 us).
 __global__ void __launch_bounds__(kThreads, 1)
 prefill_split_kernel(const __grid_constant__ CUtensorMap tmq,
                      const __grid_constant__ CUtensorMap tmk,
                      const __grid_constant__ CUtensorMap tmv, PrefillArgs a) {
   extern __shared__ uint8_t smem_raw[];
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(&tmq); tma_prefetch_desc(&tmk); tma_prefetch_desc(&tmv);
+  }
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (a.parts > 1) asm volatile("griddepcontrol.launch_dependents;");
   if (a.num_seqs == 0) {
     zero_tail_share(a, threadIdx.x, kThreads);
     return;
   }
-  const int s = blockIdx.z / a.parts, part = blockIdx.z - s * a.parts;
-  prefill_body<true>(&tmq, &tmk, &tmv, a, s, blockIdx.y, gridDim.x - 1 - blockIdx.x, smem_raw,
-                     part);
+  int x = blockIdx.x, h = blockIdx.y, z = blockIdx.z;
+  if (a.longest_first) {
+    const int others = gridDim.y * gridDim.z, id = x + gridDim.x * (h + gridDim.y * z);
+    x = id / others;
+    h = (id - x * others) % gridDim.y;
+    z = (id - x * others) / gridDim.y;
+  }
+  const int s = z / a.parts, part = z - s * a.parts;
+  prefill_body<true>(&tmq, &tmk, &tmv, a, s, h, gridDim.x - 1 - x, smem_raw, part);
 }
 
 // Joins the parts of the rows [cu[0], cu[num_seqs]) and zeroes those behind. kWarps
@@ -629,7 +665,7 @@ int prefill_setup(const std::string &what, const void *q, const void *k_cache, c
                   int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int64_t num_blocks,
                   int32_t block_size, int32_t bt_width, int32_t bt_stride, int64_t stride_block,
                   int64_t stride_token, int64_t stride_head, int32_t max_seqlen_q, float scale,
-                  int32_t *error_flag, PrefillArgs *args, int64_t *pairs) {
+                  int32_t *error_flag, bool in_order, PrefillArgs *args, int64_t *pairs) {
   *pairs = -1;
   if (num_tokens < 0 || num_seqs < 0 || num_q_heads <= 0 || num_kv_heads <= 0 ||
       num_blocks <= 0 || bt_width < 0 || bt_stride < bt_width) {
@@ -658,7 +694,7 @@ int prefill_setup(const std::string &what, const void *q, const void *k_cache, c
   }
   if (num_tokens == 0) return VJ_OK;
   if (!q || !k_cache || !v_cache || !cu_seqlens_q || !out || !error_flag ||
-      (num_seqs > 0 && !block_tables)) {
+      (num_seqs > 0 && !block_tables && !in_order)) {
     return set_error(VJ_ERR_INVALID_ARGUMENT, what + ": null pointer");
   }
   PrefillArgs &a = *args;
@@ -678,6 +714,7 @@ int prefill_setup(const std::string &what, const void *q, const void *k_cache, c
   a.err = error_flag;
   a.parts = 1;
   a.num_seqs = num_seqs;
+  a.longest_first = 0;
   a.part_o = nullptr;
   a.part_ml = nullptr;
   const int64_t maxq = max_seqlen_q > 0 ? max_seqlen_q : num_tokens;
@@ -735,7 +772,7 @@ extern "C" vj_status vj_paged_prefill(
   int rc = prefill_setup("vj_paged_prefill", q, k_cache, v_cache, block_tables, cu_seqlens_q,
                          context_lens, out, num_tokens, num_seqs, num_q_heads, num_kv_heads,
                          head_dim, num_blocks, block_size, bt_width, bt_stride, stride_block,
-                         stride_token, stride_head, max_seqlen_q, scale, error_flag, &a, &mpairs);
+                         stride_token, stride_head, max_seqlen_q, scale, error_flag, false, &a, &mpairs);
   if (rc || mpairs < 0) return rc;
   rc = prefill_maps(a, q, k_cache, v_cache, stride_token, stride_head, &tmq, &tmk, &tmv);
   if (rc) return rc;
@@ -783,6 +820,9 @@ extern "C" vj_status vj_paged_prefill_split(
   if (max_context_len < 0) {
     return set_error(VJ_ERR_INVALID_ARGUMENT, what + ": negative or zero size");
   }
+  if (!block_tables && static_cast<int64_t>(num_seqs) * bt_stride > INT32_MAX) {
+    return set_error(VJ_ERR_UNSUPPORTED, what + ": sizes beyond 2^31");
+  }
   // the row maximum is taken of q.k, before the scale; 0 times a masked key's -inf is NaN
   if (!(scale > 0.f) || std::isinf(scale)) {
     return set_error(VJ_ERR_INVALID_ARGUMENT, what + ": scale must be positive and finite");
@@ -793,9 +833,11 @@ extern "C" vj_status vj_paged_prefill_split(
   int rc = prefill_setup(what, q, k_cache, v_cache, block_tables, cu_seqlens_q, context_lens, out,
                          num_tokens, num_seqs, num_q_heads, num_kv_heads, head_dim, num_blocks,
                          block_size, bt_width, bt_stride, stride_block, stride_token, stride_head,
-                         max_seqlen_q, scale, error_flag, &a, &mpairs);
+                         max_seqlen_q, scale, error_flag, true, &a, &mpairs);
   if (rc || mpairs < 0) return rc;
   a.parts = prefill_parts(mpairs, num_kv_heads, num_seqs, max_context_len);
+  const int64_t kv_bytes = 2ll * num_seqs * max_context_len * num_kv_heads * kD * 2;
+  a.longest_first = mpairs < num_sms() && kv_bytes <= kResidentKv;
   const int64_t rows = num_tokens * num_q_heads;
   if (a.parts > 1) {
     const size_t need = vj_paged_prefill_split_workspace_size(

@@ -10,7 +10,6 @@
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/sub.h>
-#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -34,7 +33,6 @@ decltype(&vj_paged_prefill_split_workspace_size) prefill_workspace_entry;
 PyObject *native;             // module: check(status), launch_count
 PyObject *error_flag_of;      // (device index) -> address
 PyObject *rope_table_of;      // (device, theta) -> tensor
-PyObject *pages_in_order;     // (device index, n) -> tensor
 
 struct Raised {};             // a Python error is set
 
@@ -132,30 +130,6 @@ int32_t *error_flag(int index) {
   int32_t *p = reinterpret_cast<int32_t *>(integer(address.p));
   if (index < 64) flags[index] = p;
   return p;
-}
-
-// n pages in order, or more of them. What the package keeps stays where it is for
-// good, so its address is remembered; what a capture makes is not kept.
-struct Pages {
-  const int32_t *ptr;
-  int64_t n;
-  PyObject *made;                // a reference to drop after the launches
-};
-Pages in_order(int index, int64_t n) {
-  static Pages kept[64];
-  if (index < 64 && kept[index].n >= n) return kept[index];
-  const bool capturing =
-      c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None;
-  PyObject *made = raise_if_null(
-      PyObject_CallFunction(pages_in_order, "iL", index, static_cast<long long>(n)));
-  const Arg t = tensor(made, "pages");
-  const Pages p = {static_cast<const int32_t *>(t.ptr()), t->numel(), nullptr};
-  if (!capturing && index < 64) {
-    kept[index] = p;
-    Py_DECREF(made);             // the package keeps it
-    return p;
-  }
-  return {p.ptr, p.n, made};
 }
 
 // A C entry without the interpreter's lock; counts its launches, raises its errors.
@@ -491,12 +465,6 @@ PyObject *paged_prefill(PyObject *const *args) {
                                                      hq, p.hkv, p.D, max_new, len);
   const at::Tensor scratch = at::empty(
       {2 * group * len * row + static_cast<int64_t>(split_bytes / 2)}, q->options());
-  const Pages listed = in_order(dev, group * per_seq);
-  struct Drop {
-    PyObject *p;
-    ~Drop() { Py_XDECREF(p); }
-  } const drop{listed.made};
-  const int32_t *const pages = listed.ptr;
   const int32_t *const cu_ptr = static_cast<const int32_t *>(cu.ptr());
   const void *q_ptr = q.ptr();
   void *const out_ptr = out.data_ptr(), *const k_ptr = scratch.data_ptr();
@@ -513,7 +481,7 @@ PyObject *paged_prefill(PyObject *const *args) {
     if (need > split_bytes) more = at::empty({static_cast<int64_t>(need)}, q->options().dtype(at::kByte));
     void *const part_ws = more.defined() ? more.data_ptr() : ws;
     enter(need > 0 ? 2 : 1, [&] {
-      return prefill_entry(q_ptr, k_ptr, static_cast<uint8_t *>(k_ptr) + n * len * row * 2, pages,
+      return prefill_entry(q_ptr, k_ptr, static_cast<uint8_t *>(k_ptr) + n * len * row * 2, nullptr,
                            cu_ptr + s, part.lens, out_ptr, T, n, hq, p.hkv, p.D,
                            static_cast<int64_t>(std::max(n, 1)) * per_seq, kPage, per_seq, per_seq,
                            kPage * row, row, p.D, max_new, len, scale, part_ws, need, err, stream);
@@ -522,7 +490,7 @@ PyObject *paged_prefill(PyObject *const *args) {
   return given ? Py_NewRef(given.o) : THPVariable_Wrap(std::move(out));
 }
 
-// (addresses of the six entries in the order above, then the four objects)
+// (addresses of the six entries in the order above, then the three objects)
 PyObject *bind(PyObject *const *args) {
   store_entry = reinterpret_cast<decltype(store_entry)>(integer(args[0]));
   decode_entry = reinterpret_cast<decltype(decode_entry)>(integer(args[1]));
@@ -533,7 +501,6 @@ PyObject *bind(PyObject *const *args) {
   native = Py_NewRef(args[6]);
   error_flag_of = Py_NewRef(args[7]);
   rope_table_of = Py_NewRef(args[8]);
-  pages_in_order = Py_NewRef(args[9]);
   Py_RETURN_NONE;
 }
 
@@ -559,7 +526,7 @@ PyMethodDef entry(const char *name) {
 }
 PyMethodDef methods[] = {entry<kv_store, 14>("kv_store"), entry<paged_decode, 7>("paged_decode"),
                          entry<read_kv_cache, 5>("read_kv_cache"),
-                         entry<paged_prefill, 10>("paged_prefill"), entry<bind, 10>("bind"),
+                         entry<paged_prefill, 10>("paged_prefill"), entry<bind, 9>("bind"),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_torch_calls", nullptr, -1, methods};
 

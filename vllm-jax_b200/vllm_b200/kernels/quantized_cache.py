@@ -65,7 +65,7 @@ def _bound():
                          ("vj_kv_store_quantized", "vj_paged_decode_quantized",
                           "vj_paged_decode_quantized_workspace_size", "vj_kv_read_quantized",
                           "vj_paged_prefill_split", "vj_paged_prefill_split_workspace_size")),
-                       _native, _error_address, rope_table, _identity_pages)
+                       _native, _error_address, rope_table)
             _calls = calls
     return _calls
 
@@ -123,28 +123,6 @@ def read_kv_cache(cache: QuantizedKVCache, block_tables: torch.Tensor,
     (default: what a block table row holds); longer contexts are cut there."""
     return (_calls or _bound()).read_kv_cache(cache, block_tables, context_lens,
                                               int(max_context_len), out)
-
-
-_identity: dict[int, torch.Tensor] = {}
-_retired_identity: list[torch.Tensor] = []
-
-
-def _identity_pages(index: int, n: int) -> torch.Tensor:
-    """0, 1, .., n - 1 or further, the block tables of a scratch whose pages lie in order, kept
-    per device and only grown. An outgrown tensor is kept too: a captured graph may
-    read it. What a capture makes is the graph's own."""
-    t = _identity.get(index)
-    if t is not None and t.numel() >= n:
-        return t
-    dev = torch.device("cuda", index)
-    if torch.cuda.is_current_stream_capturing():
-        return torch.arange(n, dtype=torch.int32, device=dev)
-    if t is not None:
-        _retired_identity.append(t)
-    # a blocking copy: complete for every stream when it returns
-    t = torch.arange(max(n, 1 << 16), dtype=torch.int32).to(dev)
-    _identity[index] = t
-    return t
 
 
 # bf16 rows (token x KV head) of one read-back inside paged_prefill_quantized:
