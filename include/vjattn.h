@@ -497,7 +497,7 @@ VJ_API vj_status vj_paged_prefill_split(
  * is the smallest power of two that brings the row's largest magnitude to at
  * most 448 (e4m3) or 127 (int8), never below 2^-126 (a row of zeros has that
  * one); a row holding an infinity or NaN has byte 255 and zero elements, and
- * reads as NaN everywhere. A power of two times an element is a bf16 number,
+ * reads as NaN everywhere. No element is e4m3's NaN. A power of two times an element is a bf16 number,
  * so reading the cache back rounds nothing.
  *
  *   elements: (blk,t,h,d) at base + blk*stride_block + t*stride_token +
@@ -565,6 +565,35 @@ VJ_API vj_status vj_paged_decode_quantized(
     int32_t num_kv_heads, int32_t head_dim, int64_t num_blocks, int32_t block_size,
     int32_t bt_width, int32_t bt_stride, int64_t stride_block, int64_t stride_token,
     int64_t stride_head, int64_t scale_stride_block, int64_t scale_stride_head, float scale,
+    void *workspace, size_t workspace_bytes, int32_t *error_flag, cudaStream_t stream);
+
+/* Causal attention of few new tokens over the quantised cache, straight from its
+ * pages: q, out, cu_seqlens_q, context_lens (new tokens included; not NULL),
+ * max_seqlen_q as in vj_paged_prefill, the cache as above. Rows of out behind
+ * cu_seqlens_q[num_seqs] are zeroed. The keys of a row tile (128 rows of tokens x
+ * query heads of one KV head) are split over CTAs that would be idle. Where there
+ * are many row tiles, vj_kv_read_quantized (zero_to = 128, max_len a multiple of
+ * 128) and vj_paged_prefill_split on what it leaves are faster.
+ *   max_context_len: a bound on context_lens, which with max_seqlen_q, the batch
+ *   and the heads decides how far is split
+ *   workspace: vj_paged_prefill_quantized_workspace_size(...) bytes on the current
+ *   device (0 without a split: may be NULL), 16-byte aligned, need not be
+ *   initialised; calls whose kernels may overlap need one each
+ *   scale: positive and finite
+ *   error_flag: device int32 (may be NULL), set to 1 if a wait timed out */
+VJ_API size_t vj_paged_prefill_quantized_workspace_size(int64_t num_tokens, int32_t num_seqs,
+                                                        int32_t num_q_heads,
+                                                        int32_t num_kv_heads, int32_t head_dim,
+                                                        int32_t max_seqlen_q,
+                                                        int32_t max_context_len);
+VJ_API vj_status vj_paged_prefill_quantized(
+    const void *q, const void *k_cache, const void *v_cache, const void *k_scales,
+    const void *v_scales, int32_t cache_dtype, const int32_t *block_tables,
+    const int32_t *cu_seqlens_q, const int32_t *context_lens, void *out, int64_t num_tokens,
+    int32_t num_seqs, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+    int64_t num_blocks, int32_t block_size, int32_t bt_width, int32_t bt_stride,
+    int64_t stride_block, int64_t stride_token, int64_t stride_head, int64_t scale_stride_block,
+    int64_t scale_stride_head, int32_t max_seqlen_q, int32_t max_context_len, float scale,
     void *workspace, size_t workspace_bytes, int32_t *error_flag, cudaStream_t stream);
 
 #ifdef __cplusplus

@@ -82,6 +82,14 @@ def _split(lib, **kw):
     return lib.vj_paged_prefill_split(*a.values())
 
 
+def _prefill(lib, **kw):
+    a = dict(q=16, kc=16, vc=16, ks=16, vs=16, dt=1, bt=16, cu=16, ctx=16, out=16, T=4, S=1, Hq=8,
+             Hkv=2, D=128, nb=200, bs=16, w=200, bts=200, sb=4096, st=256, sh=128, cb=32, ch=16,
+             mq=4, mc=3200, scale=0.1, ws=None, wsb=0, err=None, stream=None)
+    a.update(kw)
+    return lib.vj_paged_prefill_quantized(*a.values())
+
+
 COMMON = [
     (dict(D=64), "UNSUPPORTED", b"head_dim"),
     (dict(dt=0), "INVALID_ARGUMENT", b"cache_dtype"),
@@ -100,7 +108,7 @@ COMMON = [
 ]
 
 
-@pytest.mark.parametrize("entry", [_store, _decode, _read])
+@pytest.mark.parametrize("entry", [_store, _decode, _read, _prefill])
 @pytest.mark.parametrize("kw,status,msg", COMMON)
 def test_refusals_of_every_entry(entry, kw, status, msg):
     from vllm_b200 import _native
@@ -153,6 +161,21 @@ def test_refusals_of_every_entry(entry, kw, status, msg):
     (_read, dict(Hkv=5000, st=128 * 5000, sb=16 * 128 * 5000), "UNSUPPORTED", b"4096"),
     (_read, dict(ko=None), "INVALID_ARGUMENT", b"null"),
     (_read, dict(vo=8), "INVALID_ARGUMENT", b"aligned"),
+    (_prefill, dict(scale=0.0), "INVALID_ARGUMENT", b"positive"),
+    (_prefill, dict(scale=-1.0), "INVALID_ARGUMENT", b"positive"),
+    (_prefill, dict(scale=float("nan")), "INVALID_ARGUMENT", b"positive"),
+    (_prefill, dict(mc=-1), "INVALID_ARGUMENT", b"size"),
+    (_prefill, dict(S=-1), "INVALID_ARGUMENT", b"size"),
+    (_prefill, dict(bts=3), "INVALID_ARGUMENT", b"size"),
+    (_prefill, dict(Hq=7), "INVALID_ARGUMENT", b"divisible"),
+    (_prefill, dict(Hq=12), "UNSUPPORTED", b"divide 128"),
+    (_prefill, dict(q=None), "INVALID_ARGUMENT", b"null"),
+    (_prefill, dict(bt=None), "INVALID_ARGUMENT", b"null"),
+    (_prefill, dict(ctx=None), "INVALID_ARGUMENT", b"null"),
+    (_prefill, dict(q=8), "INVALID_ARGUMENT", b"aligned"),
+    (_prefill, dict(), "WORKSPACE", b"workspace"),
+    (_prefill, dict(ws=8, wsb=1 << 30), "WORKSPACE", b"workspace"),
+    (_prefill, dict(S=70000), "UNSUPPORTED", b"grid"),
     (_split, dict(scale=0.0), "INVALID_ARGUMENT", b"positive"),
     (_split, dict(scale=-1.0), "INVALID_ARGUMENT", b"positive"),
     (_split, dict(scale=float("nan")), "INVALID_ARGUMENT", b"positive"),
@@ -180,6 +203,7 @@ def test_empty_calls_need_no_memory():
     assert _store(lib, T=0, **none) == 0
     assert _decode(lib, B=0, **none) == 0
     assert _read(lib, B=0, **none) == 0
+    assert _prefill(lib, T=0, **none) == 0
     size = lib.vj_paged_decode_quantized_workspace_size
     assert size(4, 8, 2, 64, 4, 16) == size(4, 8, 2, 128, 4, 0) == size(4, 0, 2, 128, 4, 16) == 0
     assert 16 <= size(4, 8, 2, 128, 4, 16) <= size(400, 8, 2, 128, 4000, 16)

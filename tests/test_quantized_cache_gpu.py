@@ -407,12 +407,12 @@ def test_layouts_and_strides(dtype):
     qp = _t(bf16(rng.standard_normal((30, 8, D))))
     cu, ln = _i([0, 10, 20, 30]), _i(lens)
     ref = (paged_decode_quantized(q, a, _i(bt), ln), read_kv_cache(a, _i(bt), ln),
-           paged_prefill_quantized(qp, a, _i(bt), cu, ln))
+           paged_prefill_quantized(qp, a, _i(bt), cu, ln, 10))
     for c in (QuantizedKVCache(head_major, a.scales),
               QuantizedKVCache(wide[:, :, :, 1:H + 1].view(TORCH[dtype]), wide_s[:, :, 2:H + 2])):
         t = tables[:, 5:18]
         got = (paged_decode_quantized(q, c, t, ln), read_kv_cache(c, t, ln),
-               paged_prefill_quantized(qp, c, t, cu, ln))
+               paged_prefill_quantized(qp, c, t, cu, ln, 10))
         for x, y in zip(got, ref):
             assert torch.equal(x, y)
 
@@ -477,15 +477,17 @@ def test_prefill_matches_oracle(Hq, Hkv, bs, new, prefix, dtype, monkeypatch):
     assert torch.equal(got, again)
 
 
-def test_prefill_scratch_garbage_does_not_matter():
+@pytest.mark.parametrize("lens", [(70, 1, 129), (900, 1, 1029)])
+def test_prefill_scratch_garbage_does_not_matter(lens):
     """The scratch comes uninitialised: memory full of NaN gives the same bits."""
     from vllm_b200.kernels import quantized_cache as qc
     rng = np.random.default_rng(20)
-    lens = [70, 1, 129]
-    codes, scales = _random_pool(rng, 20, 16, 2, "e4m3")
-    bt = _tables(rng, lens, 20, 16, 9)
-    q = _t(bf16(rng.standard_normal((200, 4, D))))
-    args = (q, _cache(codes, scales, "e4m3"), _i(bt), _i([0, 70, 71, 200]), _i(lens), 129)
+    need = sum(-(-n // 16) for n in lens)
+    codes, scales = _random_pool(rng, need, 16, 2, "e4m3")
+    bt = _tables(rng, lens, need, 16, -(-max(lens) // 16))
+    q = _t(bf16(rng.standard_normal((sum(lens), 16, D))))
+    args = (q, _cache(codes, scales, "e4m3"), _i(bt), _i(np.cumsum((0,) + lens)), _i(lens),
+            max(lens))
     a = qc.paged_prefill_quantized(*args)
     junk = [torch.full((1 << 22,), float("nan"), device="cuda") for _ in range(8)]
     torch.cuda.synchronize()
@@ -502,6 +504,8 @@ def test_prefill_scratch_garbage_does_not_matter():
     (8, 1, 16, [300], [1400]),                  # parts that early rows see nothing of
     (16, 1, 48, [700], [2500]),
     (12, 3, 16, [1, 1, 1, 1], [3000, 1023, 1024, 1025]),
+    (32, 8, 16, [256], [2500]),                 # these two are read back first
+    (8, 1, 32, [900, 40], [1400, 9]),
 ])
 def test_prefill_split_over_keys_matches_oracle(Hq, Hkv, bs, new, prefix, dtype):
     """Few new tokens after long prefixes; scratch full of NaN; the same bits again."""
@@ -516,8 +520,9 @@ def test_prefill_split_over_keys_matches_oracle(Hq, Hkv, bs, new, prefix, dtype)
     T = int(cu[-1])
     q = bf16(rng.standard_normal((T + 5, Hq, D)))          # five padding rows
     args = (_t(q), _cache(codes, scales, dtype), _i(bt), _i(cu), _i(ctx), max(new))
-    assert _native.load().vj_paged_prefill_split_workspace_size(T + 5, len(new), Hq, Hkv, D,
-                                                                max(new), max(ctx)) > 0
+    sizes = (T + 5, len(new), Hq, Hkv, D, max(new), max(ctx))
+    assert _native.load().vj_paged_prefill_split_workspace_size(*sizes) > 0
+    assert _native.load().vj_paged_prefill_quantized_workspace_size(*sizes) > 0 or max(new) > 500
     junk = [torch.full((1 << 22,), float("nan"), device="cuda") for _ in range(8)]
     torch.cuda.synchronize()
     del junk
@@ -534,36 +539,41 @@ def test_prefill_split_over_keys_matches_oracle(Hq, Hkv, bs, new, prefix, dtype)
         assert torch.equal(got, qc.paged_prefill_quantized(*args, max_context_len=max(ctx)))
 
 
+@pytest.mark.parametrize("longest", [2, 0, 800])
 @pytest.mark.parametrize("S,new", [(0, 0), (3, 0), (1, 2)])
-def test_prefill_rows_behind_the_last_sequence_are_zeroed(S, new):
-    """Also where there is no sequence, or none has new tokens."""
+def test_prefill_rows_behind_the_last_sequence_are_zeroed(S, new, longest):
+    """Also where there is no sequence, or none has new tokens; for every way there is
+    (the bound on the new tokens chooses)."""
     from vllm_b200.kernels.quantized_cache import QuantizedKVCache, paged_prefill_quantized
     cache = QuantizedKVCache.zeros(8, 16, 2, device="cuda")
     cache.data.view(torch.uint8).fill_(0x38)                   # ones
-    q = torch.ones((1000, 4, D), dtype=torch.bfloat16, device="cuda")
+    q = torch.ones((1000, 16, D), dtype=torch.bfloat16, device="cuda")
     out = torch.full_like(q, float("nan"))
     paged_prefill_quantized(q, cache, _i(np.zeros((S, 2))), _i(np.arange(S + 1) * new),
-                            _i(np.full(S, new)), new, out=out)
+                            _i(np.full(S, new)), longest, out=out,
+                            max_context_len=16 if longest == 2 else 0)
     assert (out[:S * new] == 1).all() and not out[S * new:].any()
 
 
-@pytest.mark.parametrize("prefix", [0, 2000])
-def test_prefill_nan_row_stays_in_its_sequence(prefix):
+@pytest.mark.parametrize("prefix,new", [(0, (5, 7)), (2000, (5, 7)), (2000, (300, 310)),
+                                        (0, (1300, 1240))])
+def test_prefill_nan_row_stays_in_its_sequence(prefix, new):
     """A NaN row in the first page of the first sequence, whose block every unused table
     entry stands for."""
     from vllm_b200.kernels.quantized_cache import paged_prefill_quantized
     rng = np.random.default_rng(23)
-    new, ctx = [5, 7], [prefix + 5, prefix + 7]
+    ctx = [prefix + n for n in new]
     need = [-(-n // 16) for n in ctx]
     codes, scales = _random_pool(rng, sum(need), 16, 2, "e4m3")
     codes[:, 0, 0], scales[:, 0, :, 0] = 0, 255
-    bt = np.full((2, need[1] + 3), -1, np.int32)
+    bt = np.full((2, max(need) + 3), -1, np.int32)
     bt[0, :need[0]] = np.arange(need[0])
     bt[1, :need[1]] = need[0] + np.arange(need[1])
-    q = _t(bf16(rng.standard_normal((12, 4, D))))
-    out = paged_prefill_quantized(q, _cache(codes, scales, "e4m3"), _i(bt), _i([0, 5, 12]),
+    a, T = new[0], sum(new)
+    q = _t(bf16(rng.standard_normal((T, 16, D))))
+    out = paged_prefill_quantized(q, _cache(codes, scales, "e4m3"), _i(bt), _i([0, a, T]),
                                   _i(ctx), max(new))
-    assert torch.isnan(out[:5]).all() and torch.isfinite(out[5:]).all()
+    assert torch.isnan(out[:a]).all() and torch.isfinite(out[a:]).all()
 
 
 # ----------------------------------------------------------------------------- streams, graphs
@@ -695,7 +705,7 @@ def test_calls_keep_nothing_and_count_their_launches():
     for _ in range(20):
         calls()
     torch.cuda.synchronize()
-    assert _native.launch_count - before == 20 * (1 + 2 + 2 + 1 + 2)
+    assert _native.launch_count - before == 20 * (1 + 2 + 2 + 1 + 1)
     assert torch.cuda.memory_allocated() == mem
     assert [sys.getrefcount(x) for x in things] == refs
 

@@ -39,6 +39,7 @@
 // CTAs. Each leaves its rows' sums in 32 bits, not normalised, with their maximum
 // and sum of weights, and prefill_join_kernel joins them.
 #include "../../include/vjattn.h"
+#include "prefill_join.cuh"
 #include "vj_common.cuh"
 
 #include <algorithm>
@@ -133,7 +134,6 @@ struct PrefillArgs {
   float *part_o;            // [parts][tokens][Hq][128]
   float2 *part_ml;          // [parts][tokens][Hq] maximum (log2), sum
 };
-constexpr float kLowest = -1e30f;       // a maximum that no key has moved yet
 
 // Token coordinate (flat pool token index of the page's first token) of page
 // first + grp*32 + lane of sequence s: one coalesced block-table read per 4 KV tiles.
@@ -184,19 +184,6 @@ VJ_DEV bool produce_kv(const CUtensorMap *tm, uint8_t *ring, uint64_t *full, uin
     }
   }
   return true;
-}
-
-// This CTA's share of the rows past cu_seqlens_q[num_seqs] -> 0, by n of its threads.
-VJ_DEV void zero_tail_share(const PrefillArgs &a, int i, int n) {
-  const int64_t per_row = static_cast<int64_t>(a.Hq) * (kD / 8), from = a.cu[a.num_seqs] * per_row;
-  const int64_t tail = a.num_tokens * per_row - from;
-  if (tail <= 0) return;
-  const int64_t cta = (static_cast<int64_t>(blockIdx.z) * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x;
-  const int64_t ctas = static_cast<int64_t>(gridDim.x) * gridDim.y * gridDim.z;
-  uint4 *o = reinterpret_cast<uint4 *>(a.out) + from;
-  for (int64_t k = tail * cta / ctas + i; k < tail * (cta + 1) / ctas; k += n) {
-    o[k] = make_uint4(0u, 0u, 0u, 0u);
-  }
 }
 
 // The work of one CTA: tile pair m2 of (sequence s, kv head h), and with kSplit
@@ -579,65 +566,6 @@ prefill_split_kernel(const __grid_constant__ CUtensorMap tmq,
   prefill_body<true>(&tmq, &tmk, &tmv, a, s, h, gridDim.x - 1 - x, smem_raw, part);
 }
 
-// Joins the parts of the rows [cu[0], cu[num_seqs]) and zeroes those behind. kWarps
-// warps take a (token, query head), each every kWarps-th part, four of them in flight.
-constexpr int kJoinWarps = 8;
-template <int kWarps>
-__global__ void __launch_bounds__(kJoinWarps * 32)
-prefill_join_kernel(const PrefillArgs a) {
-  __shared__ float4 so[kJoinWarps][32];
-  __shared__ float2 sml[kJoinWarps];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, w = warp % kWarps;
-  const int64_t rows = static_cast<int64_t>(a.num_tokens) * a.Hq;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kJoinWarps / kWarps) + warp / kWarps;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int64_t first = static_cast<int64_t>(a.cu[0]) * a.Hq;
-  const int64_t end = static_cast<int64_t>(a.cu[a.num_seqs]) * a.Hq;
-  uint2 *dst = reinterpret_cast<uint2 *>(a.out + row * kD) + lane;
-  const bool mine = row >= first && row < end && row < rows;
-  if (row >= end && row < rows && w == 0) *dst = make_uint2(0u, 0u);
-  float m = kLowest, l = 0.f;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  auto add = [&](float2 ml, float4 x) {
-    if (ml.y == 0.f) return;            // no key of the part: its sums may not be there
-    const float top = fmaxf(m, ml.x), f0 = exp2f(m - top), f1 = exp2f(ml.x - top);
-    m = top;
-    l = fmaf(ml.y, f1, l * f0);
-    o.x = fmaf(x.x, f1, o.x * f0); o.y = fmaf(x.y, f1, o.y * f0);
-    o.z = fmaf(x.z, f1, o.z * f0); o.w = fmaf(x.w, f1, o.w * f0);
-  };
-  if (mine) {
-    constexpr int kFly = 4;
-    for (int i0 = w; i0 < a.parts; i0 += kFly * kWarps) {
-      float2 ml[kFly];
-      float4 x[kFly];
-#pragma unroll
-      for (int k = 0; k < kFly; ++k) {
-        const int i = i0 + k * kWarps;
-        ml[k] = make_float2(kLowest, 0.f);
-        x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (i < a.parts) {
-          const int64_t at = i * rows + row;
-          ml[k] = a.part_ml[at];
-          x[k] = reinterpret_cast<const float4 *>(a.part_o + at * kD)[lane];
-        }
-      }
-#pragma unroll
-      for (int k = 0; k < kFly; ++k) add(ml[k], x[k]);
-    }
-  }
-  if constexpr (kWarps > 1) {
-    so[warp][lane] = o;
-    if (lane == 0) sml[warp] = make_float2(m, l);
-    __syncthreads();
-    if (w != 0) return;
-    for (int k = 1; k < kWarps; ++k) add(sml[warp + k], so[warp + k][lane]);
-  }
-  if (!mine) return;
-  const float inv = 1.f / l;
-  *dst = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
-}
-
 // Rows of the packed output past cu_seqlens_q[num_seqs] (bucket padding) -> 0,
 // as the reference's scatter leaves them (prefill_paged_attention.py:384-388).
 __global__ void prefill_zero_tail_kernel(__nv_bfloat16 *out, const int32_t *cu, int num_seqs,
@@ -870,11 +798,7 @@ extern "C" vj_status vj_paged_prefill_split(
   rc = launch_dependent(what.c_str(), prefill_split_kernel, grid, kThreads, kSmemBytes, stream, tmq,
                         tmk, tmv, a);
   if (rc || a.parts == 1) return rc;
-  // few rows: eight warps each
-  const bool few = rows <= 8 * num_sms();
-  const int64_t blocks = few ? rows : (rows + kJoinWarps - 1) / kJoinWarps;
-  return launch_dependent(what.c_str(), few ? prefill_join_kernel<kJoinWarps> : prefill_join_kernel<1>,
-                          dim3(static_cast<unsigned>(blocks)), kJoinWarps * 32, 0, stream, a);
+  return launch_join(what.c_str(), a, stream);
 }
 
 extern "C" size_t vj_paged_attention_mixed_workspace_size(int32_t num_decode,

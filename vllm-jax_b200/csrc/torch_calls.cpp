@@ -8,6 +8,7 @@
 #include <Python.h>
 
 #include <ATen/core/Tensor.h>
+#include <ATen/cuda/CUDAContextLight.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/sub.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -30,6 +31,8 @@ decltype(&vj_paged_decode_quantized_workspace_size) workspace_entry;
 decltype(&vj_kv_read_quantized) read_entry;
 decltype(&vj_paged_prefill_split) prefill_entry;
 decltype(&vj_paged_prefill_split_workspace_size) prefill_workspace_entry;
+decltype(&vj_paged_prefill_quantized) direct_entry;
+decltype(&vj_paged_prefill_quantized_workspace_size) direct_workspace_entry;
 PyObject *native;             // module: check(status), launch_count
 PyObject *error_flag_of;      // (device index) -> address
 PyObject *rope_table_of;      // (device, theta) -> tensor
@@ -263,6 +266,7 @@ Tables tables(const Arg &bt, const Arg &lens, int64_t B) {
   return t;
 }
 
+int num_sms() { return at::cuda::getCurrentDeviceProperties()->multiProcessorCount; }
 cudaStream_t stream_of(int index) { return c10::cuda::getCurrentCUDAStream(index).stream(); }
 
 // (q, k, v, cache, slot_mapping, positions, q_norm_weight, k_norm_weight, eps,
@@ -420,6 +424,19 @@ PyObject *read_kv_cache(PyObject *const *args) {
   return given ? Py_NewRef(given.o) : THPVariable_Wrap(std::move(out));
 }
 
+// Whether to take the pages in directly instead of reading the contexts back first:
+// every row tile (128 rows) of a sequence and head converts its keys again, which pays
+// while there is one of them, or few in all, or one wave of them with short contexts.
+// Read back / direct, us, B200, 32 / 8 heads: 1 token after 4096 15.5 / 12.9; 32
+// sequences of 20 after up to 300 30.7 / 24.2; 2 x 256 after up to 1000 22.6 / 19.9; 256
+// after 4096 27.3 / 29.2; 2 x 600 after 4096 66 / 97.
+bool direct_prefill(int64_t S, int64_t T, int64_t hq, const Pool &p, int64_t longest, int64_t len) {
+  if (128 % (hq / p.hkv) != 0) return false;         // the other way refuses it
+  const int64_t tt = 128 / (hq / p.hkv), tiles = (longest + tt - 1) / tt;
+  const int64_t ctas = std::min(tiles * S, T / tt + S) * p.hkv;
+  return tiles == 1 || ctas <= 32 || (ctas <= num_sms() && len <= 768);
+}
+
 // (q, cache, block_tables, cu_seqlens_q, context_lens, max_seqlen_q, scale, out,
 //  max_context_len, scratch_rows)
 PyObject *paged_prefill(PyObject *const *args) {
@@ -454,23 +471,36 @@ PyObject *paged_prefill(PyObject *const *args) {
       i32(std::max<int64_t>((most + kKeyTile - 1) / kKeyTile, 1) * kKeyTile, "max_context_len");
   const float scale = static_cast<float>(args[6] == Py_None ? 1.0 / std::sqrt(p.D) : number(args[6]));
   at::Tensor out = output(given, q);
+  const int64_t T = q->size(0);
+  const void *q_ptr = q.ptr();
+  void *const out_ptr = out.data_ptr();
+  const int32_t *const cu_ptr = static_cast<const int32_t *>(cu.ptr());
+  int32_t *const err = error_flag(dev);
+  const cudaStream_t stream = stream_of(dev);
+  if (direct_prefill(S, T, hq, p, max_new > 0 ? max_new : T, len)) {
+    const size_t need = direct_workspace_entry(T, S, hq, p.hkv, p.D, max_new, len);
+    at::Tensor ws;
+    if (need) ws = at::empty({static_cast<int64_t>(need)}, q->options().dtype(at::kByte));
+    void *const ws_ptr = need ? ws.data_ptr() : nullptr;
+    enter(need ? 2 : 1, [&] {
+      return direct_entry(q_ptr, p.k, p.v, p.ks, p.vs, p.code, t.ptr, cu_ptr, t.lens, out_ptr, T, S,
+                          hq, p.hkv, p.D, p.nb, p.bs, t.width, t.stride, p.sb, p.st, p.sh, p.cb,
+                          p.ch, max_new, len, scale, ws_ptr, need, err, stream);
+    });
+    return given ? Py_NewRef(given.o) : THPVariable_Wrap(std::move(out));
+  }
   // the scratch: K and V, where page i of a group's sequence b is block b * per_seq
   // + i, then what a split over keys needs
   const int64_t row = static_cast<int64_t>(p.hkv) * p.D;
   const int64_t group = std::max<int64_t>(
       1, std::min<int64_t>(S, integer(args[9]) / (static_cast<int64_t>(len) * p.hkv)));
   const int32_t per_seq = len / kPage;
-  const int64_t T = q->size(0);
   const size_t split_bytes = prefill_workspace_entry(T, static_cast<int32_t>(std::min<int64_t>(group, S)),
                                                      hq, p.hkv, p.D, max_new, len);
   const at::Tensor scratch = at::empty(
       {2 * group * len * row + static_cast<int64_t>(split_bytes / 2)}, q->options());
-  const int32_t *const cu_ptr = static_cast<const int32_t *>(cu.ptr());
-  const void *q_ptr = q.ptr();
-  void *const out_ptr = out.data_ptr(), *const k_ptr = scratch.data_ptr();
+  void *const k_ptr = scratch.data_ptr();
   void *const ws = static_cast<uint8_t *>(k_ptr) + 4 * group * len * row;
-  int32_t *const err = error_flag(dev);
-  const cudaStream_t stream = stream_of(dev);
   for (int64_t s = 0; s < std::max(S, 1); s += group) {
     const int32_t n = static_cast<int32_t>(std::min<int64_t>(group, S - s));
     const Tables part = {t.ptr + s * t.stride, t.lens + s, t.width, t.stride};
@@ -490,7 +520,7 @@ PyObject *paged_prefill(PyObject *const *args) {
   return given ? Py_NewRef(given.o) : THPVariable_Wrap(std::move(out));
 }
 
-// (addresses of the six entries in the order above, then the three objects)
+// (addresses of the eight entries in the order above, then the three objects)
 PyObject *bind(PyObject *const *args) {
   store_entry = reinterpret_cast<decltype(store_entry)>(integer(args[0]));
   decode_entry = reinterpret_cast<decltype(decode_entry)>(integer(args[1]));
@@ -498,9 +528,11 @@ PyObject *bind(PyObject *const *args) {
   read_entry = reinterpret_cast<decltype(read_entry)>(integer(args[3]));
   prefill_entry = reinterpret_cast<decltype(prefill_entry)>(integer(args[4]));
   prefill_workspace_entry = reinterpret_cast<decltype(prefill_workspace_entry)>(integer(args[5]));
-  native = Py_NewRef(args[6]);
-  error_flag_of = Py_NewRef(args[7]);
-  rope_table_of = Py_NewRef(args[8]);
+  direct_entry = reinterpret_cast<decltype(direct_entry)>(integer(args[6]));
+  direct_workspace_entry = reinterpret_cast<decltype(direct_workspace_entry)>(integer(args[7]));
+  native = Py_NewRef(args[8]);
+  error_flag_of = Py_NewRef(args[9]);
+  rope_table_of = Py_NewRef(args[10]);
   Py_RETURN_NONE;
 }
 
@@ -526,7 +558,7 @@ PyMethodDef entry(const char *name) {
 }
 PyMethodDef methods[] = {entry<kv_store, 14>("kv_store"), entry<paged_decode, 7>("paged_decode"),
                          entry<read_kv_cache, 5>("read_kv_cache"),
-                         entry<paged_prefill, 10>("paged_prefill"), entry<bind, 9>("bind"),
+                         entry<paged_prefill, 10>("paged_prefill"), entry<bind, 11>("bind"),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_torch_calls", nullptr, -1, methods};
 

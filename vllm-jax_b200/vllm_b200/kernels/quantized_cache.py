@@ -64,7 +64,9 @@ def _bound():
             calls.bind(*(_native.address(name) for name in
                          ("vj_kv_store_quantized", "vj_paged_decode_quantized",
                           "vj_paged_decode_quantized_workspace_size", "vj_kv_read_quantized",
-                          "vj_paged_prefill_split", "vj_paged_prefill_split_workspace_size")),
+                          "vj_paged_prefill_split", "vj_paged_prefill_split_workspace_size",
+                          "vj_paged_prefill_quantized",
+                          "vj_paged_prefill_quantized_workspace_size")),
                        _native, _error_address, rope_table)
             _calls = calls
     return _calls
