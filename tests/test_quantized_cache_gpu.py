@@ -477,6 +477,30 @@ def test_prefill_matches_oracle(Hq, Hkv, bs, new, prefix, dtype, monkeypatch):
     assert torch.equal(got, again)
 
 
+@pytest.mark.parametrize("dtype", ["e4m3", "int8"])
+def test_prefill_of_every_code_and_scale(dtype):
+    """One token that sees itself alone: its result is its V row, whatever element and
+    scale, and NaN for byte 255. Where the row's value leaves bf16's range or its normal
+    numbers, it is what reading back gives."""
+    from vllm_b200.kernels.quantized_cache import paged_prefill_quantized, read_kv_cache
+    S = 512
+    codes = np.zeros((2, S, 16, 1, D), np.uint8)
+    codes[1, :, 0, 0] = np.arange(2 * D).reshape(2, D)[np.arange(S) % 2]
+    if dtype == "e4m3":
+        codes = np.where((codes & 127) == 127, 0, codes)      # no NaN codes
+    scales = np.full((2, S, 1, 16), 127, np.uint8)
+    scales[1, :, 0, 0] = np.arange(S) // 2
+    codes[1, 510:, 0] = 0
+    cache, bt = _cache(codes, scales, dtype), _i(np.arange(S)[:, None])
+    one, cu = _i(np.ones(S)), _i(np.arange(S + 1))
+    q = _t(bf16(np.random.default_rng(24).standard_normal((S, 2, D))))
+    out = paged_prefill_quantized(q, cache, bt, cu, one, 1)
+    ref = read_kv_cache(cache, bt, one, 1)[1, :, 0]           # [S, 1, D]
+    assert torch.equal(out.nan_to_num(7.0, 1e38, -1e38),
+                       ref.expand(S, 2, D).nan_to_num(7.0, 1e38, -1e38))
+    assert torch.isnan(out[510:]).all() and torch.isfinite(out[:480]).all()
+
+
 @pytest.mark.parametrize("lens", [(70, 1, 129), (900, 1, 1029)])
 def test_prefill_scratch_garbage_does_not_matter(lens):
     """The scratch comes uninitialised: memory full of NaN gives the same bits."""

@@ -2,26 +2,25 @@
 // attention of each sequence's new tokens over its cached context.
 //
 // A tile of 128 rows (tokens x query heads of one KV head) meets key tiles of 128 on
-// tcgen05.mma in bf16. Two groups of four warps read the pages and write bf16 tiles to
-// shared memory, element times scale, which rounds nothing: 8 lanes read a row of 128
-// bytes, and an element pair goes from e4m3 or int8 to f16, from there to bf16 by
-// moving its bits (a bf16 with f16's exponent is the number times 2^-112), and gets
-// 2^112 and the row's scale in one product. Reading the context back to bf16 in a
-// launch of its own and taking it in from there does that work once instead of once
-// per row tile, and costs its launch and 4 bytes per element of traffic: the caller
-// takes that way where there are many row tiles.
+// tcgen05.mma in bf16. Eight warps read the pages and write bf16 tiles to shared memory,
+// element times scale, which rounds nothing; 8 lanes read a row of 128 bytes. Reading
+// the context back to bf16 in a launch of its own and taking it in from there does that
+// work once instead of once per row tile, and costs its launch and 4 bytes per element
+// of traffic: the caller takes that way where there are many row tiles.
 //   The keys of a row tile are split over as many CTAs as leave no SM idle; their
 // results are joined by prefill_join_kernel.
 //
-//   TMEM columns: [0,128) S of even key tiles | [128,256) of odd ones | [256,384) O;
-//   P (bf16 pairs) overwrites the first half of its S.
-// Warps: 0-3 softmax (a row a thread), 4-7 K tiles, 8-11 V tiles, 12 the products
-// (and q by TMA). S(j+1) is computed while the softmax of S(j) runs; O is rescaled
-// only where a row's maximum grows by more than 2^8, and then behind PV(j - 1).
+//   TMEM columns: [0,128) S of even key tiles | [128,256) of odd ones | [256,384) O of
+//   the first 64 keys of every tile | [384,512) of the others; P (bf16 pairs) overwrites
+//   the first half of its 64 columns of S.
+// Warps: 0-3 softmax of the first 64 keys of a tile (a row a thread), 4-7 of the others,
+// 8-11 K tiles, 12-15 V tiles, 16 the products (and q by TMA). The two halves are two softmaxes
+// with maxima, sums and outputs of their own, joined at the end: one thread a row took
+// 2.1 us a key tile, since one warp is then all that a quarter of the SM has for it.
+// S(j+1) is computed while the softmax of S(j) runs; O is rescaled only where a row's
+// maximum grows by more than 2^8, and then behind PV(j - 1).
 // Latency-bound: a few key tiles a CTA, each load -> convert -> scores -> softmax ->
-// product (2.1 us a key tile in the steady state, of which leaving out the conversion,
-// the loads or the softmax saves 0.2 to 0.4 each). 13 warps leave 128 registers a
-// thread, so the softmax takes the scores twice, half of them at a time.
+// product.
 //   One token after 1421 cached ones, 32 / 8 heads: 13 us (15.5 with the context read
 // back first); 32 after 11129: 25 (36); four prompts of up to 300 tokens: 14 (16.4).
 #include "prefill_join.cuh"
@@ -30,6 +29,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cmath>
+#include <type_traits>
 
 namespace vj {
 namespace {
@@ -40,9 +40,11 @@ constexpr int kHalfTile = 128 * 128;           // 128 rows of 64 bf16, 128-byte 
 constexpr int kTileBytes = 2 * kHalfTile;
 constexpr int kRing = 2;                       // tiles of K, and of V
 constexpr int kOffK = kTileBytes, kOffV = kOffK + kRing * kTileBytes;
-constexpr int kOffBars = kOffV + kRing * kTileBytes;
-constexpr int kPrefillThreads = 13 * 32;
-constexpr uint32_t kColO = 256;
+// pages on their way: [2 tiles][K, V][4 warps][8 pages][32 lanes] 16 bytes
+constexpr int kOffRaw = kOffV + kRing * kTileBytes, kRawHalf = 4 * 8 * 512;
+constexpr int kOffBars = kOffRaw + 4 * kRawHalf;
+constexpr int kPrefillThreads = 17 * 32;
+constexpr uint32_t kColO = 256;                // + 128 for the second half of the keys
 constexpr float kGrow = 8.0f;                  // log2 of what a maximum may grow by unseen
 
 struct PrefillBars {
@@ -51,6 +53,7 @@ struct PrefillBars {
   uint32_t tmem;
 };
 constexpr size_t kPrefillSmem = 1024 + kOffBars + sizeof(PrefillBars);
+static_assert(kPrefillSmem <= 227 * 1024, "shared memory");
 
 struct QPrefillArgs {
   Pool pool;
@@ -70,23 +73,87 @@ VJ_DEV uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
   asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
   return d;
 }
-// An f16 pair (of at most 8 significant bits) as the bf16 pair of 2^-112 times it.
-VJ_DEV uint32_t f16_as_bf16(uint32_t y) { return (y & 0x80008000u) | ((y & 0x7fff7fffu) >> 3); }
+VJ_DEV void sts128(uint32_t addr, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(x), "r"(y), "r"(z), "r"(w)
+               : "memory");
+}
+VJ_DEV uint4 lds128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+// 16 bytes from global to shared memory, of which `bytes` (0 or 16) are read, the rest 0.
+VJ_DEV void cp_async16(uint32_t dst, const void *src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
+               : "memory");
+}
+VJ_DEV void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kLeft>
+VJ_DEV void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory"); }
+VJ_DEV uint32_t sub_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+VJ_DEV float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 
-// The K (or V) tiles of one CTA into their ring, by one group of four warps: warp cw
-// takes rows 4 cw .. + 3 of every page, 8 lanes a row. `limit`: tokens from there on are
-// zeros. False if a wait ran out.
+// What brings a pair of to_bf16 to its value times the row's scale, and the byte up to
+// which one bf16 number holds it (beyond: 2^127 and the rest). NaN for byte 255.
 template <bool kInt8>
-VJ_DEV bool convert_tiles(const QPrefillArgs &a, const uint8_t *rows, const uint8_t *scales,
-                          uint8_t *ring, uint64_t *full, uint64_t *empty, int s, int j0, int n,
-                          int limit, int cw, int lane) {
+constexpr uint32_t kScaleUp = kInt8 ? 0 : 120;
+template <bool kInt8>
+VJ_DEV uint32_t scale_pair(uint32_t byte) {
+  const uint32_t b = byte == 255u ? 0x7fffu
+                     : kInt8 && byte == 0u ? 0x0040u               // 2^-127
+                                           : min(byte + kScaleUp<kInt8>, 254u) << 7;
+  return b * 0x10001u;
+}
+// The elements in the low or high half of a word as a pair of bf16 numbers, exactly.
+// int8: 128 + its low 7 bits, less 128 or (negative) 256. e4m3: 2^-120 times it, since
+// bf16 gives the 4 bits of the exponent 2^(x - 127) instead of 2^(x - 7). (By way of
+// f16, whose bits are moved, it takes twice the instructions of the busiest pipe.)
+template <bool kInt8, bool kHi>
+VJ_DEV uint32_t to_bf16(uint32_t w) {
+  uint32_t y;                                  // a byte in each half
+  asm("prmt.b32 %0, %1, 0, %2;" : "=r"(y) : "r"(w), "n"(kHi ? 0x4342 : 0x4140));
+  if constexpr (kInt8) {
+    return sub_bf16x2((y & 0x007f007fu) | 0x43004300u, (y & 0x00800080u) | 0x43004300u);
+  } else {
+    return y * 16u + (y & 0x00800080u) * 240u;   // sign to bit 15, the rest to bits 10 .. 4
+  }
+}
+
+// The K (v = 0) or V tiles of one CTA into their ring, by four warps: warp cw takes rows
+// 4 cw .. + 3 of every page, 8 lanes a row. `limit`: tokens from there on are zeros.
+// False if a wait ran out.
+template <bool kInt8>
+VJ_DEV bool convert_tiles(const QPrefillArgs &a, uint8_t *smem, PrefillBars &bar, int v, int s, int h,
+                          int j0, int n, int limit, int cw, int lane) {
   const int c = lane & 7, r0 = 4 * cw + (lane >> 3);
   const bool upper = c >= 4;                   // dims 64 and up
   const int32_t *bt = a.bt + static_cast<int64_t>(s) * a.bt_stride;
-  uint4 x[8];
-  uint32_t sc[8];
-  // where page `lane & 7` of a key tile lies: looked up a tile before its loads
-  int64_t at_rows = 0, at_scales = 0;
+  const int64_t row_at = h * a.pool.sh + r0 * a.pool.st + c * 16, scale_at = h * a.pool.ssh + 4 * cw;
+  // where this lane's 32 bytes of bf16 go in a tile (16 rows on, the swizzle is the same).
+  // The half of the lanes that has dims 64 and up starts with its second 16 bytes, so
+  // that 8 lanes store to 8 different bank groups.
+  const uint32_t to = smem_u32(smem) + (upper ? kHalfTile : 0);
+  const uint32_t to0 = to + sw128(r0, 2 * (c & 3) + (upper ? 1 : 0));
+  const uint32_t to1 = to + sw128(r0, 2 * (c & 3) + (upper ? 0 : 1));
+  // this lane's 16 bytes of a page on its way (it reads what it copied itself)
+  const uint32_t raw = smem_u32(smem) + kOffRaw + v * kRawHalf + cw * (8 * 512) + lane * 16;
+  const uint8_t *const rows = (v ? a.pool.v : a.pool.k) + row_at;
+  const uint8_t *const scale_bytes = (v ? a.pool.vs : a.pool.ks) + scale_at;
+  uint64_t *const empty = v ? bar.v_empty : bar.k_empty, *const full = v ? bar.v_full : bar.k_full;
+  // where page `lane & 7` of a key tile lies: its table entry is read two tiles before
+  // its rows are needed, and the scale bytes of the warp's four rows with the rows
+  int64_t at_rows = 0;
   int ahead_blk = 0, ahead_off = 0;
   auto look_up = [&](int j) {
     const int page = (j0 + j) * 8 + c;
@@ -97,67 +164,83 @@ VJ_DEV bool convert_tiles(const QPrefillArgs &a, const uint8_t *rows, const uint
       ahead_blk = bt[entry];
     }
   };
-  auto looked_up = [&]() {
+  auto looked_up = [&]() {                     // leaves at_rows; the scale bytes
     // (blocks that are none are read as block 0, as the other attention kernels do)
     const int blk = ahead_blk < 0 || ahead_blk >= a.pool.num_blocks ? 0 : ahead_blk;
     at_rows = blk * a.pool.sb + ahead_off * a.pool.st;
-    at_scales = blk * a.pool.ssb + ahead_off;
+    return *reinterpret_cast<const uint32_t *>(scale_bytes + blk * a.pool.ssb + ahead_off);
   };
-  auto load = [&](int j, int i) {              // page i of key tile j
-    const int64_t rp = __shfl_sync(0xffffffffu, at_rows, i);
-    const int64_t sp = __shfl_sync(0xffffffffu, at_scales, i);
-    x[i] = make_uint4(0, 0, 0, 0);
-    sc[i] = 127;
-    if ((j0 + j) * kKeys + i * 16 + r0 < limit) {
-      x[i] = *reinterpret_cast<const uint4 *>(rows + rp + r0 * a.pool.st + c * 16);
-      sc[i] = scales[sp + r0];
-    }
-  };
-  look_up(0);
-  looked_up();
-  look_up(1);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) load(0, i);
-  for (int j = 0; j < n; ++j) {
-    const int st = j % kRing;
-    bool ok = j < kRing || mbar_wait(&empty[st], (j / kRing - 1) & 1);
-    if (!__all_sync(0xffffffffu, ok)) return false;
-    looked_up();
-    look_up(j + 2);
-    uint8_t *tile = ring + st * kTileBytes + (upper ? kHalfTile : 0);
+  auto load = [&](int j) {                     // a key tile's pages
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      // (the next tile's page travels while the others are converted)
-      const uint4 y = x[i];
-      const uint32_t m = sc[i];
-      if (j + 1 < n) load(j + 1, i);
-      // 2^112 times the scale: the exponent of bf16 holds byte + 112 up to 254
-      const uint32_t first = m == 255u ? 0x7fffu : min(m + 112u, 254u) << 7;
-      const uint32_t f2 = first * 0x10001u;
-      // (the half of the lanes that has dims 64 and up starts with its second 16
-      // bytes, so that 8 lanes store to 8 different bank groups)
-      const uint32_t w[4] = {upper ? y.z : y.x, upper ? y.w : y.y,
-                             upper ? y.x : y.z, upper ? y.y : y.w};
-      uint32_t o[8];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        o[2 * k] = mul_bf16x2(f16_as_bf16(dequant_f16x2<kInt8, false>(w[k])), f2);
-        o[2 * k + 1] = mul_bf16x2(f16_as_bf16(dequant_f16x2<kInt8, true>(w[k])), f2);
-      }
-      if (m > 142u && m != 255u) {       // rows beyond 2^15: the rest of the scale
-        const uint32_t rest = (m - 142u + 127u) << 7, r2 = rest * 0x10001u;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) o[k] = mul_bf16x2(o[k], r2);
-      }
-      const int r = i * 16 + r0, chunk = 2 * (c & 3);
-      *reinterpret_cast<uint4 *>(tile + sw128(r, chunk + (upper ? 1 : 0))) =
-          make_uint4(o[0], o[1], o[2], o[3]);
-      *reinterpret_cast<uint4 *>(tile + sw128(r, chunk + (upper ? 0 : 1))) =
-          make_uint4(o[4], o[5], o[6], o[7]);
+      const int64_t rp = __shfl_sync(0xffffffffu, at_rows, i);
+      const bool there = j < n && (j0 + j) * kKeys + i * 16 + r0 < limit;
+      cp_async16(raw + (j & 1) * (2 * kRawHalf) + i * 512, rows + rp, there ? 16 : 0);
     }
+    cp_async_commit();
+  };
+  look_up(0);
+  uint32_t scales = looked_up();
+  look_up(1);
+  load(0);
+  uint32_t next_scales = looked_up();
+  look_up(2);
+  load(1);
+  for (int j = 0; j < n; ++j) {
+    const int st = j % kRing;
+    const uint32_t last_scales = looked_up();  // of tile j + 2
+    look_up(j + 3);
+    cp_async_wait<1>();                      // this tile's pages; the next one's travel
+    const bool ok = j < kRing || mbar_wait(&empty[st], (j / kRing - 1) & 1);
+    if (!__all_sync(0xffffffffu, ok)) {
+      cp_async_wait<0>();
+      return false;
+    }
+    const uint32_t tile = (v ? kOffV : kOffK) + st * kTileBytes;
+    const uint32_t from = raw + (j & 1) * (2 * kRawHalf);
+    // the scales first, then no branches: the pages' chains run into one another
+    uint32_t f2[8];
+    bool beyond = false;                     // e4m3: rows beyond 2^7
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      uint32_t m = __shfl_sync(0xffffffffu, scales, i) >> (lane & 24) & 0xffu;
+      if ((j0 + j) * kKeys + i * 16 + r0 >= limit) m = 127u;
+      f2[i] = scale_pair<kInt8>(m);
+      beyond |= !kInt8 && m > 254u - kScaleUp<kInt8> && m != 255u;
+    }
+    auto convert = [&](auto big) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint4 y = lds128(from + i * 512);
+        const uint32_t w[4] = {upper ? y.z : y.x, upper ? y.w : y.y,
+                               upper ? y.x : y.z, upper ? y.y : y.w};
+        uint32_t o[8];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          o[2 * k] = mul_bf16x2(to_bf16<kInt8, false>(w[k]), f2[i]);
+          o[2 * k + 1] = mul_bf16x2(to_bf16<kInt8, true>(w[k]), f2[i]);
+        }
+        if constexpr (big.value) {           // the rest of the scale
+          uint32_t m = __shfl_sync(0xffffffffu, scales, i) >> (lane & 24) & 0xffu;
+          if ((j0 + j) * kKeys + i * 16 + r0 >= limit) m = 127u;
+          const uint32_t rest = m == 255u ? 127u : max(m + kScaleUp<kInt8>, 254u) - 254u + 127u;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) o[k] = mul_bf16x2(o[k], (rest << 7) * 0x10001u);
+        }
+        const uint32_t at = tile + i * (16 * 128);
+        sts128(to0 + at, o[0], o[1], o[2], o[3]);
+        sts128(to1 + at, o[4], o[5], o[6], o[7]);
+      }
+    };
+    if (__any_sync(0xffffffffu, beyond)) convert(std::true_type{});
+    else convert(std::false_type{});
     fence_proxy_async_smem();
     mbar_arrive(&full[st]);
+    load(j + 2);                               // into the place that is read now
+    scales = next_scales;
+    next_scales = last_scales;
   }
+  cp_async_wait<0>();
   return true;
 }
 
@@ -182,7 +265,7 @@ quant_prefill_kernel(const __grid_constant__ CUtensorMap tmq, const QPrefillArgs
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bar.s_full[i], 1);
-      mbar_init(&bar.p_full[i], kRows);
+      mbar_init(&bar.p_full[i], 2 * kRows);
       mbar_init(&bar.pv_done[i], 1);
     }
     fence_mbar_init();
@@ -206,31 +289,27 @@ quant_prefill_kernel(const __grid_constant__ CUtensorMap tmq, const QPrefillArgs
   const int all = (p0 + min(n, tq0 + a.tt) + kKeys - 1) / kKeys;
   const int j0 = static_cast<int>(static_cast<int64_t>(all) * part / a.parts);
   const int nkv = static_cast<int>(static_cast<int64_t>(all) * (part + 1) / a.parts) - j0;
-  // this thread's row, in the softmax warps
-  const int r = threadIdx.x & (kRows - 1), tq = tq0 + r / a.g;
-  const bool valid = threadIdx.x < kRows && tq < n && q0 + tq < a.num_tokens;
+  // this thread's row and half of the keys, in the softmax warps
+  const int half = threadIdx.x / kRows, r = threadIdx.x % kRows, tq = tq0 + r / a.g;
+  const bool valid = half < 2 && tq < n && q0 + tq < a.num_tokens;
   const int64_t row = static_cast<int64_t>(q0 + tq) * a.Hq + h * a.g + r % a.g;
   const int64_t part_row = static_cast<int64_t>(part) * a.num_tokens * a.Hq + row;
   if (nkv == 0) {              // more parts than key tiles
-    if (valid) a.part_ml[part_row] = make_float2(kLowest, 0.f);
+    if (valid && half == 0) a.part_ml[part_row] = make_float2(kLowest, 0.f);
     return;
   }
-  if (warp == 12) tmem_alloc(&bar.tmem, 512);
+  if (warp == 16) tmem_alloc(&bar.tmem, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = bar.tmem;
   bool ok = true;
 
-  if (warp >= 4 && warp < 12) {
-    const bool is_v = warp >= 8;
-    const Pool &p = a.pool;
-    ok = convert_tiles<kInt8>(a, (is_v ? p.v : p.k) + h * p.sh, (is_v ? p.vs : p.ks) + h * p.ssh,
-                              smem + (is_v ? kOffV : kOffK), is_v ? bar.v_full : bar.k_full,
-                              is_v ? bar.v_empty : bar.k_empty, s, j0, nkv,
-                              min(ctx, a.max_pages * 16), warp & 3, lane);
-    if (a.parts == 1 && warp == 11) zero_tail_share(a, lane, 32);
-  } else if (warp == 12) {
+  if (warp >= 8 && warp < 16) {
+    ok = convert_tiles<kInt8>(a, smem, bar, warp >= 12, s, h, j0, nkv, min(ctx, a.max_pages * 16),
+                              warp & 3, lane);
+    if (a.parts == 1 && warp == 15) zero_tail_share(a, lane, 32);
+  } else if (warp == 16) {
     if (lane == 0) {
       mbar_arrive_expect_tx(&bar.q_full, kTileBytes);
       tma_load_3d(smem, &tmq, &bar.q_full, 0, h * a.g, q0 + tq0);
@@ -264,10 +343,11 @@ quant_prefill_kernel(const __grid_constant__ CUtensorMap tmq, const QPrefillArgs
         tc_fence_after();
         const uint32_t vb = sv + st * kTileBytes;
 #pragma unroll
-        for (int kk = 0; kk < kKeys / 16; ++kk) {              // O += P V
-          umma_ts(tmem + kColO, tmem + (j & 1) * kKeys + kk * 8,
+        for (int kk = 0; kk < kKeys / 16; ++kk) {              // O += P V, a half of the keys each
+          const int hf = kk >> 2, k4 = kk & 3;
+          umma_ts(tmem + kColO + hf * kD, tmem + (j & 1) * kKeys + hf * 64 + k4 * 8,
                   umma_desc_sw128(vb + kk * 2048, kHalfTile, 1024), idesc_pv,
-                  (j > 0 || kk > 0) ? 1u : 0u);
+                  (j > 0 || k4 > 0) ? 1u : 0u);
         }
         umma_commit(&bar.v_empty[st]);
         umma_commit(&bar.pv_done[j & 1]);
@@ -280,59 +360,50 @@ quant_prefill_kernel(const __grid_constant__ CUtensorMap tmq, const QPrefillArgs
       }
     }
   } else {
-    // ---- softmax: one row a thread
+    // ---- softmax: a row and half of the keys a thread
     const int qpos = p0 + tq, qpos_min = p0 + tq0;
-    const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t tO = tmem + lanes + kColO;
     float m_run = kLowest, l_run = 0.f;
     for (int j = 0; j < nkv; ++j) {
-      const uint32_t tS = tmem + lanes + (j & 1) * kKeys;
+      const uint32_t tS = tmem + lanes + (j & 1) * kKeys + half * 64;
       ok = mbar_wait(&bar.s_full[j & 1], (j >> 1) & 1);
       if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
       tc_fence_after();
-      const int kbase = (j0 + j) * kKeys;
-      // half of the keys at a time, twice: 128 registers a thread hold no more
-      auto scores = [&](float (&v)[64], int hf) {
-        tmem_ld64(tS + hf * 64, v);
-        if (kbase + kKeys - 1 > qpos_min) {
+      float v[64];
+      tmem_ld64(tS, v);
+      const int kbase = (j0 + j) * kKeys + half * 64;
+      if (kbase + 63 > qpos_min) {
 #pragma unroll
-          for (int i = 0; i < 64; ++i) {
-            if (kbase + hf * 64 + i > qpos) v[i] = -INFINITY;
-          }
+        for (int i = 0; i < 64; ++i) {
+          if (kbase + i > qpos) v[i] = -INFINITY;
         }
-      };
-      float top = -INFINITY;
-#pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        float v[64], mx[4];
-        scores(v, hf);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) mx[k] = v[k];
-#pragma unroll
-        for (int i = 4; i < 64; ++i) mx[i & 3] = fmaxf(mx[i & 3], v[i]);
-        top = fmaxf(top, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
       }
+      float mx[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) mx[k] = max3(v[k], v[k + 4], v[k + 8]);
+#pragma unroll
+      for (int i = 12; i < 60; i += 8) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) mx[k] = max3(mx[k], v[i + k], v[i + 4 + k]);
+      }
+      const float top = max3(max3(mx[0], mx[1], v[60]), max3(mx[2], mx[3], v[61]), fmaxf(v[62], v[63]));
       const float m_new = fmaxf(m_run, top * a.scale_log2);
       const bool grown = m_new - m_run > kGrow;
       const float m_use = j == 0 || grown ? m_new : m_run;
       const float corr = j == 0 ? 0.f : fast_exp2(m_run - m_use);
       uint64_t sum2[4] = {0ull, 0ull, 0ull, 0ull};
       const uint64_t sc2 = f32x2(a.scale_log2, a.scale_log2), nm2 = f32x2(-m_use, -m_use);
+      uint32_t pw[32];
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        float v[64];
-        scores(v, hf);
-        uint32_t pw[32];
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          float x0, x1;
-          f32x2_split(f32x2_fma(f32x2(v[2 * i], v[2 * i + 1]), sc2, nm2), x0, x1);
-          const float e0 = fast_exp2(x0), e1 = fast_exp2(x1);
-          sum2[i & 3] = f32x2_add(sum2[i & 3], f32x2(e0, e1));
-          pw[i] = pack_bf16(e0, e1);
-        }
-        tmem_st32u_nowait(tS + hf * 32, pw);
+      for (int i = 0; i < 32; ++i) {
+        float x0, x1;
+        f32x2_split(f32x2_fma(f32x2(v[2 * i], v[2 * i + 1]), sc2, nm2), x0, x1);
+        const float e0 = fast_exp2(x0), e1 = fast_exp2(x1);
+        sum2[i & 3] = f32x2_add(sum2[i & 3], f32x2(e0, e1));
+        pw[i] = pack_bf16(e0, e1);
       }
+      tmem_st32u_nowait(tS, pw);
       float u[8];
 #pragma unroll
       for (int k = 0; k < 4; ++k) f32x2_split(sum2[k], u[2 * k], u[2 * k + 1]);
@@ -343,12 +414,12 @@ quant_prefill_kernel(const __grid_constant__ CUtensorMap tmq, const QPrefillArgs
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
         tc_fence_after();
 #pragma unroll 1
-        for (int cidx = 0; cidx < kD / 32; ++cidx) {
+        for (int k = 0; k < kD / 32; ++k) {
           float o[32];
-          tmem_ld32(tO + cidx * 32, o);
+          tmem_ld32(tO + half * kD + k * 32, o);
 #pragma unroll
           for (int i = 0; i < 32; ++i) o[i] *= corr;
-          tmem_st32(tO + cidx * 32, o);
+          tmem_st32(tO + half * kD + k * 32, o);
         }
       }
       tmem_st_wait();
@@ -356,40 +427,51 @@ quant_prefill_kernel(const __grid_constant__ CUtensorMap tmq, const QPrefillArgs
       mbar_arrive(&bar.p_full[j & 1]);
     }
     if (ok) ok = mbar_wait(&bar.pv_done[(nkv - 1) & 1], ((nkv - 1) >> 1) & 1);
-    ok = __all_sync(0xffffffffu, ok);
-    if (ok) {
+    // ---- the halves of the keys together: half of the dims a thread
+    float2 *const ml = reinterpret_cast<float2 *>(smem);   // q's place, which no product reads now
+    ml[half * kRows + r] = make_float2(m_run, l_run);
+    named_bar_sync(1, 2 * kRows);
+    if (__all_sync(0xffffffffu, ok)) {
       tc_fence_after();
-      const float inv = 1.f / l_run;
-      if (a.parts > 1 && valid) a.part_ml[part_row] = make_float2(m_run, l_run);
+      const float2 ml0 = ml[r], ml1 = ml[kRows + r];
+      const float m = fmaxf(ml0.x, ml1.x), g0 = exp2f(ml0.x - m), g1 = exp2f(ml1.x - m);
+      const float l = ml0.y * g0 + ml1.y * g1, inv = a.parts > 1 ? 1.f : 1.f / l;
+      const float f0 = g0 * inv, f1 = g1 * inv;
+      if (a.parts > 1 && valid && half == 0) a.part_ml[part_row] = make_float2(m, l);
 #pragma unroll 1
-      for (int cidx = 0; cidx < kD / 32; ++cidx) {
-        float o[32];
-        tmem_ld32(tO + cidx * 32, o);
-        if (!valid) continue;
-        if (a.parts > 1) {
-          float4 *dst = reinterpret_cast<float4 *>(a.part_o + part_row * kD + cidx * 32);
+      for (int k = 2 * half; k < 2 * half + 2; ++k) {
+        float o[32], o1[32];
+        tmem_ld32(tO + k * 32, o);
+        tmem_ld32(tO + kD + k * 32, o1);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[i] = o[i] * f0 + o1[i] * f1;
+        if (valid && a.parts > 1) {
+          float4 *dst = reinterpret_cast<float4 *>(a.part_o + part_row * kD + k * 32);
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             dst[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
           }
-        } else {
-          uint4 *dst = reinterpret_cast<uint4 *>(a.out + row * kD + cidx * 32);
+        } else if (valid) {
+          uint4 *dst = reinterpret_cast<uint4 *>(a.out + row * kD + k * 32);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            dst[i] = make_uint4(pack_bf16(o[8 * i] * inv, o[8 * i + 1] * inv),
-                                pack_bf16(o[8 * i + 2] * inv, o[8 * i + 3] * inv),
-                                pack_bf16(o[8 * i + 4] * inv, o[8 * i + 5] * inv),
-                                pack_bf16(o[8 * i + 6] * inv, o[8 * i + 7] * inv));
+            dst[i] = make_uint4(pack_bf16(o[8 * i], o[8 * i + 1]),
+                                pack_bf16(o[8 * i + 2], o[8 * i + 3]),
+                                pack_bf16(o[8 * i + 4], o[8 * i + 5]),
+                                pack_bf16(o[8 * i + 6], o[8 * i + 7]));
           }
         }
+        __syncwarp();
       }
+    } else {
+      ok = false;
     }
   }
   if (!ok && a.err != nullptr) atomicExch(a.err, 1);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 12) tmem_dealloc(tmem, 512);
+  if (warp == 16) tmem_dealloc(tmem, 512);
 }
 
 // Parts of a row tile's key tiles: as many as fill the GPU, of two key tiles or more
