@@ -449,6 +449,7 @@ def test_decode_pool_beyond_32_bit_offsets():
     (8, 2, 32, [130, 5, 0, 1], [0, 200, 16, 300]),
     (4, 1, 16, [300], [129]),
     (16, 1, 64, [33, 40], [7, 600]),
+    (32, 8, 16, [100, 90, 1, 100, 77, 100, 99, 3], [0, 5, 0, 20, 16, 0, 17, 100]),   # read back first
 ])
 def test_prefill_matches_oracle(Hq, Hkv, bs, new, prefix, dtype, monkeypatch):
     from vllm_b200.kernels import quantized_cache as qc

@@ -424,17 +424,28 @@ PyObject *read_kv_cache(PyObject *const *args) {
   return given ? Py_NewRef(given.o) : THPVariable_Wrap(std::move(out));
 }
 
-// Whether to take the pages in directly instead of reading the contexts back first:
-// every row tile (128 rows) of a sequence and head converts its keys again, which pays
-// while there is one of them, or few in all, or one wave of them with short contexts.
-// Read back / direct, us, B200, 32 / 8 heads: 1 token after 4096 15.5 / 12.9; 32
-// sequences of 20 after up to 300 30.7 / 24.2; 2 x 256 after up to 1000 22.6 / 19.9; 256
-// after 4096 27.3 / 29.2; 2 x 600 after 4096 66 / 97.
-bool direct_prefill(int64_t S, int64_t T, int64_t hq, const Pool &p, int64_t longest, int64_t len) {
-  if (128 % (hq / p.hkv) != 0) return false;         // the other way refuses it
-  const int64_t tt = 128 / (hq / p.hkv), tiles = (longest + tt - 1) / tt;
-  const int64_t ctas = std::min(tiles * S, T / tt + S) * p.hkv;
-  return tiles == 1 || ctas <= 32 || (ctas <= num_sms() && len <= 768);
+// Whether to take the pages in directly instead of reading the contexts back first, by
+// what each way takes in us, fitted to 40 shapes of 1 to 2000 new tokens after 0 to 13854
+// (B200). A wave of CTAs costs its start and so much per key tile; direct, a CTA has one
+// row tile of 128 rows and converts its keys; read back, it has two and takes them
+// ready, after a launch that writes them. Both join what a split over keys leaves.
+// Measured read back / direct, 32 / 8 heads: 1 token after 1421 15.5 / 11.9; 32 after
+// 11129 35.6 / 22.3; 2 x 256 after 347 22 / 16.6; 300 after 2774 36 / 51; 2 x 600 after
+// 1420 66 / 82.
+bool direct_prefill(int64_t S, int64_t T, int64_t hq, const Pool &p, int64_t longest, int64_t len,
+                    size_t direct_bytes, size_t back_bytes) {
+  const int64_t g = hq / p.hkv;
+  if (S == 0 || T == 0 || 128 % g != 0) return S == 0 || T == 0;     // (the other way refuses it)
+  const int64_t part_bytes = T * hq * (p.D + 2) * 4, keys = (len + 127) / 128;
+  auto cost = [&](int64_t rows, size_t bytes, double start, double tile) {
+    const int64_t tt = rows / g, tiles = std::min((longest + tt - 1) / tt * S, T / tt + S);
+    const int64_t parts = std::max<int64_t>(1, bytes / part_bytes);
+    const int64_t waves = (tiles * p.hkv * parts + num_sms() - 1) / num_sms();
+    return waves * (start + tile * ((keys + parts - 1) / parts)) +
+           (parts > 1 ? 2.5 + 2.0 * bytes / 6e6 : 0.0);
+  };
+  const double read_back = S * len * p.hkv * 770.0 / 6e6;            // both ways through HBM
+  return 2.0 + cost(128, direct_bytes, 5.5, 1.8) <= 5.0 + cost(256, back_bytes, 5.0, 1.45) + read_back;
 }
 
 // (q, cache, block_tables, cu_seqlens_q, context_lens, max_seqlen_q, scale, out,
@@ -477,8 +488,9 @@ PyObject *paged_prefill(PyObject *const *args) {
   const int32_t *const cu_ptr = static_cast<const int32_t *>(cu.ptr());
   int32_t *const err = error_flag(dev);
   const cudaStream_t stream = stream_of(dev);
-  if (direct_prefill(S, T, hq, p, max_new > 0 ? max_new : T, len)) {
-    const size_t need = direct_workspace_entry(T, S, hq, p.hkv, p.D, max_new, len);
+  const size_t need = direct_workspace_entry(T, S, hq, p.hkv, p.D, max_new, len);
+  if (direct_prefill(S, T, hq, p, max_new > 0 ? max_new : T, len, need,
+                     prefill_workspace_entry(T, S, hq, p.hkv, p.D, max_new, len))) {
     at::Tensor ws;
     if (need) ws = at::empty({static_cast<int64_t>(need)}, q->options().dtype(at::kByte));
     void *const ws_ptr = need ? ws.data_ptr() : nullptr;
@@ -506,15 +518,16 @@ PyObject *paged_prefill(PyObject *const *args) {
     const Tables part = {t.ptr + s * t.stride, t.lens + s, t.width, t.stride};
     read_back(p, part, k_ptr, n, len, kKeyTile, stream);
     // (the last group may be smaller and split further than the others)
-    const size_t need = prefill_workspace_entry(T, n, hq, p.hkv, p.D, max_new, len);
+    const size_t part_need = prefill_workspace_entry(T, n, hq, p.hkv, p.D, max_new, len);
     at::Tensor more;
-    if (need > split_bytes) more = at::empty({static_cast<int64_t>(need)}, q->options().dtype(at::kByte));
+    if (part_need > split_bytes) more = at::empty({static_cast<int64_t>(part_need)}, q->options().dtype(at::kByte));
     void *const part_ws = more.defined() ? more.data_ptr() : ws;
-    enter(need > 0 ? 2 : 1, [&] {
+    enter(part_need > 0 ? 2 : 1, [&] {
       return prefill_entry(q_ptr, k_ptr, static_cast<uint8_t *>(k_ptr) + n * len * row * 2, nullptr,
                            cu_ptr + s, part.lens, out_ptr, T, n, hq, p.hkv, p.D,
                            static_cast<int64_t>(std::max(n, 1)) * per_seq, kPage, per_seq, per_seq,
-                           kPage * row, row, p.D, max_new, len, scale, part_ws, need, err, stream);
+                           kPage * row, row, p.D, max_new, len, scale, part_ws, part_need,
+                           err, stream);
     });
   }
   return given ? Py_NewRef(given.o) : THPVariable_Wrap(std::move(out));

@@ -139,12 +139,13 @@ def paged_prefill_quantized(q: torch.Tensor, cache: QuantizedKVCache, block_tabl
                             max_context_len: int = 0) -> torch.Tensor:
     """paged_prefill over a quantised cache: causal attention of the new tokens
     (rows [cu_seqlens_q[s], cu_seqlens_q[s+1]) of q) of each sequence over its
-    cached context, theirs included. The contexts are read back to bf16, which
-    is exact, and attended to from there: a prompt's attention does far more
-    work per key than reading it back, and the conversion is done once instead
-    of once per query tile. max_context_len: a bound on context_lens (default:
-    what a block table row holds); it sizes the scratch, as max_seqlen_q sizes
-    the grid."""
+    cached context, theirs included (context_lens is no less than the new tokens).
+    Few new tokens take the quantised pages in directly; for many, whose attention
+    does far more work per key, the contexts are read back to bf16 first, which is
+    exact, once instead of once per query tile. max_seqlen_q and max_context_len:
+    bounds on the new tokens and on context_lens (default: all tokens, and what a
+    block table row holds); they size the grid and the scratch, and decide how the
+    keys are split. scale: positive. Rows behind cu_seqlens_q[-1] come out 0."""
     return (_calls or _bound()).paged_prefill(q, cache, block_tables, cu_seqlens_q, context_lens,
                                               int(max_seqlen_q), scale, out, int(max_context_len),
                                               PREFILL_SCRATCH_ROWS)
