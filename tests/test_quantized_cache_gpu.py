@@ -638,6 +638,56 @@ def test_decode_is_deterministic_on_two_streams_at_once_and_in_graphs():
         assert torch.equal(o, r)
 
 
+@pytest.mark.parametrize("new,prefix,Hq,Hkv", [
+    ((1, 3), (1500, 40), 8, 2),                # direct, split
+    ((20, 60, 0), (0, 30, 50), 8, 2),          # direct, one launch
+    ((260, 30), (2400, 1000), 32, 8),          # read back, split
+    ((900, 1000), (0, 100), 32, 8),            # read back, one launch
+])
+def test_prefill_in_graphs_and_on_two_streams_at_once(new, prefix, Hq, Hkv):
+    """Captured, replayed with other inputs in the same places, and next to itself on
+    another stream: the eager call's bits."""
+    from vllm_b200.kernels.quantized_cache import QuantizedKVCache, paged_prefill_quantized
+    rng = np.random.default_rng(25)
+    ctx = [a + b for a, b in zip(new, prefix)]
+    need = sum(-(-n // 16) for n in ctx)
+    width = -(-max(ctx) // 16)
+    T, cu = sum(new), np.concatenate([[0], np.cumsum(new)])
+
+    def inputs(lens):
+        codes, scales = _random_pool(rng, need, 16, Hkv, "e4m3")
+        return (_t(bf16(rng.standard_normal((T, Hq, D)))), *_cache(codes, scales, "e4m3"),
+                _i(_tables(rng, lens, need, 16, width)), _i(lens))
+
+    def call(x, out=None):
+        return paged_prefill_quantized(x[0], QuantizedKVCache(x[1], x[2]), x[3], _i(cu) if out is None
+                                       else d_cu, x[4], max(new), max_context_len=max(ctx), out=out)
+
+    d_cu = _i(cu)
+    sets = [inputs(ctx), inputs([max(n - 7 * i, new[i]) for i, n in enumerate(ctx)])]
+    ref = [call(x) for x in sets]
+    live = [t.clone() for t in sets[0]]
+    out = torch.empty_like(ref[0])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(live, out)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for i in (1, 0, 1):
+        for a, b in zip(live, sets[i]):
+            a.copy_(b)
+        torch.cuda.synchronize()
+        beside = []
+        for _ in range(4):
+            for k, s in enumerate(streams):
+                with torch.cuda.stream(s):
+                    beside.append((k, torch.empty_like(out)))
+                    call(sets[k], beside[-1][1])
+            graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, ref[i])
+        assert all(torch.equal(o, ref[k]) for k, o in beside)
+
+
 def test_a_step_as_it_is_used():
     """Prompts stored, attended to, extended token by token and read back: every step
     against the oracle on the cache's own values, replayed from one captured graph."""
