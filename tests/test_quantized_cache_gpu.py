@@ -819,6 +819,11 @@ def test_wrapper_refusals():
         (lambda: qc.kv_store_quantized(q, kv, kv, c, ln, ln, w.float(), w), "q_norm_weight"),
         (lambda: qc.kv_store_quantized(q, kv[:, :1], kv[:, :1], c, ln, ln, w, w), "do not match"),
         (lambda: qc.kv_store_quantized(q, kv, kv, c, ln, ln, w, w, q_out=q[:, :2]), "q_out"),
+        (lambda: qc.kv_store_quantized(q, kv[:1].expand(3, 2, D), kv, c, ln, ln, w, w), "overlap"),
+        (lambda: qc.kv_store_quantized(q, kv, kv[:1].expand(3, 2, D), c, ln, ln, w, w), "overlap"),
+        (lambda: qc.kv_store_quantized(q[:1].expand(3, 4, D), kv, kv, c, ln, ln, w, w), "overlap"),
+        (lambda: qc.paged_decode_quantized(q[:, :0].contiguous(), c, bt, ln), "size"),
+        (lambda: qc.paged_prefill_quantized(q[:, :0].contiguous(), c, bt, _i([0, 1, 2, 3]), ln), "size"),
         (lambda: qc.paged_prefill_quantized(q, c, bt, ln, ln), "one row per sequence"),
         (lambda: qc.paged_prefill_quantized(q, c, bt[:2], ln, ln[:2], scale=0.0), "positive"),
         (lambda: qc.paged_prefill_quantized(q, c, bt[:2], ln, ln[:2], max_context_len=-4),

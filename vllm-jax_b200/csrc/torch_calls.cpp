@@ -210,7 +210,9 @@ Rows rows(const Arg &a, const char *name, int64_t T, int64_t D) {
   if (s.size() != 3 || s[0] != T || s[2] != D || st[2] != 1 || (st[1] != D && s[1] != 1)) {
     fail("`%s` must be a [num_tokens, H, head_dim] tensor with packed heads", name);
   }
-  return {s[1], st[0], a.ptr()};
+  // (a stride of 0 would mean packed rows to the C entries)
+  if (T > 1 && st[0] < s[1] * D) fail("rows of `%s` must not overlap", name);
+  return {s[1], T > 1 ? st[0] : s[1] * D, a.ptr()};
 }
 const int32_t *indices(const Arg &a, const char *name, int64_t T) {
   require_dtype(a, at::kInt, name, "torch.int32");
@@ -435,7 +437,8 @@ PyObject *read_kv_cache(PyObject *const *args) {
 bool direct_prefill(int64_t S, int64_t T, int64_t hq, const Pool &p, int64_t longest, int64_t len,
                     size_t direct_bytes, size_t back_bytes) {
   const int64_t g = hq / p.hkv;
-  if (S == 0 || T == 0 || 128 % g != 0) return S == 0 || T == 0;     // (the other way refuses it)
+  if (S == 0 || T == 0) return true;
+  if (g == 0 || 128 % g != 0) return false;            // the other way refuses it
   const int64_t part_bytes = T * hq * (p.D + 2) * 4, keys = (len + 127) / 128;
   auto cost = [&](int64_t rows, size_t bytes, double start, double tile) {
     const int64_t tt = rows / g, tiles = std::min((longest + tt - 1) / tt * S, T / tt + S);
