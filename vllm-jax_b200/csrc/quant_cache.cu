@@ -212,55 +212,57 @@ __device__ __noinline__ Scaled k_row_64(const uint8_t *row, const __nv_bfloat16 
 }
 
 
-// One row of k: 32 bits where they decide the rounding, else 64.
+// Sixteen elements as four words of the cache.
 template <bool kInt8>
-VJ_DEV void k_row(float (&v)[16], int &e, bool &bad, const uint8_t *row, const RowSlice &cs,
+VJ_DEV void quantise16(uint32_t (&o)[4], const float (&v)[16]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    o[j] = quantise2<kInt8>(v[4 * j], v[4 * j + 1]) |
+           quantise2<kInt8>(v[4 * j + 2], v[4 * j + 3]) << 16;
+  }
+}
+
+// One row of k, quantised: 32 bits where they decide the rounding, else 64. What 32
+// bits give is off by less than 2^-20 of itself, so they decide where an element made
+// larger and smaller by that rounds to the same.
+template <bool kInt8>
+VJ_DEV void k_row(uint32_t (&o)[4], int &e, bool &bad, const uint8_t *row, const RowSlice &cs,
                   const Turn &t, unsigned mask, const StoreArgs &a) {
   uint64_t u[4], z[4];
   turn_row(u, z, load_slice(row, threadIdx.x & 7), t, mask, a);
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    f32x2_split(u[j], v[4 * j], v[4 * j + 2]);
-    f32x2_split(z[j], v[4 * j + 1], v[4 * j + 3]);
-  }
   uint32_t amax = 0;
 #pragma unroll
-  for (int j = 0; j < 16; ++j) amax = max(amax, __float_as_uint(v[j]) & 0x7fffffffu);
+  for (int j = 0; j < 4; ++j) {
+    float x0, x1, y0, y1;
+    f32x2_split(u[j], x0, x1);
+    f32x2_split(z[j], y0, y1);
+    amax = max(max(amax, max(__float_as_uint(x0) & 0x7fffffffu, __float_as_uint(x1) & 0x7fffffffu)),
+               max(__float_as_uint(y0) & 0x7fffffffu, __float_as_uint(y1) & 0x7fffffffu));
+  }
   amax = group_max(mask, amax);
   bad = false;
   e = scale_exponent<kInt8>(amax);
   const float f = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);   // 2^-e
-  // undecided: outside of 2^-100 .. 2^120 (sums and products of 32 bits may have
-  // left their range), the largest element next to where the exponent moves, or
-  // an element within 16 units of its last place of a midpoint
-  uint32_t near = __usad(amax & 0x7fffffu, kInt8 ? 0x7e0000u : 0x600000u, 0u);
-  bool open = amax < (27u << 23) || amax >= (247u << 23);
-  float least = INFINITY;          // e4m3: smallest element that is not 0
+  // undecided too: outside of 2^-100 .. 2^120 (sums and products of 32 bits may have
+  // left their range), and the largest element next to where the exponent moves
+  bool open = amax < (27u << 23) || amax >= (247u << 23) ||
+              __usad(amax & 0x7fffffu, kInt8 ? 0x7e0000u : 0x600000u, 0u) <= 16u;
+  const uint64_t up = f32x2(f * (1.f + 0x1p-20f), f * (1.f + 0x1p-20f));
+  const uint64_t down = f32x2(f * (1.f - 0x1p-20f), f * (1.f - 0x1p-20f));
+  uint32_t apart = 0;
 #pragma unroll
-  for (int j = 0; j < 16; ++j) {
-    v[j] *= f;
-    if constexpr (kInt8) {
-      const float d = v[j] - ((v[j] + 12582912.0f) - 12582912.0f);
-      open |= fabsf(fabsf(d) - 0.5f) <= fabsf(v[j]) * 0x1p-20f;
-    } else {
-      near = min(near, __usad(__float_as_uint(v[j]) & 0xfffffu, 0x80000u, 0u));
-      least = fminf(least, fabsf(v[j]));
-    }
+  for (int j = 0; j < 4; ++j) {
+    float a0, a1, b0, b1, c0, c1, d0, d1;
+    f32x2_split(f32x2_mul(u[j], up), a0, a1);
+    f32x2_split(f32x2_mul(z[j], up), b0, b1);
+    f32x2_split(f32x2_mul(u[j], down), c0, c1);
+    f32x2_split(f32x2_mul(z[j], down), d0, d1);
+    o[j] = quantise2<kInt8>(a0, b0) | quantise2<kInt8>(a1, b1) << 16;
+    apart |= o[j] ^ (quantise2<kInt8>(c0, d0) | quantise2<kInt8>(c1, d1) << 16);
   }
-  open |= near <= 16u;
-  if constexpr (!kInt8) {
-    if (least < 0x1p-6f) {         // below the normal numbers the step is 2^-9
-#pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const float d = v[j] - ((v[j] + 24576.0f) - 24576.0f);
-        open |= fabsf(v[j]) < 0x1p-6f && fabsf(fabsf(d) - 0x1p-10f) <= fabsf(v[j]) * 0x1p-20f;
-      }
-    }
-  }
-  if (__any_sync(mask, open)) {
+  if (__any_sync(mask, open || apart != 0u)) {
     const Scaled r = k_row_64<kInt8>(row, a.kw, cs, mask, a.eps, a.norm, a.rope);
-#pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = r.v[j];
+    quantise16<kInt8>(o, r.v);
     e = r.e;
     bad = r.bad;
   }
@@ -409,7 +411,7 @@ kv_store_quantized_kernel(const StoreArgs a) {
     for (; stored && h < r1; h += 4) {
       const bool is_v = h >= a.Hq + a.Hkv;
       const int hk = is_v ? h - a.Hq - a.Hkv : h - a.Hq;
-      float y[16];
+      uint32_t o[4];
       int e;
       bool bad;                            // an infinity or NaN in the row
       if (is_v) {
@@ -423,21 +425,17 @@ kv_store_quantized_kernel(const StoreArgs a) {
         bad = amax >= 0x7f800000u;
         e = bad ? 0 : scale_exponent<kInt8>(amax);
         const float f = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);   // 2^-e
+        float y[16];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           y[2 * j] = bf16_lo(x.w[j]) * f;
           y[2 * j + 1] = bf16_hi(x.w[j]) * f;
         }
+        quantise16<kInt8>(o, y);
       } else {
-        k_row<kInt8>(y, e, bad, unit + (h - r0) * 256, cs, turn, mask, a);
+        k_row<kInt8>(o, e, bad, unit + (h - r0) * 256, cs, turn, mask, a);
       }
-      uint32_t o[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t lo = quantise2<kInt8>(y[4 * j], y[4 * j + 1]);
-        const uint32_t hi = quantise2<kInt8>(y[4 * j + 2], y[4 * j + 3]);
-        o[j] = bad ? 0u : lo | (hi << 16);
-      }
+      if (bad) o[0] = o[1] = o[2] = o[3] = 0u;
       uint8_t *row = (is_v ? a.pool.v : a.pool.k) + blk * a.pool.sb + off * a.pool.st +
                      hk * a.pool.sh + l8 * 8;
       *reinterpret_cast<uint2 *>(row) = make_uint2(o[0], o[1]);
