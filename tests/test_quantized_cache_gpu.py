@@ -281,7 +281,8 @@ def test_decode_batch_larger_than_a_block_of_threads():
 
 
 @pytest.mark.parametrize("Hq,Hkv,dtype", [(74, 37, "e4m3"), (8 * 37, 37, "int8"),
-                                          (370, 37, "e4m3"), (64, 64, "int8")])
+                                          (370, 37, "e4m3"), (64, 64, "int8"),
+                                          (128, 64, "e4m3"), (74, 37, "int8")])
 def test_decode_of_so_many_pages_that_a_part_is_dealt(Hq, Hkv, dtype):
     """Enough work (32 pages a warp and KV head) that a fifth of it is dealt in pieces:
     against 64 bits, the same bits every time, and on two streams at once."""
@@ -331,7 +332,8 @@ def test_decode_of_so_many_pages_that_a_part_is_dealt(Hq, Hkv, dtype):
     # whatever the scratch holds before the call (counts of pieces among it)
     ws = torch.empty(decode_quantized_workspace_bytes(B, Hq, Hkv, width, bs) // 4,
                      dtype=torch.int32, device="cuda")
-    for word in (0, 1, 2, 3, -1, 0x7fc00000):
+    # (and often: a stage refilled before its page is read shows in one call of ten)
+    for word in (0, 1, 2, 3, -1, 0x7fc00000) * 10:
         ws.fill_(word)
         assert torch.equal(paged_decode_quantized(q, cache, bt, ln, workspace=ws.view(torch.uint8)),
                            out)

@@ -445,7 +445,10 @@ kv_store_quantized_kernel(const StoreArgs a) {
         *sc = bad ? 255 : static_cast<uint8_t>(e + 127);
       }
     }
-    __syncwarp();            // every lane has read the unit: refill its stage
+    // every lane has read the unit: refill its stage (the copy is the async proxy's, and
+    // the fence orders the reads before it)
+    fence_proxy_async_smem();
+    __syncwarp();
     issue(s);
     if (++s == kUnitStages) { s = 0; parity ^= 1; }
     advance(t, part);

@@ -237,12 +237,13 @@ VJ_DEV uint4 lds128(uint32_t addr) {
   uint4 v;
   asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
                : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "r"(addr));
+               : "r"(addr)
+               : "memory");
   return v;
 }
 VJ_DEV uint32_t lds8(uint32_t addr) {
   uint32_t v;
-  asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(addr));
+  asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
   return v;
 }
 VJ_DEV float max_over_rows(float v) {        // over the lanes that share lane & 3
@@ -530,7 +531,8 @@ quant_decode_kernel(const __grid_constant__ CUtensorMap tm_rows,
   int stage = 0;
   uint32_t parity = 0;
   for (int it = 0; it < issued; ++it) {
-    if (!mbar_wait(&my_full[stage], parity)) {
+    // (all lanes together: what follows are warp-wide products)
+    if (!__all_sync(0xffffffffu, mbar_wait(&my_full[stage], parity))) {
       // bounded: the copies still in flight must land before the CTA ends
       for (int k = it + 1; k < issued; ++k) {
         mbar_wait(&my_full[k % kStages], (k / kStages) & 1);
@@ -656,7 +658,12 @@ quant_decode_kernel(const __grid_constant__ CUtensorMap tm_rows,
           if (2 * qd + (j & 1) + (j >> 1) * 8 >= valid) v[j] = make_uint4(0, 0, 0, 0);
         }
       }
-      __syncwarp();            // every lane has read the stage: refill it
+      // every lane has read the stage: refill it. V is still on its way to the registers
+      // here, and the copy is the async proxy's, which a barrier of the warp alone does
+      // not order behind the reads: in some builds of this kernel one page in two million
+      // was read while it was refilled. With the fence: none, and the same time.
+      fence_proxy_async_smem();
+      __syncwarp();
       issue(stage);
       const uint32_t *w0 = reinterpret_cast<const uint32_t *>(&v[0]);
       const uint32_t *w1 = reinterpret_cast<const uint32_t *>(&v[1]);
