@@ -690,6 +690,44 @@ def test_prefill_in_graphs_and_on_two_streams_at_once(new, prefix, Hq, Hkv):
         assert all(torch.equal(o, ref[k]) for k, o in beside)
 
 
+@pytest.mark.parametrize("op", ["decode", "prefill"])
+@pytest.mark.parametrize("lens,Hq,Hkv", [((2900, 17, 600, 0, 1500, 44), 8, 2), ((5000,), 16, 4)])
+def test_calls_back_to_back_on_other_inputs(op, lens, Hq, Hkv):
+    """Three inputs in turn, eager and from one graph: each call launches before the last
+    one is done, and its scratch often is the last one's memory."""
+    from vllm_b200.kernels.quantized_cache import (QuantizedKVCache, paged_decode_quantized,
+                                                   paged_prefill_quantized)
+    rng = np.random.default_rng(26)
+    B, need = len(lens), sum(-(-n // 16) for n in lens)
+    cu = _i(np.arange(B + 1))
+    sets = []
+    for _ in range(3):
+        codes, scales = _random_pool(rng, need, 16, Hkv, "int8")
+        sets.append((_t(bf16(rng.standard_normal((B, Hq, D)))), _cache(codes, scales, "int8"),
+                     _i(_tables(rng, lens, need, 16, -(-max(lens) // 16))),
+                     _i([max(n, op == "prefill") for n in lens])))
+
+    def call(k):
+        q, cache, bt, ln = sets[k]
+        if op == "decode":
+            return paged_decode_quantized(q, cache, bt, ln)
+        return paged_prefill_quantized(q, cache, bt, cu, ln, 1, max_context_len=max(lens))
+
+    ref = []
+    for k in range(3):
+        ref.append(call(k))
+        torch.cuda.synchronize()
+    got = [(i % 3, call(i % 3)) for i in range(60)]
+    graph, held = torch.cuda.CUDAGraph(), []
+    with torch.cuda.graph(graph):
+        for i in range(9):
+            held.append((i % 3, call(i % 3)))
+    for _ in range(5):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, ref[k]) for k, o in got + held)
+
+
 def test_a_step_as_it_is_used():
     """Prompts stored, attended to, extended token by token and read back: every step
     against the oracle on the cache's own values, replayed from one captured graph."""
