@@ -473,12 +473,25 @@ VJ_API vj_status vj_allreduce_add_rmsnorm(
  *   workspace: vj_paged_prefill_split_workspace_size(...) bytes on the current
  *   device (0 without a split: may be NULL), 16-byte aligned, need not be
  *   initialised; calls whose kernels may overlap need one each
- *   scale: positive and finite */
+ *   scale: positive and finite
+ * out may be q. */
 VJ_API size_t vj_paged_prefill_split_workspace_size(int64_t num_tokens, int32_t num_seqs,
                                                     int32_t num_q_heads, int32_t num_kv_heads,
                                                     int32_t head_dim, int32_t max_seqlen_q,
                                                     int32_t max_context_len);
 VJ_API vj_status vj_paged_prefill_split(
+    const void *q, const void *k_cache, const void *v_cache, const int32_t *block_tables,
+    const int32_t *cu_seqlens_q, const int32_t *context_lens, void *out, int64_t num_tokens,
+    int32_t num_seqs, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+    int64_t num_blocks, int32_t block_size, int32_t bt_width, int32_t bt_stride,
+    int64_t stride_block, int64_t stride_token, int64_t stride_head, int32_t max_seqlen_q,
+    int32_t max_context_len, float scale, void *workspace, size_t workspace_bytes,
+    int32_t *error_flag, cudaStream_t stream);
+/* The same for some neighbouring sequences of a batch (cu_seqlens_q and
+ * context_lens from the first of them on; q, out and num_tokens the whole batch's):
+ * rows of out behind the last of them are left as they are, so that where out is q
+ * the sequences behind still find their queries. */
+VJ_API vj_status vj_paged_prefill_split_part(
     const void *q, const void *k_cache, const void *v_cache, const int32_t *block_tables,
     const int32_t *cu_seqlens_q, const int32_t *context_lens, void *out, int64_t num_tokens,
     int32_t num_seqs, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
@@ -570,7 +583,7 @@ VJ_API vj_status vj_paged_decode_quantized(
 /* Causal attention of few new tokens over the quantised cache, straight from its
  * pages: q, out, cu_seqlens_q, context_lens (new tokens included; not NULL),
  * max_seqlen_q as in vj_paged_prefill, the cache as above. Rows of out behind
- * cu_seqlens_q[num_seqs] are zeroed. The keys of a row tile (128 rows of tokens x
+ * cu_seqlens_q[num_seqs] are zeroed; out may be q. The keys of a row tile (128 rows of tokens x
  * query heads of one KV head) are split over CTAs that would be idle. Where there
  * are many row tiles, vj_kv_read_quantized (zero_to = 128, max_len a multiple of
  * 128) and vj_paged_prefill_split on what it leaves are faster.

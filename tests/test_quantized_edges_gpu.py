@@ -1,0 +1,102 @@
+"""Calls of the quantised KV cache at the edges of what they accept, on the GPU
+against 64-bit NumPy (oracle/quantized.py). Tolerances as derived in
+test_quantized_cache_gpu.py: a bf16 result is off by half a step, 2^-8 |r|, the
+weights of decode by 2^-11 + 2^-12 and of prefill by 2^-8 + 2^-11 of each."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import quantized as oq
+from oracle.bf16 import bf16
+
+pytestmark = pytest.mark.gpu
+
+D = 128
+TORCH = {"e4m3": torch.float8_e4m3fn, "int8": torch.int8}
+DECODE = 2.0 ** -11 + 2.0 ** -12
+PREFILL = 2.0 ** -8 + 2.0 ** -11
+
+
+def _t(x, dtype=torch.bfloat16):
+    return torch.from_numpy(np.ascontiguousarray(x)).to(dtype).cuda()
+
+
+def _i(x):
+    return torch.tensor(np.asarray(x, np.int32), device="cuda")
+
+
+def _check(got, ref, mag, weight):
+    got = got.double().cpu().numpy()
+    err = np.abs(got - ref)
+    tol = 2.0 ** -8 * np.abs(ref) + weight * mag + 1e-30
+    assert np.isfinite(got).all() and (err <= tol).all(), \
+        f"worst {np.max(err / tol):.3f} of the tolerance"
+
+
+class _Prompts:
+    """A batch of new tokens after cached prefixes, with five padding rows of q."""
+
+    def __init__(self, Hq, Hkv, new, prefix, dtype="e4m3", bs=16, seed=0):
+        from vllm_b200.kernels.quantized_cache import QuantizedKVCache
+        rng = np.random.default_rng(seed)
+        self.new, self.prefix = new, prefix
+        self.ctx = [a + b for a, b in zip(new, prefix)]
+        need = [-(-n // bs) for n in self.ctx]
+        nb = sum(need) + 2
+        self.codes, _ = oq.quantise_rows(rng.standard_normal((2, nb, bs, Hkv, D)), dtype)
+        self.scales = rng.integers(118, 123, (2, nb, Hkv, bs)).astype(np.uint8)
+        perm, at = rng.permutation(nb), 0
+        self.bt = np.full((len(new), max(need) + 1), -1, np.int32)
+        for s, n in enumerate(need):
+            self.bt[s, :n] = perm[at:at + n]
+            at += n
+        self.cu = np.concatenate([[0], np.cumsum(new)])
+        self.q_np = bf16(rng.standard_normal((int(self.cu[-1]) + 5, Hq, D)))
+        self.dtype = dtype
+        self.q = _t(self.q_np)
+        self.args = (QuantizedKVCache(_t(self.codes, torch.uint8).view(TORCH[dtype]),
+                                      _t(self.scales, torch.uint8)),
+                     _i(self.bt), _i(self.cu), _i(self.ctx), max(new))
+
+    def call(self, q=None, out=None, **kw):
+        from vllm_b200.kernels.quantized_cache import paged_prefill_quantized
+        kw.setdefault("max_context_len", max(self.ctx))
+        return paged_prefill_quantized(self.q if q is None else q, *self.args, out=out, **kw)
+
+    def reference(self):
+        vals = [oq.dequantise(self.codes[i], self.scales[i], self.dtype) for i in range(2)]
+        ref, mag = np.zeros(self.q_np.shape), np.zeros(self.q_np.shape)
+        for s, (n, p) in enumerate(zip(self.new, self.prefix)):
+            if n:
+                k, v = (oq.gather(vals[i], self.bt[s], n + p) for i in range(2))
+                rows = slice(self.cu[s], self.cu[s + 1])
+                ref[rows], mag[rows] = oq.attend(self.q_np[rows].astype(np.float64), k, v, p,
+                                                 1 / math.sqrt(D))
+        return ref, mag
+
+
+@pytest.mark.parametrize("Hq,Hkv,new,prefix,groups,launches", [
+    (8, 2, (20, 60, 0), (0, 30, 50), 1, 1),              # from the pages
+    (8, 2, (1, 3), (1500, 40), 1, 2),                    # and their keys split
+    (32, 8, (900, 1000), (0, 100), 1, 2),                # read back first
+    (32, 8, (256,), (2500,), 1, 3),                      # and their keys split
+    (32, 8, (900, 1000, 700), (0, 100, 5), 3, 6),        # read back in groups
+    (32, 8, (300, 0, 280), (1400, 30, 1100), 3, 9),      # and their keys split
+])
+def test_prefill_in_the_queries_place(Hq, Hkv, new, prefix, groups, launches, monkeypatch):
+    """out may be q itself, however the call is carried out."""
+    from vllm_b200 import _native
+    from vllm_b200.kernels import quantized_cache as qc
+    if groups > 1:
+        monkeypatch.setattr(qc, "PREFILL_SCRATCH_ROWS", 1)
+    case = _Prompts(Hq, Hkv, new, prefix)
+    before = _native.launch_count
+    ref = case.call()
+    assert _native.launch_count - before == launches
+    q = case.q.clone()
+    assert case.call(q, out=q) is q
+    assert torch.equal(q, ref)
+    _check(q, *case.reference(), PREFILL)
+

@@ -131,6 +131,7 @@ struct PrefillArgs {
   int *err;
   // key split: parts of a tile pair's key tiles, and what they leave per (part, token, head)
   int parts, num_seqs, longest_first;
+  int keep_tail;            // whether rows past the last sequence are left as they are
   float *part_o;            // [parts][tokens][Hq][128]
   float2 *part_ml;          // [parts][tokens][Hq] maximum (log2), sum
 };
@@ -229,7 +230,7 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap *tmq_p, const CUt
   const int tq0 = m2 * 2 * a.tt;               // first token of tile A
   if (tq0 >= n) {        // whole CTA, before any barrier (kSplit: wait) or TMEM use
     if constexpr (kSplit) {
-      if (a.parts == 1) zero_tail_share(a, threadIdx.x, kThreads);
+      if (a.parts == 1 && !a.keep_tail) zero_tail_share(a, threadIdx.x, kThreads);
       __syncwarp();
       if (warp == kWarpMma) tmem_dealloc(tmem, 512);
     }
@@ -274,7 +275,7 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap *tmq_p, const CUt
   } else if (warp == kWarpV) {
     // ------------------------------------------------------------ V producer
     ok = produce_kv<kSplit, kVStages>(tmv_p, smem + OFF_V, bar.v_full, bar.v_empty, a, s, h, j0, nkv, lane);
-    if (kSplit && a.parts == 1) zero_tail_share(a, lane, 32);
+    if (kSplit && a.parts == 1 && !a.keep_tail) zero_tail_share(a, lane, 32);
   } else if (warp == kWarpMma) {
     // ------------------------------------------------------------ MMA issuer
     if (lane == 0) {
@@ -552,7 +553,7 @@ prefill_split_kernel(const __grid_constant__ CUtensorMap tmq,
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (a.parts > 1) asm volatile("griddepcontrol.launch_dependents;");
   if (a.num_seqs == 0) {
-    zero_tail_share(a, threadIdx.x, kThreads);
+    if (!a.keep_tail) zero_tail_share(a, threadIdx.x, kThreads);
     return;
   }
   int x = blockIdx.x, h = blockIdx.y, z = blockIdx.z;
@@ -643,6 +644,7 @@ int prefill_setup(const std::string &what, const void *q, const void *k_cache, c
   a.parts = 1;
   a.num_seqs = num_seqs;
   a.longest_first = 0;
+  a.keep_tail = 0;
   a.part_o = nullptr;
   a.part_ml = nullptr;
   const int64_t maxq = max_seqlen_q > 0 ? max_seqlen_q : num_tokens;
@@ -735,16 +737,17 @@ extern "C" size_t vj_paged_prefill_split_workspace_size(int64_t num_tokens, int3
                           (vj::kD * sizeof(float) + sizeof(float2));
 }
 
-extern "C" vj_status vj_paged_prefill_split(
-    const void *q, const void *k_cache, const void *v_cache, const int32_t *block_tables,
-    const int32_t *cu_seqlens_q, const int32_t *context_lens, void *out, int64_t num_tokens,
-    int32_t num_seqs, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
-    int64_t num_blocks, int32_t block_size, int32_t bt_width, int32_t bt_stride,
-    int64_t stride_block, int64_t stride_token, int64_t stride_head, int32_t max_seqlen_q,
-    int32_t max_context_len, float scale, void *workspace, size_t workspace_bytes,
-    int32_t *error_flag, cudaStream_t stream) {
-  using namespace vj;
-  const std::string what = "vj_paged_prefill_split";
+namespace vj {
+namespace {
+
+int prefill_split(const std::string &what, const void *q, const void *k_cache, const void *v_cache,
+                  const int32_t *block_tables, const int32_t *cu_seqlens_q,
+                  const int32_t *context_lens, void *out, int64_t num_tokens, int32_t num_seqs,
+                  int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int64_t num_blocks,
+                  int32_t block_size, int32_t bt_width, int32_t bt_stride, int64_t stride_block,
+                  int64_t stride_token, int64_t stride_head, int32_t max_seqlen_q,
+                  int32_t max_context_len, float scale, void *workspace, size_t workspace_bytes,
+                  int32_t *error_flag, cudaStream_t stream, bool keep_tail) {
   if (max_context_len < 0) {
     return set_error(VJ_ERR_INVALID_ARGUMENT, what + ": negative or zero size");
   }
@@ -763,6 +766,7 @@ extern "C" vj_status vj_paged_prefill_split(
                          block_size, bt_width, bt_stride, stride_block, stride_token, stride_head,
                          max_seqlen_q, scale, error_flag, true, &a, &mpairs);
   if (rc || mpairs < 0) return rc;
+  a.keep_tail = keep_tail ? 1 : 0;
   a.parts = prefill_parts(mpairs, num_kv_heads, num_seqs, max_context_len);
   const int64_t kv_bytes = 2ll * num_seqs * max_context_len * num_kv_heads * kD * 2;
   a.longest_first = mpairs < num_sms() && kv_bytes <= kResidentKv;
@@ -799,6 +803,39 @@ extern "C" vj_status vj_paged_prefill_split(
                         tmk, tmv, a);
   if (rc || a.parts == 1) return rc;
   return launch_join(what.c_str(), a, stream);
+}
+
+}  // namespace
+}  // namespace vj
+
+extern "C" vj_status vj_paged_prefill_split(
+    const void *q, const void *k_cache, const void *v_cache, const int32_t *block_tables,
+    const int32_t *cu_seqlens_q, const int32_t *context_lens, void *out, int64_t num_tokens,
+    int32_t num_seqs, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+    int64_t num_blocks, int32_t block_size, int32_t bt_width, int32_t bt_stride,
+    int64_t stride_block, int64_t stride_token, int64_t stride_head, int32_t max_seqlen_q,
+    int32_t max_context_len, float scale, void *workspace, size_t workspace_bytes,
+    int32_t *error_flag, cudaStream_t stream) {
+  return vj::prefill_split("vj_paged_prefill_split", q, k_cache, v_cache, block_tables,
+                           cu_seqlens_q, context_lens, out, num_tokens, num_seqs, num_q_heads,
+                           num_kv_heads, head_dim, num_blocks, block_size, bt_width, bt_stride,
+                           stride_block, stride_token, stride_head, max_seqlen_q, max_context_len,
+                           scale, workspace, workspace_bytes, error_flag, stream, false);
+}
+
+extern "C" vj_status vj_paged_prefill_split_part(
+    const void *q, const void *k_cache, const void *v_cache, const int32_t *block_tables,
+    const int32_t *cu_seqlens_q, const int32_t *context_lens, void *out, int64_t num_tokens,
+    int32_t num_seqs, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+    int64_t num_blocks, int32_t block_size, int32_t bt_width, int32_t bt_stride,
+    int64_t stride_block, int64_t stride_token, int64_t stride_head, int32_t max_seqlen_q,
+    int32_t max_context_len, float scale, void *workspace, size_t workspace_bytes,
+    int32_t *error_flag, cudaStream_t stream) {
+  return vj::prefill_split("vj_paged_prefill_split_part", q, k_cache, v_cache, block_tables,
+                           cu_seqlens_q, context_lens, out, num_tokens, num_seqs, num_q_heads,
+                           num_kv_heads, head_dim, num_blocks, block_size, bt_width, bt_stride,
+                           stride_block, stride_token, stride_head, max_seqlen_q, max_context_len,
+                           scale, workspace, workspace_bytes, error_flag, stream, true);
 }
 
 extern "C" size_t vj_paged_attention_mixed_workspace_size(int32_t num_decode,

@@ -1,6 +1,6 @@
 // Prefill attention whose keys are split over CTAs: what the parts leave, and the
-// kernel that joins them. Args has out, cu, num_seqs, num_tokens, Hq, parts, part_o
-// ([parts][tokens][Hq][128] sums in 32 bits, not normalised) and part_ml ([parts]
+// kernel that joins them. Args has out, cu, num_seqs, num_tokens, Hq, parts, keep_tail
+// (rows past the last sequence stay as they are), part_o ([parts][tokens][Hq][128] sums in 32 bits, not normalised) and part_ml ([parts]
 // [tokens][Hq] maximum (log2) and sum of the weights).
 #pragma once
 
@@ -25,7 +25,8 @@ VJ_DEV void zero_tail_share(const Args &a, int i, int n) {
   }
 }
 
-// Joins the parts of the rows [cu[0], cu[num_seqs]) and zeroes those behind. kWarps
+// Joins the parts of the rows [cu[0], cu[num_seqs]) and zeroes those behind (unless
+// they are kept). kWarps
 // warps take a (token, query head), each every kWarps-th part, four of them in flight.
 constexpr int kJoinWarps = 8;
 template <int kWarps, class Args>
@@ -41,7 +42,7 @@ prefill_join_kernel(const Args a) {
   const int64_t end = static_cast<int64_t>(a.cu[a.num_seqs]) * a.Hq;
   uint2 *dst = reinterpret_cast<uint2 *>(a.out + row * 128) + lane;
   const bool mine = row >= first && row < end && row < rows;
-  if (row >= end && row < rows && w == 0) *dst = make_uint2(0u, 0u);
+  if (row >= end && row < rows && w == 0 && !a.keep_tail) *dst = make_uint2(0u, 0u);
   float m = kLowest, l = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   auto add = [&](float2 ml, float4 x) {

@@ -66,7 +66,7 @@ struct QPrefillArgs {
   int bt_stride, pages_per_block, max_pages, num_tokens, num_seqs;
   float scale_log2;
   int32_t *err;
-  int parts;
+  int parts, keep_tail;
   float *part_o;
   float2 *part_ml;
 };
@@ -604,6 +604,7 @@ extern "C" vj_status vj_paged_prefill_quantized(
   a.max_pages = bt_width * a.pages_per_block;
   a.num_tokens = static_cast<int>(num_tokens);
   a.num_seqs = num_seqs;
+  a.keep_tail = 0;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.err = error_flag;
   a.part_o = static_cast<float *>(workspace);

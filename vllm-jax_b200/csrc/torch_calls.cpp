@@ -29,7 +29,7 @@ decltype(&vj_kv_store_quantized) store_entry;
 decltype(&vj_paged_decode_quantized) decode_entry;
 decltype(&vj_paged_decode_quantized_workspace_size) workspace_entry;
 decltype(&vj_kv_read_quantized) read_entry;
-decltype(&vj_paged_prefill_split) prefill_entry;
+decltype(&vj_paged_prefill_split) prefill_entry, prefill_part_entry;
 decltype(&vj_paged_prefill_split_workspace_size) prefill_workspace_entry;
 decltype(&vj_paged_prefill_quantized) direct_entry;
 decltype(&vj_paged_prefill_quantized_workspace_size) direct_workspace_entry;
@@ -525,30 +525,32 @@ PyObject *paged_prefill(PyObject *const *args) {
     at::Tensor more;
     if (part_need > split_bytes) more = at::empty({static_cast<int64_t>(part_need)}, q->options().dtype(at::kByte));
     void *const part_ws = more.defined() ? more.data_ptr() : ws;
+    // the rows behind the last sequence are zeroed once, when all queries are read: out may be q
+    const auto attend = s + n < S ? prefill_part_entry : prefill_entry;
     enter(part_need > 0 ? 2 : 1, [&] {
-      return prefill_entry(q_ptr, k_ptr, static_cast<uint8_t *>(k_ptr) + n * len * row * 2, nullptr,
-                           cu_ptr + s, part.lens, out_ptr, T, n, hq, p.hkv, p.D,
-                           static_cast<int64_t>(std::max(n, 1)) * per_seq, kPage, per_seq, per_seq,
-                           kPage * row, row, p.D, max_new, len, scale, part_ws, part_need,
-                           err, stream);
+      return attend(q_ptr, k_ptr, static_cast<uint8_t *>(k_ptr) + n * len * row * 2, nullptr,
+                    cu_ptr + s, part.lens, out_ptr, T, n, hq, p.hkv, p.D,
+                    static_cast<int64_t>(std::max(n, 1)) * per_seq, kPage, per_seq, per_seq,
+                    kPage * row, row, p.D, max_new, len, scale, part_ws, part_need, err, stream);
     });
   }
   return given ? Py_NewRef(given.o) : THPVariable_Wrap(std::move(out));
 }
 
-// (addresses of the eight entries in the order above, then the three objects)
+// (addresses of the nine entries in the order above, then the three objects)
 PyObject *bind(PyObject *const *args) {
   store_entry = reinterpret_cast<decltype(store_entry)>(integer(args[0]));
   decode_entry = reinterpret_cast<decltype(decode_entry)>(integer(args[1]));
   workspace_entry = reinterpret_cast<decltype(workspace_entry)>(integer(args[2]));
   read_entry = reinterpret_cast<decltype(read_entry)>(integer(args[3]));
   prefill_entry = reinterpret_cast<decltype(prefill_entry)>(integer(args[4]));
-  prefill_workspace_entry = reinterpret_cast<decltype(prefill_workspace_entry)>(integer(args[5]));
-  direct_entry = reinterpret_cast<decltype(direct_entry)>(integer(args[6]));
-  direct_workspace_entry = reinterpret_cast<decltype(direct_workspace_entry)>(integer(args[7]));
-  native = Py_NewRef(args[8]);
-  error_flag_of = Py_NewRef(args[9]);
-  rope_table_of = Py_NewRef(args[10]);
+  prefill_part_entry = reinterpret_cast<decltype(prefill_part_entry)>(integer(args[5]));
+  prefill_workspace_entry = reinterpret_cast<decltype(prefill_workspace_entry)>(integer(args[6]));
+  direct_entry = reinterpret_cast<decltype(direct_entry)>(integer(args[7]));
+  direct_workspace_entry = reinterpret_cast<decltype(direct_workspace_entry)>(integer(args[8]));
+  native = Py_NewRef(args[9]);
+  error_flag_of = Py_NewRef(args[10]);
+  rope_table_of = Py_NewRef(args[11]);
   Py_RETURN_NONE;
 }
 
@@ -574,7 +576,7 @@ PyMethodDef entry(const char *name) {
 }
 PyMethodDef methods[] = {entry<kv_store, 14>("kv_store"), entry<paged_decode, 7>("paged_decode"),
                          entry<read_kv_cache, 5>("read_kv_cache"),
-                         entry<paged_prefill, 10>("paged_prefill"), entry<bind, 11>("bind"),
+                         entry<paged_prefill, 10>("paged_prefill"), entry<bind, 12>("bind"),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_torch_calls", nullptr, -1, methods};
 

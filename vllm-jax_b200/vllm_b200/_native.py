@@ -70,6 +70,13 @@ PROTOTYPES: dict[str, tuple] = {
         c_i64, c_i64, c_i64,                        # strides
         c_i32, c_i32, c_f32,                        # max_seqlen_q, max_context_len, scale
         c_vp, c_sz, c_vp, c_vp]),                   # workspace, bytes, err, stream
+    "vj_paged_prefill_split_part": (c_int, [
+        c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp,   # q, k, v, bt, cu_q, ctx_lens, out
+        c_i64, c_i32, c_i32, c_i32, c_i32,          # T, S, Hq, Hkv, D
+        c_i64, c_i32, c_i32, c_i32,                 # nb, bs, bt_width, bt_stride
+        c_i64, c_i64, c_i64,                        # strides
+        c_i32, c_i32, c_f32,                        # max_seqlen_q, max_context_len, scale
+        c_vp, c_sz, c_vp, c_vp]),                   # workspace, bytes, err, stream
     "vj_paged_prefill_quantized_workspace_size": (c_sz, [c_i64, c_i32, c_i32, c_i32, c_i32, c_i32,
                                                          c_i32]),
     "vj_paged_prefill_quantized": (c_int, [

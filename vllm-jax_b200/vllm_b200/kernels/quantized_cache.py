@@ -64,7 +64,8 @@ def _bound():
             calls.bind(*(_native.address(name) for name in
                          ("vj_kv_store_quantized", "vj_paged_decode_quantized",
                           "vj_paged_decode_quantized_workspace_size", "vj_kv_read_quantized",
-                          "vj_paged_prefill_split", "vj_paged_prefill_split_workspace_size",
+                          "vj_paged_prefill_split", "vj_paged_prefill_split_part",
+                          "vj_paged_prefill_split_workspace_size",
                           "vj_paged_prefill_quantized",
                           "vj_paged_prefill_quantized_workspace_size")),
                        _native, _error_address, rope_table)
@@ -145,7 +146,7 @@ def paged_prefill_quantized(q: torch.Tensor, cache: QuantizedKVCache, block_tabl
     exact, once instead of once per query tile. max_seqlen_q and max_context_len:
     bounds on the new tokens and on context_lens (default: all tokens, and what a
     block table row holds); they size the grid and the scratch, and decide how the
-    keys are split. scale: positive. Rows behind cu_seqlens_q[-1] come out 0."""
+    keys are split. scale: positive. Rows behind cu_seqlens_q[-1] come out 0. `out` may be q."""
     return (_calls or _bound()).paged_prefill(q, cache, block_tables, cu_seqlens_q, context_lens,
                                               int(max_seqlen_q), scale, out, int(max_context_len),
                                               PREFILL_SCRATCH_ROWS)
