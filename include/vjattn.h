@@ -474,7 +474,7 @@ VJ_API vj_status vj_allreduce_add_rmsnorm(
  *   device (0 without a split: may be NULL), 16-byte aligned, need not be
  *   initialised; calls whose kernels may overlap need one each
  *   scale: positive and finite
- * out may be q. */
+ * out may be q, or must not overlap it. */
 VJ_API size_t vj_paged_prefill_split_workspace_size(int64_t num_tokens, int32_t num_seqs,
                                                     int32_t num_q_heads, int32_t num_kv_heads,
                                                     int32_t head_dim, int32_t max_seqlen_q,
@@ -583,7 +583,7 @@ VJ_API vj_status vj_paged_decode_quantized(
 /* Causal attention of few new tokens over the quantised cache, straight from its
  * pages: q, out, cu_seqlens_q, context_lens (new tokens included; not NULL),
  * max_seqlen_q as in vj_paged_prefill, the cache as above. Rows of out behind
- * cu_seqlens_q[num_seqs] are zeroed; out may be q. The keys of a row tile (128 rows of tokens x
+ * cu_seqlens_q[num_seqs] are zeroed; out may be q, or must not overlap it. The keys of a row tile (128 rows of tokens x
  * query heads of one KV head) are split over CTAs that would be idle. Where there
  * are many row tiles, vj_kv_read_quantized (zero_to = 128, max_len a multiple of
  * 128) and vj_paged_prefill_split on what it leaves are faster.

@@ -100,3 +100,17 @@ def test_prefill_in_the_queries_place(Hq, Hkv, new, prefix, groups, launches, mo
     assert torch.equal(q, ref)
     _check(q, *case.reference(), PREFILL)
 
+
+
+@pytest.mark.parametrize("Hq,Hkv,new,prefix", [(8, 2, (20, 60), (0, 30)),
+                                               (32, 8, (900, 1000), (0, 100))])
+def test_prefill_refuses_an_output_that_lies_across_the_queries(Hq, Hkv, new, prefix):
+    case = _Prompts(Hq, Hkv, new, prefix)
+    T = case.q.shape[0]
+    both = torch.cat([case.q, case.q[:1]])
+    kept = both.clone()
+    for q, out in ((both[:T], both[1:]), (both[1:], both[:T])):
+        with pytest.raises(ValueError, match="overlap"):
+            case.call(q, out=out)
+    torch.cuda.synchronize()
+    assert torch.equal(both, kept)

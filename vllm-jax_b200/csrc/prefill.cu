@@ -766,6 +766,9 @@ int prefill_split(const std::string &what, const void *q, const void *k_cache, c
                          block_size, bt_width, bt_stride, stride_block, stride_token, stride_head,
                          max_seqlen_q, scale, error_flag, true, &a, &mpairs);
   if (rc || mpairs < 0) return rc;
+  if (overlap_in_part(q, out, num_tokens * num_q_heads * kD * 2)) {
+    return set_error(VJ_ERR_INVALID_ARGUMENT, what + ": out must be q or not overlap it");
+  }
   a.keep_tail = keep_tail ? 1 : 0;
   a.parts = prefill_parts(mpairs, num_kv_heads, num_seqs, max_context_len);
   const int64_t kv_bytes = 2ll * num_seqs * max_context_len * num_kv_heads * kD * 2;

@@ -6,8 +6,17 @@
 
 #include "vj_common.cuh"
 
+#include <cstdint>
+
 namespace vj {
 namespace {
+
+// Whether two buffers of this many bytes overlap without being the same: a tile reads
+// its own rows of q alone before it writes them, so out may be q, but not lie across it.
+inline bool overlap_in_part(const void *x, const void *y, int64_t bytes) {
+  const auto p = reinterpret_cast<uintptr_t>(x), r = reinterpret_cast<uintptr_t>(y);
+  return p != r && (p < r ? r - p : p - r) < static_cast<uint64_t>(bytes);
+}
 
 constexpr float kLowest = -1e30f;       // a maximum that no key has moved yet
 

@@ -571,6 +571,9 @@ extern "C" vj_status vj_paged_prefill_quantized(
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) % 16 != 0) {
     return set_error(VJ_ERR_INVALID_ARGUMENT, what + ": q and out must be 16-byte aligned");
   }
+  if (overlap_in_part(q, out, num_tokens * num_q_heads * kD * 2)) {
+    return set_error(VJ_ERR_INVALID_ARGUMENT, what + ": out must be q or not overlap it");
+  }
   a.tt = kRows / a.g;
   const int64_t longest = max_seqlen_q > 0 ? max_seqlen_q : num_tokens;
   const int64_t tiles = num_seqs > 0 ? (longest + a.tt - 1) / a.tt : 1;

@@ -146,7 +146,8 @@ def paged_prefill_quantized(q: torch.Tensor, cache: QuantizedKVCache, block_tabl
     exact, once instead of once per query tile. max_seqlen_q and max_context_len:
     bounds on the new tokens and on context_lens (default: all tokens, and what a
     block table row holds); they size the grid and the scratch, and decide how the
-    keys are split. scale: positive. Rows behind cu_seqlens_q[-1] come out 0. `out` may be q."""
+    keys are split. scale: positive. Rows behind cu_seqlens_q[-1] come out 0. `out` may be
+    q, or must not overlap it."""
     return (_calls or _bound()).paged_prefill(q, cache, block_tables, cu_seqlens_q, context_lens,
                                               int(max_seqlen_q), scale, out, int(max_context_len),
                                               PREFILL_SCRATCH_ROWS)
