@@ -37,3 +37,21 @@ def test_prefill_refuses_an_output_that_lies_across_the_queries(entry, kw, overl
         assert status == _native.VJ_ERR_INVALID_ARGUMENT and b"overlap" in lib.vj_get_last_error()
     else:
         assert status == _native.VJ_ERR_WORKSPACE
+
+
+@pytest.mark.parametrize("size", ["vj_paged_prefill_split_workspace_size",
+                                  "vj_paged_prefill_quantized_workspace_size"])
+@pytest.mark.parametrize("Hq,Hkv", [(64, 8), (8, 8), (16, 1)])
+@pytest.mark.parametrize("new", [1, 64, 300, 2048])
+def test_prefill_workspace_is_bounded_however_large_the_batch(size, Hq, Hkv, new):
+    """Room for the rows of the sequences asked for, split over as many CTAs as the GPU
+    holds (148 of 256 rows, and a part's row is 130 32-bit words), not for the whole
+    batch's rows."""
+    from vllm_b200 import _native
+    f = getattr(_native.load(), size)
+    most = 148 * 256 * 130 * 4
+    assert f(1, 1, Hq, Hkv, 128, 1, 1 << 16) > 0
+    for seqs in (1, 2, 9):
+        for batch in (9, 257):
+            need = f(batch * new, seqs, Hq, Hkv, 128, new, 1 << 16)
+            assert need == f(seqs * new, seqs, Hq, Hkv, 128, new, 1 << 16) <= most

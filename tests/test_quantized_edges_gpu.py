@@ -114,3 +114,47 @@ def test_prefill_refuses_an_output_that_lies_across_the_queries(Hq, Hkv, new, pr
             case.call(q, out=out)
     torch.cuda.synchronize()
     assert torch.equal(both, kept)
+
+
+@pytest.mark.parametrize("most,sizes", [(4, (3, 4)), (4, (3, 3)), (2, (1, 2, 2, 2)), (1, (1,) * 6)])
+def test_prefill_in_uneven_groups_with_split_keys(most, sizes, monkeypatch):
+    """Groups of sequences read back one after another, where some are split further over
+    their keys than others: a group's parts begin at its own first token."""
+    from vllm_b200 import _native
+    from vllm_b200.kernels import quantized_cache as qc
+    new = (130, 0, 140, 129, 1, 140, 133)[:sum(sizes)]
+    prefix = (2200, 30, 1100, 2000, 1500, 1024, 2290)[:sum(sizes)]
+    case = _Prompts(32, 8, new, prefix, "int8", 32, seed=1)
+    padded = -(-max(case.ctx) // 128) * 128                  # rows that a sequence takes
+    monkeypatch.setattr(qc, "PREFILL_SCRATCH_ROWS", most * padded * 8)
+    before = _native.launch_count
+    out = torch.full_like(case.q, float("nan"))
+    case.call(out=out)
+    parts = [_native.load().vj_paged_prefill_split_workspace_size(
+        case.q.shape[0], n, 32, 8, D, max(new), max(case.ctx)) > 0 for n in sizes]
+    assert _native.launch_count - before == sum(2 + p for p in parts) and any(parts)
+    _check(out, *case.reference(), PREFILL)
+
+
+def test_prefill_scratch_of_many_small_groups_is_bounded(monkeypatch):
+    """A group's share of the scratch does not grow with the batch: 40 sequences of 64 new
+    tokens one after another, contexts of up to 8192."""
+    from vllm_b200.kernels import quantized_cache as qc
+    S, n, bound = 40, 64, 8192
+    cache = qc.QuantizedKVCache.zeros(S * 4, 16, 8, device="cuda")
+    cache.data.view(torch.uint8).fill_(0x38)                   # ones
+    q = torch.randn((S * n, 64, D), device="cuda").to(torch.bfloat16)
+    bt = torch.zeros((S, bound // 16), dtype=torch.int32, device="cuda")
+    out, cu, ln = torch.empty_like(q), _i(np.arange(S + 1) * n), _i(np.full(S, n))
+    monkeypatch.setattr(qc, "PREFILL_SCRATCH_ROWS", 1)
+    qc.paged_prefill_quantized(q, cache, bt, cu, ln, n, out=out, max_context_len=bound)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    held = torch.cuda.memory_allocated()
+    qc.paged_prefill_quantized(q, cache, bt, cu, ln, n, out=out, max_context_len=bound)
+    torch.cuda.synchronize()
+    took = torch.cuda.max_memory_allocated() - held
+    # K and V of one sequence, and the parts' rows of one (148 CTAs of 256, 130 words each)
+    assert took <= 2 * bound * 8 * D * 2 + 148 * 256 * 130 * 4 + (2 << 20)
+    scale = cache.scales[0, 0, 0, 0].float()                  # every row of V is this one
+    assert torch.equal(out, torch.full_like(out, float(torch.exp2(scale - 127))))

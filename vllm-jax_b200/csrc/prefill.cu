@@ -129,11 +129,12 @@ struct PrefillArgs {
   int num_tokens;
   float scale_log2;
   int *err;
-  // key split: parts of a tile pair's key tiles, and what they leave per (part, token, head)
+  // key split: parts of a tile pair's key tiles, and what they leave (prefill_join.cuh)
   int parts, num_seqs, longest_first;
   int keep_tail;            // whether rows past the last sequence are left as they are
-  float *part_o;            // [parts][tokens][Hq][128]
-  float2 *part_ml;          // [parts][tokens][Hq] maximum (log2), sum
+  int part_rows;            // tokens of a part, from the first sequence's first on
+  float *part_o;            // [parts][part_rows][Hq][128]
+  float2 *part_ml;          // [parts][part_rows][Hq] maximum (log2), sum
 };
 
 // Token coordinate (flat pool token index of the page's first token) of page
@@ -247,9 +248,9 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap *tmq_p, const CUt
     nkv = static_cast<int>(static_cast<int64_t>(all) * (part + 1) / a.parts) - j0;
     if (nkv == 0) {                                // more parts than key tiles
       const int t = threadIdx.x / kBM, r = threadIdx.x % kBM, tq = tq0 + t * a.tt + r / a.g;
-      if (t < 2 && tq < n && q0 + tq < a.num_tokens) {
-        a.part_ml[(static_cast<int64_t>(part) * a.num_tokens + q0 + tq) * a.Hq + h * a.g + r % a.g] =
-            make_float2(kLowest, 0.f);
+      const int64_t rel = row_of_part(a, a.cu[0], q0 + tq);
+      if (t < 2 && tq < n && rel >= 0) {
+        a.part_ml[place_in_parts(a, part, rel, h * a.g + r % a.g)] = make_float2(kLowest, 0.f);
       }
       __syncwarp();
       if (warp == kWarpMma) tmem_dealloc(tmem, 512);
@@ -434,14 +435,15 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap *tmq_p, const CUt
       const float inv = 1.f / l_run;
       const bool valid = tq < n && q0 + tq < a.num_tokens;
       if (kSplit && a.parts > 1) {
-        const int64_t at =
-            (static_cast<int64_t>(part) * a.num_tokens + q0 + tq) * a.Hq + h * a.g + r % a.g;
-        if (valid) a.part_ml[at] = make_float2(m_run, l_run);
+        const int64_t rel = row_of_part(a, a.cu[0], q0 + tq);
+        const int64_t at = place_in_parts(a, part, rel, h * a.g + r % a.g);
+        const bool in_parts = tq < n && rel >= 0;
+        if (in_parts) a.part_ml[at] = make_float2(m_run, l_run);
 #pragma unroll 1
         for (int c = 0; c < kD / 32; ++c) {
           float o[32];
           tmem_ld32(tO + c * 32, o);
-          if (valid) {
+          if (in_parts) {
             float4 *dst = reinterpret_cast<float4 *>(a.part_o + at * kD + c * 32);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
@@ -643,6 +645,7 @@ int prefill_setup(const std::string &what, const void *q, const void *k_cache, c
   a.err = error_flag;
   a.parts = 1;
   a.num_seqs = num_seqs;
+  a.part_rows = 0;
   a.longest_first = 0;
   a.keep_tail = 0;
   a.part_o = nullptr;
@@ -733,7 +736,8 @@ extern "C" size_t vj_paged_prefill_split_workspace_size(int64_t num_tokens, int3
   const int parts =
       vj::prefill_parts((maxq + tt2 - 1) / tt2, num_kv_heads, num_seqs, max_context_len);
   return parts == 1 ? 0
-                    : static_cast<size_t>(parts) * num_tokens * num_q_heads *
+                    : static_cast<size_t>(parts) * vj::rows_of_parts(num_tokens, num_seqs, maxq) *
+                          num_q_heads *
                           (vj::kD * sizeof(float) + sizeof(float2));
 }
 
@@ -774,6 +778,8 @@ int prefill_split(const std::string &what, const void *q, const void *k_cache, c
   const int64_t kv_bytes = 2ll * num_seqs * max_context_len * num_kv_heads * kD * 2;
   a.longest_first = mpairs < num_sms() && kv_bytes <= kResidentKv;
   const int64_t rows = num_tokens * num_q_heads;
+  a.part_rows = static_cast<int>(
+      rows_of_parts(num_tokens, num_seqs, max_seqlen_q > 0 ? max_seqlen_q : num_tokens));
   if (a.parts > 1) {
     const size_t need = vj_paged_prefill_split_workspace_size(
         num_tokens, num_seqs, num_q_heads, num_kv_heads, head_dim, max_seqlen_q, max_context_len);
@@ -782,7 +788,8 @@ int prefill_split(const std::string &what, const void *q, const void *k_cache, c
                                              " bytes, 16-byte aligned");
     }
     a.part_o = static_cast<float *>(workspace);
-    a.part_ml = reinterpret_cast<float2 *>(a.part_o + a.parts * rows * kD);
+    a.part_ml = reinterpret_cast<float2 *>(
+        a.part_o + static_cast<int64_t>(a.parts) * a.part_rows * num_q_heads * kD);
   }
   const int64_t z = std::max<int64_t>(static_cast<int64_t>(num_seqs) * a.parts, 1);
   if (z > 65535 || rows > INT32_MAX) {

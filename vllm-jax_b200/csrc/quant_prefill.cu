@@ -66,7 +66,7 @@ struct QPrefillArgs {
   int bt_stride, pages_per_block, max_pages, num_tokens, num_seqs;
   float scale_log2;
   int32_t *err;
-  int parts, keep_tail;
+  int parts, part_rows, keep_tail;             // prefill_join.cuh
   float *part_o;
   float2 *part_ml;
 };
@@ -279,7 +279,7 @@ quant_prefill_kernel(const __grid_constant__ CUtensorMap tmq, const QPrefillArgs
     zero_tail_share(a, threadIdx.x, kPrefillThreads);
     return;
   }
-  const int q0 = a.cu[s], q1 = a.cu[s + 1];
+  const int first = a.cu[0], q0 = a.cu[s], q1 = a.cu[s + 1];
   int ctx = a.lens[s];
   const int n = q1 - q0;
   const int tq0 = (gridDim.x - 1 - blockIdx.x) * a.tt;     // first token of the row tile
@@ -296,9 +296,11 @@ quant_prefill_kernel(const __grid_constant__ CUtensorMap tmq, const QPrefillArgs
   const int half = threadIdx.x / kRows, r = threadIdx.x % kRows, tq = tq0 + r / a.g;
   const bool valid = half < 2 && tq < n && q0 + tq < a.num_tokens;
   const int64_t row = static_cast<int64_t>(q0 + tq) * a.Hq + h * a.g + r % a.g;
-  const int64_t part_row = static_cast<int64_t>(part) * a.num_tokens * a.Hq + row;
+  const int64_t rel = row_of_part(a, first, q0 + tq);
+  const bool in_parts = valid && rel >= 0;
+  const int64_t part_row = place_in_parts(a, part, rel, h * a.g + r % a.g);
   if (nkv == 0) {              // more parts than key tiles
-    if (valid && half == 0) a.part_ml[part_row] = make_float2(kLowest, 0.f);
+    if (in_parts && half == 0) a.part_ml[part_row] = make_float2(kLowest, 0.f);
     return;
   }
   if (warp == 16) tmem_alloc(&bar.tmem, 512);
@@ -440,7 +442,7 @@ quant_prefill_kernel(const __grid_constant__ CUtensorMap tmq, const QPrefillArgs
       const float m = fmaxf(ml0.x, ml1.x), g0 = exp2f(ml0.x - m), g1 = exp2f(ml1.x - m);
       const float l = ml0.y * g0 + ml1.y * g1, inv = a.parts > 1 ? 1.f : 1.f / l;
       const float f0 = g0 * inv, f1 = g1 * inv;
-      if (a.parts > 1 && valid && half == 0) a.part_ml[part_row] = make_float2(m, l);
+      if (a.parts > 1 && in_parts && half == 0) a.part_ml[part_row] = make_float2(m, l);
 #pragma unroll 1
       for (int k = 2 * half; k < 2 * half + 2; ++k) {
         float o[32], o1[32];
@@ -448,13 +450,13 @@ quant_prefill_kernel(const __grid_constant__ CUtensorMap tmq, const QPrefillArgs
         tmem_ld32(tO + kD + k * 32, o1);
 #pragma unroll
         for (int i = 0; i < 32; ++i) o[i] = o[i] * f0 + o1[i] * f1;
-        if (valid && a.parts > 1) {
+        if (a.parts > 1 && in_parts) {
           float4 *dst = reinterpret_cast<float4 *>(a.part_o + part_row * kD + k * 32);
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             dst[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
           }
-        } else if (valid) {
+        } else if (a.parts == 1 && valid) {
           uint4 *dst = reinterpret_cast<uint4 *>(a.out + row * kD + k * 32);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -521,7 +523,8 @@ extern "C" size_t vj_paged_prefill_quantized_workspace_size(int64_t num_tokens, 
   const int parts = vj::quant_prefill_parts((longest + tt - 1) / tt, num_kv_heads, num_seqs,
                                             max_context_len);
   return parts == 1 ? 0
-                    : static_cast<size_t>(parts) * num_tokens * num_q_heads *
+                    : static_cast<size_t>(parts) * vj::rows_of_parts(num_tokens, num_seqs, longest) *
+                          num_q_heads *
                           (vj::kD * sizeof(float) + sizeof(float2));
 }
 
@@ -611,7 +614,10 @@ extern "C" vj_status vj_paged_prefill_quantized(
   a.scale_log2 = scale * 1.4426950408889634f;
   a.err = error_flag;
   a.part_o = static_cast<float *>(workspace);
-  a.part_ml = a.parts > 1 ? reinterpret_cast<float2 *>(a.part_o + a.parts * rows * kD) : nullptr;
+  a.part_rows = static_cast<int>(rows_of_parts(num_tokens, num_seqs, longest));
+  a.part_ml = a.parts > 1 ? reinterpret_cast<float2 *>(
+                                a.part_o + static_cast<int64_t>(a.parts) * a.part_rows * num_q_heads * kD)
+                          : nullptr;
   const dim3 grid(static_cast<unsigned>(tiles), static_cast<unsigned>(num_kv_heads),
                   static_cast<unsigned>(z));
   rc = cache_dtype == VJ_CACHE_INT8 ? launch_quant_prefill<true>(what, tmq, a, grid, stream)

@@ -439,7 +439,7 @@ bool direct_prefill(int64_t S, int64_t T, int64_t hq, const Pool &p, int64_t lon
   const int64_t g = hq / p.hkv;
   if (S == 0 || T == 0) return true;
   if (g == 0 || 128 % g != 0) return false;            // the other way refuses it
-  const int64_t part_bytes = T * hq * (p.D + 2) * 4, keys = (len + 127) / 128;
+  const int64_t part_bytes = std::min(T, S * longest) * hq * (p.D + 2) * 4, keys = (len + 127) / 128;
   auto cost = [&](int64_t rows, size_t bytes, double start, double tile) {
     const int64_t tt = rows / g, tiles = std::min((longest + tt - 1) / tt * S, T / tt + S);
     const int64_t parts = std::max<int64_t>(1, bytes / part_bytes);
@@ -507,31 +507,33 @@ PyObject *paged_prefill(PyObject *const *args) {
   // the scratch: K and V, where page i of a group's sequence b is block b * per_seq
   // + i, then what a split over keys needs
   const int64_t row = static_cast<int64_t>(p.hkv) * p.D;
-  const int64_t group = std::max<int64_t>(
+  const int64_t most_seqs = std::max<int64_t>(
       1, std::min<int64_t>(S, integer(args[9]) / (static_cast<int64_t>(len) * p.hkv)));
+  // groups of the same size, or one sequence less
+  const int64_t groups = S ? (S + most_seqs - 1) / most_seqs : 1, group = (S + groups - 1) / groups;
   const int32_t per_seq = len / kPage;
-  const size_t split_bytes = prefill_workspace_entry(T, static_cast<int32_t>(std::min<int64_t>(group, S)),
-                                                     hq, p.hkv, p.D, max_new, len);
+  size_t split_bytes = 0;               // (a smaller group may be split further)
+  for (int64_t n = group; n >= std::max<int64_t>(group - 1, 0); --n) {
+    split_bytes = std::max(split_bytes, prefill_workspace_entry(T, static_cast<int32_t>(n), hq, p.hkv,
+                                                                p.D, max_new, len));
+  }
   const at::Tensor scratch = at::empty(
       {2 * group * len * row + static_cast<int64_t>(split_bytes / 2)}, q->options());
   void *const k_ptr = scratch.data_ptr();
   void *const ws = static_cast<uint8_t *>(k_ptr) + 4 * group * len * row;
-  for (int64_t s = 0; s < std::max(S, 1); s += group) {
-    const int32_t n = static_cast<int32_t>(std::min<int64_t>(group, S - s));
+  for (int64_t i = 0; i < groups; ++i) {
+    const int64_t s = S * i / groups;
+    const int32_t n = static_cast<int32_t>(S * (i + 1) / groups - s);
     const Tables part = {t.ptr + s * t.stride, t.lens + s, t.width, t.stride};
     read_back(p, part, k_ptr, n, len, kKeyTile, stream);
-    // (the last group may be smaller and split further than the others)
     const size_t part_need = prefill_workspace_entry(T, n, hq, p.hkv, p.D, max_new, len);
-    at::Tensor more;
-    if (part_need > split_bytes) more = at::empty({static_cast<int64_t>(part_need)}, q->options().dtype(at::kByte));
-    void *const part_ws = more.defined() ? more.data_ptr() : ws;
     // the rows behind the last sequence are zeroed once, when all queries are read: out may be q
     const auto attend = s + n < S ? prefill_part_entry : prefill_entry;
     enter(part_need > 0 ? 2 : 1, [&] {
       return attend(q_ptr, k_ptr, static_cast<uint8_t *>(k_ptr) + n * len * row * 2, nullptr,
                     cu_ptr + s, part.lens, out_ptr, T, n, hq, p.hkv, p.D,
                     static_cast<int64_t>(std::max(n, 1)) * per_seq, kPage, per_seq, per_seq,
-                    kPage * row, row, p.D, max_new, len, scale, part_ws, part_need, err, stream);
+                    kPage * row, row, p.D, max_new, len, scale, ws, part_need, err, stream);
     });
   }
   return given ? Py_NewRef(given.o) : THPVariable_Wrap(std::move(out));
