@@ -523,10 +523,11 @@ VJ_API vj_status vj_paged_prefill_split_part(
 /* vj_kv_store_qknorm_rope for the quantised cache: per-head RMSNorm
  * (VJ_KV_NORM) and RoPE (VJ_KV_ROPE, interleaved pairs, rope_table as there)
  * of q and k; q_out in bf16, k and v into their slots. A row of q is computed
- * in 32 bits and rounded once at the end; one of k in 32 bits where those
- * decide its rounding, else in 64, so a cached row is the correctly rounded one (q of vj_kv_store_qknorm_rope is
- * rounded to bf16 after every step as the reference does, so the two differ by
- * roundings). Tokens whose slot lies outside [0, num_blocks*block_size) store
+ * in 32 bits and rounded once at the end (a mean square plus eps outside of
+ * their normal numbers loses bits, or is 0 or infinite); one of k in 32 bits where those decide its
+ * rounding, else in 64, so a cached row is the correctly rounded one, whatever
+ * its magnitude and eps (q of vj_kv_store_qknorm_rope is rounded to bf16 after
+ * every step as the reference does, so the two differ by roundings). Tokens whose slot lies outside [0, num_blocks*block_size) store
  * nothing (their q is still written). Slots that are stored must differ from
  * each other within a call. q_out may equal q_in with the same row stride.
  *   q_out [T,Hq,D] with row stride q_out_row_stride (0: packed); num_q_heads

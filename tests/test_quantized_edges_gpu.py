@@ -158,3 +158,42 @@ def test_prefill_scratch_of_many_small_groups_is_bounded(monkeypatch):
     assert took <= 2 * bound * 8 * D * 2 + 148 * 256 * 130 * 4 + (2 << 20)
     scale = cache.scales[0, 0, 0, 0].float()                  # every row of V is this one
     assert torch.equal(out, torch.full_like(out, float(torch.exp2(scale - 127))))
+
+
+# ----------------------------------------------------------------------------- store
+@pytest.mark.parametrize("dtype", ["e4m3", "int8"])
+@pytest.mark.parametrize("eps", [1e-6, 0.0, 1e-38, 1e-12, 1e30, -1e-8])
+def test_stored_k_rows_of_every_magnitude_are_correctly_rounded(dtype, eps):
+    """Normalised and turned rows from 2^-130 to 2^125, whose squares leave the range of
+    32 bits at both ends, and rows of zeros, infinities and NaN."""
+    from vllm_b200.kernels.kv_store import rope_table
+    from vllm_b200.kernels.quantized_cache import QuantizedKVCache, kv_store_quantized
+    rng = np.random.default_rng(31)
+    T, Hkv, bs = 256, 3, 16
+    with np.errstate(over="ignore"):
+        kv = bf16(rng.standard_normal((T, 2 * Hkv, D)) * np.exp2(np.arange(T) - 130.0)[:, None, None])
+    kv[5] = 0
+    kv[200, :, 3] = np.inf
+    kv[201, :, 100] = np.nan
+    kv[202, 0] = 0
+    kv[202, 0, 64] = bf16(np.float32(1e-40))
+    kv[203] = 0
+    kv[203, :, 7] = bf16(np.float32(3e38))
+    w = bf16(1 + 0.3 * rng.standard_normal(D))
+    pos = rng.integers(0, 4096, T)
+    slots = rng.permutation(T)
+    table = rope_table(torch.device("cuda", 0), 1e6, 4096)
+    cache = QuantizedKVCache.zeros(T // bs, bs, Hkv, dtype=dtype, device="cuda")
+    d = _t(kv)
+    kv_store_quantized(None, d[:, :Hkv], d[:, Hkv:], cache, _i(slots), _i(pos), None, _t(w), eps=eps,
+                       table=table)
+    cs = table.view(torch.bfloat16).double().cpu().numpy().reshape(-1, D // 2, 2)[pos]
+    x = kv.astype(np.float64)
+    with np.errstate(invalid="ignore", over="ignore", divide="ignore"):
+        rows = oq.norm_rope(x[:, :Hkv], w.astype(np.float64), cs, eps), x[:, Hkv:]
+        new = [oq.quantise_rows(y, dtype) for y in rows]
+    data, scales = cache.data.view(torch.uint8).cpu().numpy(), cache.scales.cpu().numpy()
+    for i in range(2):
+        got = data[i].reshape(T, Hkv, D)[slots], scales[i].transpose(0, 2, 1).reshape(T, Hkv)[slots]
+        np.testing.assert_array_equal(got[1], new[i][1], err_msg="scales of " + "kv"[i])
+        np.testing.assert_array_equal(got[0], new[i][0], err_msg="elements of " + "kv"[i])

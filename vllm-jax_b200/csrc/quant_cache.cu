@@ -74,8 +74,8 @@ VJ_DEV Turn make_turn(const RowSlice &w, const RowSlice &cs) {
 // u, 2i + 1 in z. Relative error below 12.5 * 2^-24: the sum of squares adds
 // 128 exact squares in at most 11 roundings, then eps (its own cast and one
 // more), which the root halves to 6.25; rsqrtf 4, the turn 1 (its products are
-// exact), the last product 1.
-VJ_DEV void turn_row(uint64_t (&u)[4], uint64_t (&z)[4], const RowSlice &x, const Turn &t,
+// exact), the last product 1. That holds where decided_range() does. Returns 1 / rms.
+VJ_DEV float turn_row(uint64_t (&u)[4], uint64_t (&z)[4], const RowSlice &x, const Turn &t,
                      unsigned mask, const StoreArgs &a) {
   uint64_t x0[4], x1[4];
 #pragma unroll
@@ -108,6 +108,16 @@ VJ_DEV void turn_row(uint64_t (&u)[4], uint64_t (&z)[4], const RowSlice &x, cons
     u[j] = f32x2_mul(u[j], inv2);
     z[j] = f32x2_mul(z[j], inv2);
   }
+  return inv;
+}
+// Whether nothing of a row in turn_row has left the range of 32 bits so far that its bound
+// fails: 1 / rms in 2^-40 .. 2^20 (squares of a mean above 2^-40 that are subnormal, off by
+// 2^-150 each, do not count in it), the result's largest magnitude in 2^-80 .. 2^120 (before
+// the last product it is then above 2^-100, against which subnormal products, off by 2^-149,
+// do not count either), and no negative eps that the mean square cancels with.
+VJ_DEV bool decided_range(float inv, uint32_t amax_bits, const StoreArgs &a) {
+  return inv >= 0x1p-40f && inv <= 0x1p20f && amax_bits >= (47u << 23) &&
+         amax_bits < (247u << 23) && (!a.norm || a.eps >= 0.0);
 }
 
 // One row of q: rounded to bf16 at the end.
@@ -229,7 +239,7 @@ template <bool kInt8>
 VJ_DEV void k_row(uint32_t (&o)[4], int &e, bool &bad, const uint8_t *row, const RowSlice &cs,
                   const Turn &t, unsigned mask, const StoreArgs &a) {
   uint64_t u[4], z[4];
-  turn_row(u, z, load_slice(row, threadIdx.x & 7), t, mask, a);
+  const float inv = turn_row(u, z, load_slice(row, threadIdx.x & 7), t, mask, a);
   uint32_t amax = 0;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
@@ -243,9 +253,9 @@ VJ_DEV void k_row(uint32_t (&o)[4], int &e, bool &bad, const uint8_t *row, const
   bad = false;
   e = scale_exponent<kInt8>(amax);
   const float f = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);   // 2^-e
-  // undecided too: outside of 2^-100 .. 2^120 (sums and products of 32 bits may have
-  // left their range), and the largest element next to where the exponent moves
-  bool open = amax < (27u << 23) || amax >= (247u << 23) ||
+  // undecided too: rows out of 32 bits' range, and the largest element next to where the
+  // exponent moves
+  bool open = !decided_range(inv, amax, a) ||
               __usad(amax & 0x7fffffu, kInt8 ? 0x7e0000u : 0x600000u, 0u) <= 16u;
   const uint64_t up = f32x2(f * (1.f + 0x1p-20f), f * (1.f + 0x1p-20f));
   const uint64_t down = f32x2(f * (1.f - 0x1p-20f), f * (1.f - 0x1p-20f));
