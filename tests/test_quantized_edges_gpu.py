@@ -197,3 +197,25 @@ def test_stored_k_rows_of_every_magnitude_are_correctly_rounded(dtype, eps):
         got = data[i].reshape(T, Hkv, D)[slots], scales[i].transpose(0, 2, 1).reshape(T, Hkv)[slots]
         np.testing.assert_array_equal(got[1], new[i][1], err_msg="scales of " + "kv"[i])
         np.testing.assert_array_equal(got[0], new[i][0], err_msg="elements of " + "kv"[i])
+
+
+# ----------------------------------------------------------------------------- decode
+@pytest.mark.parametrize("dtype", ["e4m3", "int8"])
+def test_rows_that_nothing_stored_count_as_zeros(dtype):
+    """Rows of a fresh pool inside a context, next to values of 1e-6: their scales must not
+    outweigh the others'."""
+    from vllm_b200.kernels.quantized_cache import (QuantizedKVCache, kv_store_quantized,
+                                                   paged_decode_quantized)
+    rng = np.random.default_rng(32)
+    cache = QuantizedKVCache.zeros(4, 16, 2, dtype=dtype, device="cuda")
+    n = 40
+    slots = np.arange(n)
+    slots[[3, 20, 39]] = -1
+    k, v = bf16(rng.standard_normal((n, 2, D))), bf16(1e-6 * rng.standard_normal((n, 2, D)))
+    kv_store_quantized(None, _t(k), _t(v), cache, _i(slots), norm=False, rope=False)
+    q = bf16(rng.standard_normal((1, 8, D)))
+    out = paged_decode_quantized(_t(q), cache, _i([[0, 1, 2, 3]]), _i([n]))
+    codes, scales = cache.data.view(torch.uint8).cpu().numpy(), cache.scales.cpu().numpy()
+    vals = [oq.gather(oq.dequantise(codes[i], scales[i], dtype), np.arange(4), n) for i in range(2)]
+    assert not vals[1][[3, 20, 39]].any() and vals[1][4].any()
+    _check(out, *oq.attend(q.astype(np.float64), *vals, n - 1, 1 / math.sqrt(D)), DECODE)

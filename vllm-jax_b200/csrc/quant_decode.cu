@@ -579,9 +579,9 @@ quant_decode_kernel(const __grid_constant__ CUtensorMap tm_rows,
       }
     }
     const uint32_t vb0 = lds8(vsb + r), vb1 = lds8(vsb + r + 8);
-    const float ev0 = vb0 == 255u ? __uint_as_float(0x7fffffffu)
+    float ev0 = vb0 == 255u ? __uint_as_float(0x7fffffffu)
                                   : __uint_as_float(0x4b000000u | vb0) - 8388735.0f;   // vb0 - 127
-    const float ev1 = vb1 == 255u ? __uint_as_float(0x7fffffffu)
+    float ev1 = vb1 == 255u ? __uint_as_float(0x7fffffffu)
                                   : __uint_as_float(0x4b000000u | vb1) - 8388735.0f;
     // ---- arguments of the exponentials, against the running maxima
     float ap[NT][4], aw[NT][4];
@@ -615,6 +615,18 @@ quant_decode_kernel(const __grid_constant__ CUtensorMap tm_rows,
       }
     }
     if (__any_sync(0xffffffffu, over > kSlack || over_w > kSlack + kUp)) {
+      // a row of zeros moves no maximum, whatever its scale: rows that nothing was stored
+      // to have the scale 1 (four lanes look at a row; no cost where no maximum moves)
+      auto zero_row = [&](int row) {
+        const uint4 x = lds128(vb + sw128(row, 2 * qd)), y = lds128(vb + sw128(row, 2 * qd + 1));
+        uint32_t any = (x.x | x.y | x.z | x.w | y.x | y.y | y.z | y.w) & (kInt8 ? ~0u : 0x7f7f7f7fu);
+        any |= __shfl_xor_sync(0xffffffffu, any, 1);
+        any |= __shfl_xor_sync(0xffffffffu, any, 2);
+        return any == 0;
+      };
+      const bool zero0 = zero_row(r), zero1 = zero_row(r + 8);
+      if (zero0 && vb0 != 255u) ev0 = -126.f;
+      if (zero1 && vb1 != 255u) ev1 = -126.f;
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
 #pragma unroll
