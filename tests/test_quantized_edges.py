@@ -55,3 +55,15 @@ def test_prefill_workspace_is_bounded_however_large_the_batch(size, Hq, Hkv, new
         for batch in (9, 257):
             need = f(batch * new, seqs, Hq, Hkv, 128, new, 1 << 16)
             assert need == f(seqs * new, seqs, Hq, Hkv, 128, new, 1 << 16) <= most
+
+
+def test_calls_of_another_torch_are_neither_loaded_nor_kept(monkeypatch):
+    """The compiled calls hold what they were built for: another torch or Python refuses
+    them, and the build makes them again."""
+    from vllm_b200 import _native, build
+    assert _native.load_calls().target == _native.calls_target()
+    assert _native.calls_match()
+    monkeypatch.setattr(_native, "calls_target", lambda: "vllm_b200 calls for torch 9.9, cpython-399;")
+    assert build._calls_stale()
+    with pytest.raises(RuntimeError, match="torch 9.9"):
+        _native.load_calls()

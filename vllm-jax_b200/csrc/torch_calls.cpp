@@ -584,4 +584,12 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_torch_calls", nullptr, -1, method
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__torch_calls() { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__torch_calls() {
+  PyObject *const m = PyModule_Create(&module);
+  // read from the file before it is loaded, too
+  if (m && PyModule_AddStringConstant(m, "target", VJ_CALLS_TARGET) < 0) {
+    Py_DECREF(m);
+    return nullptr;
+  }
+  return m;
+}

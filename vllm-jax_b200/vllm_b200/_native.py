@@ -9,6 +9,7 @@ import ctypes
 import importlib.machinery
 import importlib.util
 import os
+import sys
 import threading
 from pathlib import Path
 
@@ -196,10 +197,25 @@ def load() -> ctypes.CDLL:
     return _lib
 
 
+def calls_target() -> str:
+    """What csrc/torch_calls.cpp is compiled for, and holds: this torch and this Python."""
+    import torch
+    return f"vllm_b200 calls for torch {torch.__version__}, {sys.implementation.cache_tag};"
+
+
+def calls_match() -> bool:
+    """Whether the compiled calls were built for this torch and this Python (read, not loaded:
+    their binary interfaces differ)."""
+    return calls_target().encode() in _CALLS_PATH.read_bytes()
+
+
 def load_calls():
     """The compiled calls of the quantised cache (csrc/torch_calls.cpp), not bound yet."""
     if not _CALLS_PATH.exists():
         raise RuntimeError(f"{_CALLS_PATH} not found: build it with `python -m vllm_b200.build`")
+    if not calls_match():
+        raise RuntimeError(f"{_CALLS_PATH} was built for another torch or Python than "
+                           f"{calls_target()!r}: build it again with `python -m vllm_b200.build`")
     loader = importlib.machinery.ExtensionFileLoader("vllm_b200._torch_calls", str(_CALLS_PATH))
     spec = importlib.util.spec_from_loader(loader.name, loader)
     module = importlib.util.module_from_spec(spec)

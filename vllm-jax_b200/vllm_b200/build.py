@@ -20,6 +20,8 @@ import sys
 import sysconfig
 from pathlib import Path
 
+from . import _native
+
 PKG_DIR = Path(__file__).resolve().parent
 CSRC = PKG_DIR.parent / "csrc"
 INCLUDE = PKG_DIR.parent.parent / "include"
@@ -62,6 +64,14 @@ def _compile(src: Path, obj: Path, ptxas_v: bool) -> str:
     return r.stderr
 
 
+def _calls_stale() -> bool:
+    """Whether _torch_calls.so is missing, older than its sources, or another torch's or
+    Python's."""
+    newest = max(p.stat().st_mtime for p in (CALLS_SRC, INCLUDE / "vjattn.h"))
+    return (not CALLS_PATH.exists() or CALLS_PATH.stat().st_mtime < newest
+            or not _native.calls_match())
+
+
 def _build_calls() -> None:
     import torch
     root = Path(torch.__file__).resolve().parent
@@ -74,6 +84,7 @@ def _build_calls() -> None:
     tmp = CALLS_PATH.with_suffix(".so.tmp")
     cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-shared",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+           f'-DVJ_CALLS_TARGET="{_native.calls_target()}"',
            *(f"-I{i}" for i in inc), str(CALLS_SRC), "-o", str(tmp), f"-L{root / 'lib'}",
            "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
     r = subprocess.run(cmd, capture_output=True, text=True)
@@ -94,10 +105,7 @@ def build(force: bool = False, ptxas_v: bool = False, verbose: bool = False) -> 
                  or obj.stat().st_mtime < max(src.stat().st_mtime, hdr_t))
         if stale:
             jobs.append((src, obj))
-    header = INCLUDE / "vjattn.h"
-    stale_calls = (force or not CALLS_PATH.exists()
-                   or CALLS_PATH.stat().st_mtime < max(CALLS_SRC.stat().st_mtime,
-                                                       header.stat().st_mtime))
+    stale_calls = force or _calls_stale()
     with cf.ThreadPoolExecutor(max_workers=8) as ex:
         calls = ex.submit(_build_calls) if stale_calls else None
         if jobs:
