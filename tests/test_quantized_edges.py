@@ -67,3 +67,32 @@ def test_calls_of_another_torch_are_neither_loaded_nor_kept(monkeypatch):
     assert build._calls_stale()
     with pytest.raises(RuntimeError, match="torch 9.9"):
         _native.load_calls()
+
+
+@pytest.mark.parametrize("seqs,hkv,ctx", [(1, 8, 100), (256, 8, 16384), (4, 1, 300), (2, 8, 300_000)])
+def test_pool_leaves_room_for_the_prefill_scratch(seqs, hkv, ctx):
+    """A gpu_memory_utilization that leaves a bf16 engine enough leaves a quantised one as
+    much beside its prefill's scratch, which is what the wrapper and the C entries ask for."""
+    from vllm_b200 import Config, _native
+    from vllm_b200.kernels.quantized_cache import PREFILL_SCRATCH_ROWS, prefill_scratch_bytes
+    from vllm_b200.model.qwen3 import Qwen3Config
+    from vllm_b200.src import model_runner as mr
+    mcfg = Qwen3Config(num_attention_heads=4 * hkv, num_key_value_heads=hkv)
+    base = dict(model="tiny", max_num_batched_tokens=8192, max_num_seqs=seqs, num_blocks=0,
+                block_size=16, max_model_len=ctx, compat=False, gpu_memory_utilization=0.9)
+    free = 150 << 30
+    bf16, e4m3 = Config(**base), Config(**base, kv_cache_dtype="e4m3")
+    assert mr.kv_cache_num_blocks(free, bf16, mcfg, 1) == \
+        int(free * 0.9) // mr.kv_cache_bytes_per_block(mcfg, 16, 1)
+    n = mr.kv_cache_num_blocks(free, e4m3, mcfg, 1)
+    taken = n * mr.kv_cache_bytes_per_block(mcfg, 16, 1, "e4m3")
+    held = -(-ctx // 16) * 16                       # what a sequence's block table holds
+    padded = -(-held // 128) * 128
+    groups = -(-seqs // min(seqs, max(1, PREFILL_SCRATCH_ROWS // (padded * hkv))))
+    group = -(-seqs // groups)
+    needs = 2 * group * padded * hkv * 128 * 2 + max(
+        _native.load().vj_paged_prefill_split_workspace_size(8192, s, 4 * hkv, hkv, 128, new, padded)
+        for s in (group, max(group - 1, 1)) for new in (1, 33, 64, 100, 300))
+    assert needs <= prefill_scratch_bytes(seqs, hkv, held)
+    assert taken + prefill_scratch_bytes(seqs, hkv, held) <= int(free * 0.9)
+    assert mr.kv_cache_num_blocks(1 << 20, e4m3, mcfg, 1) == 0

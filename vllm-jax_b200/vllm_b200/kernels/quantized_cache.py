@@ -133,6 +133,16 @@ def read_kv_cache(cache: QuantizedKVCache, block_tables: torch.Tensor,
 PREFILL_SCRATCH_ROWS = 1 << 21
 
 
+def prefill_scratch_bytes(num_seqs: int, num_kv_heads: int, max_context_len: int,
+                          head_dim: int = 128) -> int:
+    """A bound on the memory that a paged_prefill_quantized call of up to num_seqs
+    sequences allocates beside its output: the contexts read back (whole key tiles of
+    128), and the parts of split keys (256 rows a CTA at most, one CTA an SM of 148)."""
+    rows = -(-max_context_len // 128) * 128 * num_kv_heads
+    rows = min(num_seqs * rows, max(PREFILL_SCRATCH_ROWS, rows))
+    return rows * 2 * head_dim * 2 + 148 * 256 * (head_dim + 2) * 4
+
+
 def paged_prefill_quantized(q: torch.Tensor, cache: QuantizedKVCache, block_tables: torch.Tensor,
                             cu_seqlens_q: torch.Tensor, context_lens: torch.Tensor | None = None,
                             max_seqlen_q: int = 0, scale: float | None = None,

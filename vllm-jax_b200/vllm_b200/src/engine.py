@@ -25,7 +25,7 @@ from ..config import Config
 from ..model.qwen3 import Qwen3Config, Qwen3Weights, get_config
 from ..sampling_params import SamplingParams
 from .kv_cache_manager import KVCacheManager
-from .model_runner import ModelRunner, check_kv_cache_dtype, kv_cache_bytes_per_block
+from .model_runner import ModelRunner, check_kv_cache_dtype, kv_cache_num_blocks
 from .request import Request
 from .scheduler import ChunkedScheduler, Scheduler
 
@@ -84,9 +84,7 @@ class Engine:
         num_blocks = config.num_blocks
         if num_blocks <= 0:
             free, _ = torch.cuda.mem_get_info(device)
-            per = kv_cache_bytes_per_block(self.mcfg, config.block_size, self.tp_size,
-                                           config.kv_cache_dtype)
-            num_blocks = int(free * config.gpu_memory_utilization) // per
+            num_blocks = kv_cache_num_blocks(free, config, self.mcfg, self.tp_size)
             if self.tp_size > 1:   # every rank must agree on the pool size
                 t = torch.tensor([num_blocks], device=device)
                 torch.distributed.all_reduce(t, op=torch.distributed.ReduceOp.MIN,

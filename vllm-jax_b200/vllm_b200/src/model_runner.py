@@ -23,7 +23,7 @@ from ..kernels.decode_paged_attention import decode_workspace_bytes
 from ..kernels.kv_store import rope_table
 from ..kernels.metadata import DecodeMeta, DeviceTables, bucket_size
 from ..kernels.quantized_cache import (CACHE_DTYPES, QuantizedKVCache,
-                                       decode_quantized_workspace_bytes)
+                                       decode_quantized_workspace_bytes, prefill_scratch_bytes)
 from ..kernels.sampler import sample
 from ..model.qwen3 import Qwen3Config, Qwen3Model, Qwen3Weights
 from .kv_cache_manager import KVCacheManager
@@ -35,6 +35,18 @@ def kv_cache_bytes_per_block(mcfg: Qwen3Config, block_size: int, tp_size: int,
     row = mcfg.head_dim * 2 if kv_cache_dtype == "bf16" else mcfg.head_dim + 1   # and its scale
     return (mcfg.num_hidden_layers * 2 * block_size * (mcfg.num_key_value_heads // tp_size)
             * row)
+
+
+def kv_cache_num_blocks(free: int, config: Config, mcfg: Qwen3Config, tp_size: int) -> int:
+    """Blocks of the pool, of `free` bytes of the device's memory: gpu_memory_utilization of
+    them, less what a prefill over a quantised pool allocates (a bf16 pool is read in place)."""
+    room = int(free * config.gpu_memory_utilization)
+    if config.kv_cache_dtype != "bf16":
+        room -= prefill_scratch_bytes(min(config.max_num_seqs, config.max_num_batched_tokens),
+                                      mcfg.num_key_value_heads // tp_size,
+                                      config.max_blocks_per_seq * config.block_size, mcfg.head_dim)
+    return max(room, 0) // kv_cache_bytes_per_block(mcfg, config.block_size, tp_size,
+                                                    config.kv_cache_dtype)
 
 
 def check_kv_cache_dtype(config: Config) -> None:
