@@ -96,3 +96,22 @@ def test_pool_leaves_room_for_the_prefill_scratch(seqs, hkv, ctx):
     assert needs <= prefill_scratch_bytes(seqs, hkv, held)
     assert taken + prefill_scratch_bytes(seqs, hkv, held) <= int(free * 0.9)
     assert mr.kv_cache_num_blocks(1 << 20, e4m3, mcfg, 1) == 0
+
+
+def test_bf16_calls_name_the_quantised_ones():
+    import torch
+    from vllm_b200.kernels.decode_paged_attention import decode_paged_attention
+    from vllm_b200.kernels.prefill_paged_attention import prefill_paged_attention
+    q, pages = torch.zeros(2, 4, 128), torch.zeros(2, 3, 16, 128)
+    bt, n = torch.zeros(2, 1, dtype=torch.int32), torch.ones(2, dtype=torch.int32)
+    cu, scales = torch.tensor([0, 1, 2], dtype=torch.int32), torch.zeros(2, 3, 16)
+    for kw in (dict(k_scales_pages=scales), dict(v_scales_pages=scales)):
+        with pytest.raises(NotImplementedError, match="paged_decode_quantized"):
+            decode_paged_attention(q, pages, pages, bt, n, **kw)
+        with pytest.raises(NotImplementedError, match="paged_prefill_quantized"):
+            prefill_paged_attention(q, pages, pages, bt, cu, n, n, max_seqlen_bucket=1, **kw)
+    with pytest.raises(NotImplementedError, match="soft-cap"):
+        decode_paged_attention(q, pages, pages, bt, n, attn_logits_soft_cap=30.0)
+    with pytest.raises(NotImplementedError, match="soft-cap"):
+        prefill_paged_attention(q, pages, pages, bt, cu, n, n, max_seqlen_bucket=1,
+                                attn_logits_soft_cap=30.0)

@@ -79,8 +79,11 @@ def decode_paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
         raise ValueError(f"The dtype of `lengths` must be int32. Got {lengths.dtype}")
     if block_h % 16:
         raise ValueError(f"block_h must divisible by 16, but is {block_h}.")
-    if k_scales_pages is not None or v_scales_pages is not None or attn_logits_soft_cap is not None:
-        raise NotImplementedError("quantized pages and logit soft-cap are not implemented")
+    if k_scales_pages is not None or v_scales_pages is not None:
+        raise NotImplementedError("quantized pages are not implemented here: use "
+                                  "kernels.quantized_cache.paged_decode_quantized")
+    if attn_logits_soft_cap is not None:
+        raise NotImplementedError("logit soft-cap is not implemented")
     if interpret:
         raise NotImplementedError("interpret=True (CPU) is not available: the B200 path has no "
                                   "CPU fallback")

@@ -88,8 +88,11 @@ def prefill_paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: tor
         raise ValueError("cu_seqlens must have shape [batch + 1]")
     if block_tables.dtype != torch.int32:
         raise ValueError("block_tables must be int32")
-    if k_scales_pages is not None or v_scales_pages is not None or attn_logits_soft_cap is not None:
-        raise NotImplementedError("quantized pages and logit soft-cap are not implemented")
+    if k_scales_pages is not None or v_scales_pages is not None:
+        raise NotImplementedError("quantized pages are not implemented here: use "
+                                  "kernels.quantized_cache.paged_prefill_quantized")
+    if attn_logits_soft_cap is not None:
+        raise NotImplementedError("logit soft-cap is not implemented")
     if interpret:
         raise NotImplementedError("interpret=True (CPU) is not available: the B200 path has no "
                                   "CPU fallback")
