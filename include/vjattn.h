@@ -216,7 +216,7 @@ VJ_API vj_status vj_paged_decode_noalloc(
  *
  *   q [num_tokens, Hq, D] bf16 packed; sequence s owns rows
  *   [cu_seqlens_q[s], cu_seqlens_q[s+1]); out has the same shape, rows past
- *   cu_seqlens_q[num_seqs] are written as 0
+ *   cu_seqlens_q[num_seqs] are written as 0; both 16-byte aligned
  *   context_lens [num_seqs] int32 = cached prefix + new tokens (keys already
  *   in the pool), or NULL when keys == new tokens (the reference's case)
  *   new token i of sequence s sits at position context_len - n_s + i and

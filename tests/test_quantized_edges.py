@@ -22,6 +22,29 @@ PREFILLS = [_prefill, _split("vj_paged_prefill_split"), _split("vj_paged_prefill
 ROWS = 4 * 8 * 128 * 2        # bytes of q, and of out
 
 
+def _bf16_prefill(lib, **kw):
+    a = dict(q=16, k=16, v=16, bt=16, cu=16, ctx=16, out=16, T=4, S=1, Hq=8, Hkv=2, D=128, nb=200,
+             bs=16, w=200, bts=200, sb=4096, st=256, sh=128, mq=4, scale=0.1, err=16, stream=None)
+    return lib.vj_paged_prefill(*{**a, **kw}.values())
+
+
+def _mixed(lib, **kw):
+    a = dict(q=16, k=16, v=16, bt=16, cu=16, ctx=16, out=16, T=4, S=2, nd=1, Hq=8, Hkv=2, D=128,
+             nb=200, bs=16, w=200, bts=200, sb=4096, st=256, sh=128, mq=4, scale=0.1, mc=0, plan=1,
+             ws=None, wsb=0, err=16, stream=None)
+    return lib.vj_paged_attention_mixed(*{**a, **kw}.values())
+
+
+@pytest.mark.parametrize("entry", PREFILLS + [_bf16_prefill, _mixed])
+@pytest.mark.parametrize("kw", [dict(out=16 + 8), dict(out=1 << 20 | 2), dict(q=1 << 20 | 8)])
+def test_prefill_refuses_rows_off_16_byte_boundaries(entry, kw):
+    """Rows are written 16 bytes at a time: elsewhere that is a fault on the GPU."""
+    from vllm_b200 import _native
+    lib = _native.load()
+    assert entry(lib, **kw) == _native.VJ_ERR_INVALID_ARGUMENT
+    assert b"aligned" in lib.vj_get_last_error()
+
+
 @pytest.mark.parametrize("entry", PREFILLS)
 @pytest.mark.parametrize("kw,overlaps", [
     (dict(out=32), True), (dict(q=32), True), (dict(out=16 + ROWS - 16), True),

@@ -628,6 +628,9 @@ int prefill_setup(const std::string &what, const void *q, const void *k_cache, c
       (num_seqs > 0 && !block_tables && !in_order)) {
     return set_error(VJ_ERR_INVALID_ARGUMENT, what + ": null pointer");
   }
+  if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) % 16 != 0) {
+    return set_error(VJ_ERR_INVALID_ARGUMENT, what + ": q and out must be 16-byte aligned");
+  }
   PrefillArgs &a = *args;
   a.out = static_cast<__nv_bfloat16 *>(out);
   a.bt = block_tables;
@@ -897,6 +900,10 @@ extern "C" vj_status vj_paged_attention_mixed(
   if (!q || !k_cache || !v_cache || !block_tables || !cu_seqlens_q || !context_lens || !out ||
       !error_flag) {
     return set_error(VJ_ERR_INVALID_ARGUMENT, "vj_paged_attention_mixed: null pointer");
+  }
+  if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) % 16 != 0) {
+    return set_error(VJ_ERR_INVALID_ARGUMENT,
+                     "vj_paged_attention_mixed: q and out must be 16-byte aligned");
   }
   if (max_chunks <= 0) max_chunks = 4096 + num_decode;
   if (num_decode > 0) {
