@@ -529,7 +529,9 @@ VJ_API vj_status vj_paged_prefill_split_part(
  * its magnitude and eps (q of vj_kv_store_qknorm_rope is rounded to bf16 after
  * every step as the reference does, so the two differ by roundings). Tokens whose slot lies outside [0, num_blocks*block_size) store
  * nothing (their q is still written). Slots that are stored must differ from
- * each other within a call. q_out may equal q_in with the same row stride.
+ * each other within a call. q_out may equal q_in with the same row stride;
+ * otherwise its rows must not overlap those of q_in, k_in and v_in (they may be
+ * other columns of the same rows).
  *   q_out [T,Hq,D] with row stride q_out_row_stride (0: packed); num_q_heads
  *   may be 0 (q_in, q_out unused). Other flags are rejected.
  *   error_flag: device int32 (may be NULL), set to 1 if a wait timed out */

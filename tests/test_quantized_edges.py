@@ -138,3 +138,30 @@ def test_bf16_calls_name_the_quantised_ones():
     with pytest.raises(NotImplementedError, match="soft-cap"):
         prefill_paged_attention(q, pages, pages, bt, cu, n, n, max_seqlen_bucket=1,
                                 attn_logits_soft_cap=30.0)
+
+
+def _store(lib, **kw):
+    """Five tokens of 4/2 heads, q, k and v side by side in rows of 8 heads from 1 << 20 on."""
+    at = 1 << 20
+    a = dict(q=at, k=at + 4 * 256, v=at + 6 * 256, qw=16, kw=16, pos=16, slots=16, qo=1 << 24, kc=16,
+             vc=16, ks=16, vs=16, dt=1, T=5, Hq=4, Hkv=2, D=128, nb=4, bs=16, sb=4096, st=256, sh=128,
+             cb=32, ch=16, qrs=1024, krs=1024, vrs=1024, qors=1024, tab=None, tl=0, eps=1e-6, th=1e6,
+             fl=3, err=None, stream=None)
+    return lib.vj_kv_store_quantized(*{**a, **kw}.values())
+
+
+@pytest.mark.parametrize("kw", [
+    dict(qo=1 << 20, qors=512),                            # packed, over rows that are not
+    dict(qo=(1 << 20) + 256),                              # a head further on, into k
+    dict(qo=(1 << 20) - 256),                              # a head back, into v of the row before
+    dict(qo=(1 << 20) + 1024),                             # k's and v's place
+    dict(qo=(1 << 20) + 2048 * 2 + 512),                   # two rows on
+    dict(qo=(1 << 20) + 256, T=1, qrs=0, krs=0, vrs=0),
+    dict(k=1 << 24),
+    dict(v=(1 << 24) + 2048 * 4),
+])
+def test_store_refuses_an_output_that_lies_across_its_inputs(kw):
+    from vllm_b200 import _native
+    lib = _native.load()
+    assert _store(lib, **kw) == _native.VJ_ERR_INVALID_ARGUMENT
+    assert b"overlap" in lib.vj_get_last_error()

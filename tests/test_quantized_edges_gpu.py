@@ -199,6 +199,36 @@ def test_stored_k_rows_of_every_magnitude_are_correctly_rounded(dtype, eps):
         np.testing.assert_array_equal(got[0], new[i][0], err_msg="elements of " + "kv"[i])
 
 
+@pytest.mark.parametrize("T", [1, 33])
+def test_store_in_place_and_next_to_its_inputs(T):
+    """q_out as q's own columns of one projection's output, and as columns of the same rows
+    that nothing else takes."""
+    from vllm_b200.kernels.quantized_cache import QuantizedKVCache, kv_store_quantized
+    rng = np.random.default_rng(33)
+    x = _t(bf16(rng.standard_normal((T, 4 + 2 + 2 + 4, D))))
+    w, pos, slots = _t(np.ones(D)), _i(np.arange(T)), _i(np.arange(T) + 5)
+
+    def call(y, out):
+        cache = QuantizedKVCache.zeros(4, 16, 2, device="cuda")
+        q = kv_store_quantized(y[:, :4], y[:, 4:6], y[:, 6:8], cache, slots, pos, w, w, q_out=out)
+        return q, cache.data.view(torch.uint8), cache.scales
+
+    ref = call(x, None)
+    for columns in (slice(0, 4), slice(8, 12)):
+        y = x.clone()
+        for a, b in zip(call(y, y[:, columns]), ref):
+            assert torch.equal(a, b)
+        keep = [i for i in range(12) if i not in range(*columns.indices(12))]
+        assert torch.equal(y[:, keep], x[:, keep])
+    if T > 1:
+        y = x.clone()
+        for columns in (slice(1, 5), slice(3, 7), slice(5, 9)):
+            with pytest.raises(ValueError, match="overlap"):
+                call(y, y[:, columns])
+        torch.cuda.synchronize()
+        assert torch.equal(y, x)
+
+
 # ----------------------------------------------------------------------------- decode
 @pytest.mark.parametrize("dtype", ["e4m3", "int8"])
 def test_rows_that_nothing_stored_count_as_zeros(dtype):

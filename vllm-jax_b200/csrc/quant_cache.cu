@@ -465,6 +465,22 @@ kv_store_quantized_kernel(const StoreArgs a) {
   }
 }
 
+// Whether T rows of `out` (out_w elements, out_s from one to the next) may share memory with
+// those of x: not where the one is the other (a unit reads its rows before it writes them),
+// nor where they are separate columns of one buffer's rows.
+bool rows_overlap(const void *out, int64_t out_w, int64_t out_s, const void *x, int64_t x_w,
+                  int64_t x_s, int64_t T, bool may_be_same) {
+  const auto o = reinterpret_cast<uintptr_t>(out), p = reinterpret_cast<uintptr_t>(x);
+  const uint64_t out_bytes = ((T - 1) * out_s + out_w) * 2, x_bytes = ((T - 1) * x_s + x_w) * 2;
+  if (o < p ? p - o >= out_bytes : o - p >= x_bytes) return false;
+  if (T == 1) return !(may_be_same && o == p);
+  if (out_s != x_s || (o - p) % 2 != 0) return true;
+  if (o == p) return !may_be_same;
+  int64_t column = (static_cast<int64_t>(o - p) / 2) % x_s;       // of out in x's rows
+  if (column < 0) column += x_s;
+  return column < x_w || column + out_w > x_s;
+}
+
 template <bool kInt8>
 int launch_store(const StoreArgs &a, unsigned grid, cudaStream_t stream) {
   // the shared-memory opt-in is a per-device attribute of the kernel
@@ -636,6 +652,15 @@ extern "C" vj_status vj_kv_store_quantized(
     return set_error(VJ_ERR_INVALID_ARGUMENT,
                      std::string(what) + ": q/k/v rows and weights must start on 16-byte "
                                          "boundaries");
+  }
+  if (num_q_heads > 0) {
+    const int64_t qw = static_cast<int64_t>(num_q_heads) * kD, kw = static_cast<int64_t>(num_kv_heads) * kD;
+    if (rows_overlap(q_out, qw, a.qors, q_in, qw, a.qrs, num_tokens, true) ||
+        rows_overlap(q_out, qw, a.qors, k_in, kw, a.krs, num_tokens, false) ||
+        rows_overlap(q_out, qw, a.qors, v_in, kw, a.vrs, num_tokens, false)) {
+      return set_error(VJ_ERR_INVALID_ARGUMENT,
+                       std::string(what) + ": q_out must be q (with its row stride) or not overlap q, k, v");
+    }
   }
   a.q = static_cast<const __nv_bfloat16 *>(q_in);
   a.k = static_cast<const __nv_bfloat16 *>(k_in);

@@ -90,7 +90,8 @@ def kv_store_quantized(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor,
     The arguments are kv_store_qknorm_rope's. q is rounded to bf16 once, k and
     v to 8 bits once (kv_store_qknorm_rope rounds after every step, as the
     reference does). Slots outside the pool store nothing (there is no wrap of
-    negative ones); the others must differ from each other within a call."""
+    negative ones); the others must differ from each other within a call. q_out may
+    be q, or must not overlap q, k and v."""
     return (_calls or _bound()).kv_store(q, k, v, cache, slot_mapping, positions, q_norm_weight,
                                          k_norm_weight, eps, rope_theta, norm, rope, q_out, table)
 
