@@ -954,7 +954,8 @@ def run_e2e(args, rank, world, local_rank):
                    max_num_seqs=cfg["max_num_seqs"], num_blocks=0, block_size=16,
                    tensor_parallel_size=tp, gpu_memory_utilization=0.9,
                    max_model_len=((max_len + 15) // 16) * 16, compat=False,
-                   enable_chunked_prefill=c5, fused_gemm_max_rows=args.fused_gemm)
+                   enable_chunked_prefill=c5, fused_gemm_max_rows=args.fused_gemm,
+                   kv_cache_dtype=args.kv_cache_dtype)
 
     def progress(msg):
         print(f"[rank {rank}] {msg}", file=sys.stderr, flush=True)
@@ -1009,7 +1010,8 @@ def run_e2e(args, rank, world, local_rank):
     # per decode step, over the CUDA-event time of the decode forwards
     wbytes = sum(p.numel() * 2 for lw in eng.weights.layers for p in
                  (lw.w_qkv, lw.w_o, lw.w_gate_up, lw.w_down)) + eng.weights.lm_head.numel() * 2
-    kvb = mcfg.num_hidden_layers * 2 * (mcfg.num_key_value_heads // tp) * mcfg.head_dim * 2
+    row = mcfg.head_dim * 2 if args.kv_cache_dtype == "bf16" else mcfg.head_dim + 1
+    kvb = mcfg.num_hidden_layers * 2 * (mcfg.num_key_value_heads // tp) * row
     dec_steps = sum(st["decode_steps"] for st in stats)
     dec_ctx = sum(st["decode_ctx_tokens"] for st in stats)
     achieved = (dec_steps * wbytes + dec_ctx * kvb) / max(dec_s, 1e-9) / 1e9
@@ -1066,6 +1068,8 @@ def run_e2e(args, rank, world, local_rank):
         "gpu_launches": launches,
         "clocks": clk.summary(),
     }
+    if args.kv_cache_dtype != "bf16":
+        line["config"]["kv_cache_dtype"] = args.kv_cache_dtype
     if cpu is not None:
         line["cpu_baseline"] = cpu
     print(json.dumps(line), flush=True)
@@ -1438,6 +1442,8 @@ def main():
     ap.add_argument("--fused-gemm", type=int, default=0,
                     help="e2e/c5/c4step: forwards of at most this many rows run their "
                          "projections on the fused tcgen05 GEMMs (0: cuBLAS)")
+    ap.add_argument("--kv-cache-dtype", default="bf16", choices=["bf16", "e4m3", "int8"],
+                    help="e2e/c5: elements of the engine's KV cache")
     ap.add_argument("--gemm-op", default="all", choices=["all", "qkv", "o_proj", "gate_up", "down"],
                     help="gemm: time one projection only (profiling)")
     ap.add_argument("--new-tokens", type=int, default=None,
