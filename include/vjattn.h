@@ -510,8 +510,8 @@ VJ_API vj_status vj_paged_prefill_split_part(
  * is the smallest power of two that brings the row's largest magnitude to at
  * most 448 (e4m3) or 127 (int8), never below 2^-126 (a row of zeros has that
  * one); a row holding an infinity or NaN has byte 255 and zero elements, and
- * reads as NaN everywhere. No element is e4m3's NaN. A power of two times an element is a bf16 number,
- * so reading the cache back rounds nothing.
+ * reads as NaN everywhere. No element is e4m3's NaN. A power of two times an
+ * element is a bf16 number, so reading the cache back rounds nothing.
  *
  *   elements: (blk,t,h,d) at base + blk*stride_block + t*stride_token +
  *   h*stride_head + d, strides multiples of 16, base 16-byte aligned
@@ -586,10 +586,13 @@ VJ_API vj_status vj_paged_decode_quantized(
 /* Causal attention of few new tokens over the quantised cache, straight from its
  * pages: q, out, cu_seqlens_q, context_lens (new tokens included; not NULL),
  * max_seqlen_q as in vj_paged_prefill, the cache as above. Rows of out behind
- * cu_seqlens_q[num_seqs] are zeroed; out may be q, or must not overlap it. The keys of a row tile (128 rows of tokens x
- * query heads of one KV head) are split over CTAs that would be idle. Where there
- * are many row tiles, vj_kv_read_quantized (zero_to = 128, max_len a multiple of
- * 128) and vj_paged_prefill_split on what it leaves are faster.
+ * cu_seqlens_q[num_seqs] are zeroed; out may be q, or must not overlap it; both
+ * are 16-byte aligned. A row of byte 255 makes NaN of every new token of its
+ * sequence that sees it, and may of others that share its 128 keys. The keys of
+ * a row tile (128 rows of tokens x query heads of one KV head) are split over
+ * CTAs that would be idle. Where there are many row tiles, vj_kv_read_quantized
+ * (zero_to = 128, max_len a multiple of 128) and vj_paged_prefill_split on what
+ * it leaves are faster.
  *   max_context_len: a bound on context_lens, which with max_seqlen_q, the batch
  *   and the heads decides how far is split
  *   workspace: vj_paged_prefill_quantized_workspace_size(...) bytes on the current

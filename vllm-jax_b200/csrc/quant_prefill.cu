@@ -19,6 +19,9 @@
 // row took 2.1 us a key tile, since one warp is then all that a quarter of the SM has
 // for it. Pages travel two tiles ahead through shared memory (loads held in registers
 // one tile ahead: 2.1 us; four warps for K and V together: 2.5).
+// The weights enter their product rounded to bf16 (half a step: 2^-8 of each), since its
+// two operands have one type and V's rows, element times scale, need bf16's range; their
+// sum, which divides them, and all outputs up to the last rounding are in 32 bits.
 // S(j+1) is computed while the softmax of S(j) runs; O is rescaled only where a row's
 // maximum grows by more than 2^8, and then behind PV(j - 1).
 // Latency-bound: a few key tiles a CTA, each load -> convert -> scores -> softmax ->

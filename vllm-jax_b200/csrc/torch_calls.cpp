@@ -135,7 +135,8 @@ int32_t *error_flag(int index) {
   return p;
 }
 
-// A C entry without the interpreter's lock; counts its launches, raises its errors.
+// A C entry without the interpreter's lock; counts the launches of its longest form (as
+// _native.call does), raises its errors.
 template <typename F>
 void enter(int launches, F &&entry) {
   int status;

@@ -236,7 +236,9 @@ def check(status: int) -> None:
         raise VJError(status, msg)
 
 
-# kernels launched by one successful call of each entry point
+# Kernels that one successful call of each entry point counts: those of its longest form.
+# (An empty batch launches none of them, and a quantised decode whose units take whole
+# sequences leaves out the second, so launch_count is a bound where such calls are made.)
 KERNELS_PER_CALL = {"vj_paged_decode": 3, "vj_paged_decode_planned": 2,
                     "vj_paged_decode_noalloc": 3, "vj_paged_prefill": 2,
                     "vj_paged_attention_mixed": 3, "vj_paged_decode_quantized": 2}
