@@ -509,7 +509,7 @@ VJ_API vj_status vj_paged_prefill_split_part(
  * and one scale byte; it stands for element * 2^(byte - 127) (E8M0). The scale
  * is the smallest power of two that brings the row's largest magnitude to at
  * most 448 (e4m3) or 127 (int8), never below 2^-126 (a row of zeros has that
- * one); a row holding an infinity or NaN has byte 255 and zero elements, and
+ * one, or byte 127 where nothing was stored); a row holding an infinity or NaN has byte 255 and zero elements, and
  * reads as NaN everywhere. No element is e4m3's NaN. A power of two times an
  * element is a bf16 number, so reading the cache back rounds nothing.
  *

@@ -102,6 +102,27 @@ def test_prefill_in_the_queries_place(Hq, Hkv, new, prefix, groups, launches, mo
 
 
 
+def test_prefill_groups_in_the_queries_place_in_a_graph(monkeypatch):
+    """Captured with groups of one sequence, replayed on other queries next to eager calls on
+    another stream."""
+    from vllm_b200.kernels import quantized_cache as qc
+    monkeypatch.setattr(qc, "PREFILL_SCRATCH_ROWS", 1)
+    case = _Prompts(32, 8, (300, 0, 280), (1400, 30, 1100))
+    queries = [case.q, _t(bf16(np.random.default_rng(3).standard_normal(case.q_np.shape)))]
+    refs = [case.call(q) for q in queries]
+    live, graph, side = queries[0].clone(), torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph):
+        case.call(live, out=live)
+    for i in (1, 0, 1):
+        live.copy_(queries[i])
+        torch.cuda.synchronize()
+        graph.replay()
+        with torch.cuda.stream(side):
+            beside = case.call(queries[1 - i])
+        torch.cuda.synchronize()
+        assert torch.equal(live, refs[i]) and torch.equal(beside, refs[1 - i])
+
+
 @pytest.mark.parametrize("Hq,Hkv,new,prefix", [(8, 2, (20, 60), (0, 30)),
                                                (32, 8, (900, 1000), (0, 100))])
 def test_prefill_refuses_an_output_that_lies_across_the_queries(Hq, Hkv, new, prefix):
@@ -231,21 +252,28 @@ def test_store_in_place_and_next_to_its_inputs(T):
 
 # ----------------------------------------------------------------------------- decode
 @pytest.mark.parametrize("dtype", ["e4m3", "int8"])
-def test_rows_that_nothing_stored_count_as_zeros(dtype):
+@pytest.mark.parametrize("n,Hq", [(40, 8), (40, 32), (3000, 2), (3000, 32)])
+def test_rows_that_nothing_stored_count_as_zeros(n, Hq, dtype):
     """Rows of a fresh pool inside a context, next to values of 1e-6: their scales must not
-    outweigh the others'."""
+    outweigh the others'. Whole pages of them too, and a row of NaN in another sequence."""
     from vllm_b200.kernels.quantized_cache import (QuantizedKVCache, kv_store_quantized,
                                                    paged_decode_quantized)
     rng = np.random.default_rng(32)
-    cache = QuantizedKVCache.zeros(4, 16, 2, dtype=dtype, device="cuda")
-    n = 40
+    nb = -(-n // 16) + 1
+    cache = QuantizedKVCache.zeros(nb + 1, 16, 2, dtype=dtype, device="cuda")
+    cache.scales[:, nb] = 255
     slots = np.arange(n)
-    slots[[3, 20, 39]] = -1
+    missing = [3, 20, n - 1] + list(range(0 if n < 99 else 700, 0 if n < 99 else 760))
+    slots[missing] = -1
     k, v = bf16(rng.standard_normal((n, 2, D))), bf16(1e-6 * rng.standard_normal((n, 2, D)))
     kv_store_quantized(None, _t(k), _t(v), cache, _i(slots), norm=False, rope=False)
-    q = bf16(rng.standard_normal((1, 8, D)))
-    out = paged_decode_quantized(_t(q), cache, _i([[0, 1, 2, 3]]), _i([n]))
+    q = bf16(rng.standard_normal((1, Hq, D)))
+    bt = np.full((2, nb), nb)
+    bt[0] = np.arange(nb)
+    out = paged_decode_quantized(_t(np.concatenate([q, q])), cache, _i(bt), _i([n, 5]))
+    assert torch.isnan(out[1]).all()
+    out = out[:1]
     codes, scales = cache.data.view(torch.uint8).cpu().numpy(), cache.scales.cpu().numpy()
-    vals = [oq.gather(oq.dequantise(codes[i], scales[i], dtype), np.arange(4), n) for i in range(2)]
-    assert not vals[1][[3, 20, 39]].any() and vals[1][4].any()
+    vals = [oq.gather(oq.dequantise(codes[i], scales[i], dtype), np.arange(nb), n) for i in range(2)]
+    assert not vals[1][missing].any() and vals[1][4].any()
     _check(out, *oq.attend(q.astype(np.float64), *vals, n - 1, 1 / math.sqrt(D)), DECODE)
